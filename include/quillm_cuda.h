@@ -37,7 +37,13 @@ enum {
 };
 
 /* tensor dtypes: the .qlm / qm_dtype values (src/qm_base.h:11-15) */
-enum { QMC_F32 = 0, QMC_F16 = 1 /* KV cache only */, QMC_Q8_0 = 2, QMC_Q4_0 = 3 };
+enum {
+    QMC_F32 = 0,
+    QMC_F16 = 1, /* KV cache and the batched-decoding operators only */
+    QMC_Q8_0 = 2,
+    QMC_Q4_0 = 3,
+    QMC_BF16 = 4, /* batched-decoding operators only */
+};
 
 const char *qmc_last_error(void);
 int qmc_device_count(int *count);
@@ -211,6 +217,117 @@ int qmc_sampler_free(qmc_sampler *s);
 /* one decode step for (token, pos) whose next token is drawn by the sampler on the device: only the
  * 4-byte token comes back (qm_model_forward + qm_sample of src/main.c without the logits copy) */
 int qmc_model_forward_sample(qmc_model *m, int32_t token, int32_t pos, qmc_sampler *s, int32_t *next_token);
+
+/* ---- operators of batched decoding over a paged KV cache (no counterpart in the reference) ----
+ * A batch of sequences (samples or beams) behind one prompt: rows of queries, keys and values are normalised
+ * and rotated, appended to pages, each sequence's token attends to the shared prefix and to its own pages, and
+ * beams are selected and their pages reordered.
+ *
+ * Common to all of them: pointers are device memory of the current device unless said otherwise; rows are
+ * `ld` elements apart (ld >= the row's elements) and a row's heads follow one another; `dtype` is the rows'
+ * QMC_F32, QMC_F16 or QMC_BF16; sums, softmax statistics and norms are float (log-sum-exp of a vocabulary:
+ * double) and every output is rounded once.  No call allocates or synchronises and each may be captured in a
+ * CUDA graph; a workspace belongs to one call at a time (two calls, or two graphs, whose executions may
+ * overlap need one each) and needs no initial contents.  Index errors that only the device can see (a
+ * page outside the pool, a position past the page table) skip the access and set the device error word:
+ * the next qmc_check_device_error() / qmc_sync() returns QMC_EINVAL.  Outputs must not overlap inputs, other
+ * than where a call allows it. */
+
+/* rotary positions: pair i of the first rot_dim dimensions of a head turns by pos * f_i radians, with
+ * f_i = theta^(-2 i / rot_dim) before scaling; the other dimensions stay.  Angles are formed in double, so
+ * far positions lose nothing. */
+enum { QMC_ROPE_INTERLEAVED = 0 /* pair (2i, 2i + 1), as qmc_rope */, QMC_ROPE_HALF = 1 /* pair (i, i + rot_dim / 2) */ };
+enum {
+    QMC_ROPE_PLAIN = 0,
+    QMC_ROPE_LINEAR = 1, /* f_i / factor */
+    QMC_ROPE_BANDS = 2,  /* with t = orig_ctx f_i / 2 pi (turns within the original context): f_i for t > high,
+                            f_i / factor for t < low, between them the mix f_i s + f_i / factor (1 - s) with
+                            s = (t - low) / (high - low) */
+    QMC_ROPE_YARN = 3,   /* f_i / factor r + f_i (1 - r) with r rising from 0 to 1 between the pair indices
+                            floor(d(high)) and ceil(d(low)), d(t) = rot_dim ln(orig_ctx / (2 pi t)) / (2 ln theta),
+                            clamped to [0, rot_dim - 1]; cos and sin times 0.1 ln(factor) + 1 */
+};
+typedef struct {
+    int32_t head_dim, rot_dim; /* even; 2 <= rot_dim <= head_dim <= 256 */
+    int32_t layout, scaling;
+    double theta, factor; /* > 0 (YARN: theta != 1); factor is read by the three scaled forms */
+    double low, high;     /* BANDS: 0 < low < high; YARN: turns 0 < low <= high */
+    int32_t orig_ctx;     /* BANDS, YARN: > 0 */
+} qmc_rope_config;
+/* a plan is host memory only: it may be used on any device, by any number of threads and calls */
+typedef struct qmc_rope_plan qmc_rope_plan;
+int qmc_rope_plan_create(const qmc_rope_config *cfg, qmc_rope_plan **out);
+int qmc_rope_plan_free(qmc_rope_plan *p);
+
+/* norms of queries and keys for each head and the rotation, in one pass over the rows:
+ *   y = x / sqrt(mean(x^2) + eps) * weight (per head; weight[head_dim] floats, NULL: y = x), then rotated at
+ *   positions[row] (int32, any sign).
+ * q rows hold n_heads heads, k rows n_kv_heads; either may be NULL with 0 heads.  q_out may be q itself with the same
+ * ld, and k_out k (in place).  q and k may be columns of one packed row. */
+int qmc_qk_norm_rope(const qmc_rope_plan *plan, int dtype, const void *q, int64_t ldq, void *q_out, int64_t ldqo,
+                     int32_t n_heads, const void *k, int64_t ldk, void *k_out, int64_t ldko, int32_t n_kv_heads,
+                     const float *q_weight, const float *k_weight, float eps, const int32_t *positions, int64_t rows,
+                     void *stream);
+
+/* a paged cache: k and v are pools [n_layers][n_pages][page_size][n_kv_heads][head_dim] of dtype (QMC_F32,
+ * QMC_F16 or QMC_BF16).  Position p of a sequence is slot p % page_size of page table[p / page_size].  The
+ * struct is the caller's, read during the call only. */
+typedef struct {
+    void *k, *v;
+    int32_t dtype, n_layers, n_pages, page_size, n_kv_heads, head_dim;
+} qmc_paged_cache;
+
+/* the rows' keys (normalised and rotated as by qmc_qk_norm_rope) and values into their slots of `layer`, each rounded
+ * once to the cache's dtype, and the rotated queries to q_out (q NULL: keys and values only; q_out may be q).
+ * Row r belongs to sequence seq[r] (NULL: sequence r) at positions[r]; a row with a negative sequence or
+ * position is padding and writes nothing, its q_out row included.  page_table is int32 [n_seq][ld_table].  No two rows
+ * may name the same slot.  plan NULL: no rotation.  A row whose slot does not exist sets the error word and
+ * writes no key or value. */
+int qmc_kv_append_paged(const qmc_rope_plan *plan, const qmc_paged_cache *cache, int32_t layer, int dtype,
+                        const void *q, int64_t ldq, void *q_out, int64_t ldqo, int32_t n_heads, const void *k,
+                        int64_t ldk, const void *v, int64_t ldv, const float *q_weight, const float *k_weight, float eps,
+                        const int32_t *seq, const int32_t *positions, const int32_t *page_table, int32_t n_seq,
+                        int32_t ld_table, int64_t rows, void *stream);
+
+/* attention of one token per sequence, for sequences that share their first prefix_len positions: row b of
+ * out = for each head softmax(scale q . k_p) v_p over p < seq_lens[b].  Positions p < prefix_len come from
+ * prefix_pages[p / page_size], once for the whole batch, the later ones from page_table[b][p / page_size] (its
+ * entries for whole prefix pages are not read; prefix_len may end inside a page).  seq_lens[b] counts
+ * the prefix too: it is 0 (an empty row: zeros) or at least prefix_len; any other value, a length past
+ * ld_table * page_size, or a page outside the pool sets the error word, and then the rows concerned are undefined (but
+ * written).  n_heads is a multiple of the cache's n_kv_heads (head h reads kv head h / (n_heads / n_kv_heads)),
+ * head_dim <= 256.  Types (rows, cache): (F32, F32), (F32, F16), (F16, F16), (BF16, BF16).  Keys and values
+ * at positions that are read must be finite; what lies in slots past a sequence's end does not matter. */
+int qmc_attn_prefix_workspace(int dtype, const qmc_paged_cache *cache, int32_t n_seq, int32_t n_heads,
+                              int32_t prefix_len, int32_t ld_table, size_t *bytes);
+int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, const void *q, int64_t ldq, void *out,
+                    int64_t ldo, int32_t n_heads, int32_t n_seq, float scale, const int32_t *prefix_pages,
+                    int32_t prefix_len, const int32_t *page_table, int32_t ld_table, const int32_t *seq_lens,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* beam search's selection: for each prompt the n_out best of its beams x n_vocab continuations by
+ *   score(b, v) = scores[b] + logits[b][v] - log sum_w exp(logits[b][w])
+ * in falling order, ties to the lower b * n_vocab + v: parents (beam within the prompt), tokens and float scores, each
+ * [n_prompts][n_out].  logits is [n_prompts * beams][ld].  A finished beam (finished[row] != 0; NULL: none)
+ * offers one continuation, eos_token at its score unchanged; all its others, those of a beam whose score is
+ * -inf or NaN, and tokens whose logit is -inf or NaN, score -inf.  Where a row holds +inf, its infinities share the
+ * probability.  beams <= 64, n_out <= min(64, beams * n_vocab). */
+int qmc_beam_workspace(int32_t n_prompts, int32_t beams, int32_t n_vocab, int32_t n_out, size_t *bytes);
+int qmc_beam_select(int dtype, const void *logits, int64_t ld, int32_t n_prompts, int32_t beams, int32_t n_vocab,
+                    const float *scores, const uint8_t *finished, int32_t eos_token, int32_t n_out, int32_t *parents,
+                    int32_t *tokens, float *out_scores, void *workspace, size_t workspace_bytes, void *stream);
+
+/* reordering of the beams' states: beam j of a prompt becomes a child of beam parents[j] (parents is
+ * [n_prompts][ld_parents], the first `beams` of a row are read).  All beams of a prompt have the length
+ * seq_lens[prompt * beams] = n; the page being filled is entry n / page_size of a table row and belongs to that
+ * beam alone.  page_table_out (not page_table) receives: the parent's entries below that one; at it the
+ * parent's page for the parent's first child, and for each further child, in order, the page of a beam
+ * without children, in order, into which the n % page_size filled slots of every layer are copied; and beyond
+ * it beam j's own entries.  With n % page_size == 0 nothing is copied, and an entry n / page_size past the table
+ * is left out. */
+int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t beams, const int32_t *parents,
+                     int32_t ld_parents, const int32_t *seq_lens, const int32_t *page_table, int32_t *page_table_out,
+                     int32_t ld_table, void *stream);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus

@@ -17,7 +17,10 @@ LIBDIR = os.path.join(HERE, "lib")
 CUDA_LIB = os.path.join(LIBDIR, "libquillm_cuda.so")
 HOST_LIB = os.path.join(LIBDIR, "libquillm.so")
 
-QMC_F32, QMC_F16, QMC_Q8_0, QMC_Q4_0 = 0, 1, 2, 3  # QMC_F16: KV cache only
+# QMC_F16: KV cache and batched-decoding operators; QMC_BF16: batched-decoding operators
+QMC_F32, QMC_F16, QMC_Q8_0, QMC_Q4_0, QMC_BF16 = 0, 1, 2, 3, 4
+QMC_ROPE_INTERLEAVED, QMC_ROPE_HALF = 0, 1
+QMC_ROPE_PLAIN, QMC_ROPE_LINEAR, QMC_ROPE_BANDS, QMC_ROPE_YARN = range(4)
 (QMC_T_TOK_EMBD, QMC_T_NORM, QMC_T_OUTPUT, QMC_T_ATTN_NORM, QMC_T_WQ, QMC_T_WK, QMC_T_WV, QMC_T_WO,
  QMC_T_FFN_NORM, QMC_T_W1, QMC_T_W2, QMC_T_W3) = range(12)
 STATUS = {0: "ok", -1: "invalid argument", -2: "cuda error", -3: "out of memory", -4: "nccl error",
@@ -32,6 +35,17 @@ class QmcConfig(C.Structure):
     _fields_ = [("dim", C.c_int32), ("hidden_dim", C.c_int32), ("n_layers", C.c_int32), ("n_heads", C.c_int32),
                 ("n_kv_heads", C.c_int32), ("vocab_size", C.c_int32), ("max_seq", C.c_int32),
                 ("rope_theta", C.c_float), ("norm_eps", C.c_float)]
+
+
+class QmcRopeConfig(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32),
+                ("theta", C.c_double), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double),
+                ("orig_ctx", C.c_int32)]
+
+
+class QmcPagedCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_layers", C.c_int32),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
 
 
 class QmTensor(C.Structure):  # include/ops.h qm_tensor
@@ -116,6 +130,15 @@ _CUDA_SIGS = {
     "qmc_sampler_rng": (I, [V, P]),
     "qmc_sampler_free": (I, [V]),
     "qmc_model_forward_sample": (I, [V, I32, I32, V, P]),
+    "qmc_rope_plan_create": (I, [C.POINTER(QmcRopeConfig), P]),
+    "qmc_rope_plan_free": (I, [V]),
+    "qmc_qk_norm_rope": (I, [V, I, P, I64, P, I64, I32, P, I64, P, I64, I32, P, P, F, P, I64, V]),
+    "qmc_kv_append_paged": (I, [V, P, I32, I, P, I64, P, I64, I32, P, I64, P, I64, P, P, F, P, P, P, I32, I32, I64, V]),
+    "qmc_attn_prefix_workspace": (I, [I, P, I32, I32, I32, I32, C.POINTER(S)]),
+    "qmc_attn_prefix": (I, [P, I32, I, P, I64, P, I64, I32, I32, F, P, I32, P, I32, P, P, S, V]),
+    "qmc_beam_workspace": (I, [I32, I32, I32, I32, C.POINTER(S)]),
+    "qmc_beam_select": (I, [I, P, I64, I32, I32, I32, P, P, I32, I32, P, P, P, P, S, V]),
+    "qmc_beam_reorder": (I, [P, I32, I32, P, I32, P, P, P, I32, V]),
 }
 
 _HOST_SIGS = {
@@ -233,6 +256,62 @@ class Sampler:
         if self.h:
             self.lib.qmc_sampler_free(self.h)
             self.h = C.c_void_p()
+
+
+def torch_stream() -> int:
+    """torch's current stream as a stream argument: NULL would mean the library's own stream, so torch's
+    default stream is passed as the runtime's handle of the legacy default stream (cudaStreamLegacy)"""
+    import torch
+
+    return torch.cuda.current_stream().cuda_stream or 1
+
+
+class RopePlan:
+    """rotary positions of heads of `head_dim` (qmc_rope_plan): the first `rot_dim` dimensions, in a layout
+    (QMC_ROPE_INTERLEAVED / QMC_ROPE_HALF), scaled by one of QMC_ROPE_PLAIN / LINEAR / BANDS / YARN; `h` is the handle"""
+
+    def __init__(self, head_dim: int, rot_dim: int = 0, layout: int = QMC_ROPE_INTERLEAVED, theta: float = 10000.0,
+                 scaling: int = QMC_ROPE_PLAIN, factor: float = 1.0, low: float = 0.0, high: float = 0.0, orig_ctx: int = 0):
+        self.lib = cuda()
+        self.h = C.c_void_p()
+        cfg = QmcRopeConfig(head_dim, rot_dim or head_dim, layout, scaling, theta, factor, low, high, orig_ctx)
+        check(self.lib.qmc_rope_plan_create(C.byref(cfg), C.byref(self.h)), "rope_plan_create")
+
+    def close(self) -> None:
+        if self.h:
+            self.lib.qmc_rope_plan_free(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedCache:
+    """a qmc_paged_cache over two device pools [n_layers][n_pages][page_size][n_kv_heads][head_dim], which it keeps alive;
+    `ref` is the pointer the operators take"""
+
+    def __init__(self, k, v, dtype: int, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int):
+        self.k, self.v = k, v
+        self.c = QmcPagedCache(ptr(k), ptr(v), dtype, n_layers, n_pages, page_size, n_kv_heads, head_dim)
+        self.ref = C.addressof(self.c)
+
+
+def attn_prefix_workspace(dtype: int, cache: PagedCache, n_seq: int, n_heads: int, prefix_len: int, ld_table: int) -> int:
+    """workspace bytes of qmc_attn_prefix on the current device"""
+    n = C.c_size_t(0)
+    check(cuda().qmc_attn_prefix_workspace(dtype, cache.ref, n_seq, n_heads, prefix_len, ld_table, C.byref(n)),
+          "attn_prefix_workspace")
+    return n.value
+
+
+def beam_workspace(n_prompts: int, beams: int, n_vocab: int, n_out: int) -> int:
+    """workspace bytes of qmc_beam_select"""
+    n = C.c_size_t(0)
+    check(cuda().qmc_beam_workspace(n_prompts, beams, n_vocab, n_out, C.byref(n)), "beam_workspace")
+    return n.value
 
 
 class Model:

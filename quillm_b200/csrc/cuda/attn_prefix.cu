@@ -1,0 +1,346 @@
+// Attention of one token per sequence over a shared prefix and own pages (qmc_attn_prefix).
+//
+// For row (b, head): o = sum_p e^(s_p - M) v_p / sum_p e^(s_p - M), s_p = scale q . k_p, over the prefix's positions
+// and the sequence's own.  The prefix's keys and values are the same for every sequence, so its part is one
+// product of all batch * group query rows of a KV head with them: a block takes a tile of those rows and a range
+// of positions, and the prefix is read once per row tile, not once per sequence.  Own positions are read once per (sequence, KV
+// head), shared by the group's heads.  Both kinds of work are jobs of one launch; each leaves its rows' running
+// maximum m, sum l and unnormalised o in the workspace, and a second launch joins the parts of every row:
+// o = sum_j e^(m_j - M) o_j / sum_j e^(m_j - M) l_j.
+#include <algorithm>
+
+#include "batch.cuh"
+
+namespace qmc {
+namespace {
+
+struct Plan {
+    int rows;                 // query rows of a KV head over the whole batch: n_seq * group
+    int ptiles, psplit;       // prefix: row tiles and position ranges
+    int gtiles, osplit;       // own positions: row tiles of a group and position ranges
+    int64_t ml_bytes, bytes;  // workspace: [parts][n_seq * n_heads] float2 (m, l), then [parts][...][hd] floats
+};
+
+struct AttnArgs {
+    const void *q, *kc, *vc;  // kc, vc: the layer's pools
+    void *out;
+    int64_t ldq, ldo;
+    const int *prefix_pages, *table, *lens;
+    int *err;
+    float2 *ml;
+    float *po;
+    int n_seq, heads, kv, group, hd, page_size, n_pages, ld_table, prefix;
+    int rows, ptiles, psplit, gtiles, osplit;
+    float scale;
+};
+
+constexpr int kQR = 16;  // query rows per block (4 per warp)
+constexpr int kPT = 32;  // positions per staged tile (one per lane)
+
+// the part of one job: rows [r0, r0 + nr) of KV head h, positions [p0, p1), and where its results go
+struct Job {
+    int h, r0, nr, p0, p1, part, b;  // b: the sequence of an own job, -1 for the prefix
+};
+
+__device__ __forceinline__ int own_len(const AttnArgs &a, int b) {
+    const int n = a.lens[b];
+    return min(max(n - a.prefix, 0), a.ld_table * a.page_size - a.prefix);
+}
+
+// jobs: prefix [h][tile][split], then own [b][h][group tile][split]
+__device__ __forceinline__ Job job_of(const AttnArgs &a, int64_t i, int tile, int quantum) {
+    Job j;
+    const int64_t np = (int64_t)a.kv * a.ptiles * a.psplit;
+    if (i < np) {
+        const int sp = (int)(i % a.psplit), t = (int)(i / a.psplit % a.ptiles);
+        j.h = (int)(i / a.psplit / a.ptiles);
+        j.r0 = t * tile, j.nr = min(tile, a.rows - j.r0);
+        const int64_t chunk = (((int64_t)a.prefix + a.psplit - 1) / a.psplit + quantum - 1) / quantum * quantum;
+        j.p0 = (int)min((int64_t)a.prefix, sp * chunk), j.p1 = (int)min((int64_t)a.prefix, j.p0 + chunk);
+        j.part = sp, j.b = -1;
+        return j;
+    }
+    i -= np;
+    const int sp = (int)(i % a.osplit), t = (int)(i / a.osplit % a.gtiles);
+    j.h = (int)(i / a.osplit / a.gtiles % a.kv);
+    j.b = (int)(i / a.osplit / a.gtiles / a.kv);
+    j.r0 = j.b * a.group + t * tile, j.nr = min(tile, a.group - t * tile);
+    const int64_t n = own_len(a, j.b), chunk = ((n + a.osplit - 1) / a.osplit + quantum - 1) / quantum * quantum;
+    j.p0 = a.prefix + (int)min(n, sp * chunk), j.p1 = a.prefix + (int)min(n, sp * chunk + chunk);
+    j.part = a.psplit + sp;
+    return j;
+}
+
+// slot of position p, -1 (and the error word) for a page outside the pool
+__device__ __forceinline__ int64_t slot_of(const AttnArgs &a, int b, int p) {
+    const int e = p / a.page_size, page = b < 0 ? a.prefix_pages[e] : a.table[(int64_t)b * a.ld_table + e];
+    if (page < 0 || page >= a.n_pages) {
+        raise_error(a.err, kErrBadIndex);
+        return -1;
+    }
+    return (int64_t)page * a.page_size + p % a.page_size;
+}
+
+// row r of a KV head: sequence r / group, query head h * group + r % group; its place among all batch * heads rows
+__device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
+    return (int64_t)(r / a.group) * a.heads + h * a.group + r % a.group;
+}
+
+// The general kernel, in float on the CUDA cores: any head_dim up to 256, any types, strides and alignments.  Per row and tile of
+// 32 positions lane p scores position p, the warp updates the row's maximum and sum once, and each lane
+// accumulates four of the head's dimensions (eight above 128).
+template <typename T, typename CT, int NG>
+__global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool vec) {
+    extern __shared__ __align__(16) float smf[];
+    const int hd = a.hd, hd4 = (hd + 3) & ~3;
+    float *Kt = smf;               // [hd4 / 4][kPT][4]
+    float *Vs = Kt + hd4 * kPT;    // [kPT][hd4]
+    float *Qs = Vs + kPT * hd4;    // [kQR][hd4]
+    __shared__ int64_t slot_s[kPT];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Job jb = job_of(a, blockIdx.x, kQR, kPT);
+    for (int i = tid; i < kQR * hd4; i += 128) {
+        const int r = i / hd4, d = i % hd4, rr = jb.r0 + r;
+        Qs[i] = (r < jb.nr && d < hd)
+                    ? to_f32(((const T *)a.q)[(rr / a.group) * a.ldq + (int64_t)(jb.h * a.group + rr % a.group) * hd + d])
+                    : 0.0f;
+    }
+    constexpr int TW = kQR / 4;
+    float m[TW], l[TW], o[TW][NG][4];
+#pragma unroll
+    for (int j = 0; j < TW; j++) {
+        m[j] = -INFINITY, l[j] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[j][g][i] = 0.0f;
+    }
+    const CT *kc = (const CT *)a.kc, *vc = (const CT *)a.vc;
+    for (int p0 = jb.p0; p0 < jb.p1; p0 += kPT) {
+        __syncthreads();  // the previous tile is no longer read
+        if (tid < kPT) slot_s[tid] = p0 + tid < jb.p1 ? slot_of(a, jb.b, p0 + tid) : -1;
+        __syncthreads();
+        for (int i = tid; i < kPT * (hd4 / 4); i += 128) {  // positions vary fastest: conflict-free transposed stores
+            const int pp = i % kPT, c = i / kPT;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (slot_s[pp] >= 0) {
+                const CT *p = kc + (slot_s[pp] * a.kv + jb.h) * hd + 4 * c;
+                if (vec) load_chunk<CT, 4>(p, v);
+                else
+                    for (int k = 0; k < 4; k++) v[k] = 4 * c + k < hd ? to_f32(p[k]) : 0.0f;
+            }
+            *(float4 *)(Kt + (c * kPT + pp) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        for (int i = tid; i < kPT * (hd4 / 4); i += 128) {
+            const int c = i % (hd4 / 4), pp = i / (hd4 / 4);
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (slot_s[pp] >= 0) {
+                const CT *p = vc + (slot_s[pp] * a.kv + jb.h) * hd + 4 * c;
+                if (vec) load_chunk<CT, 4>(p, v);
+                else
+                    for (int k = 0; k < 4; k++) v[k] = 4 * c + k < hd ? to_f32(p[k]) : 0.0f;
+            }
+            *(float4 *)(Vs + pp * hd4 + 4 * c) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TW; j++) {
+            const int r = warp * TW + j;
+            if (r >= jb.nr) break;
+            const float *q = Qs + r * hd4;
+            float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 0; c < hd4 / 4; c++) {
+                const float4 k4 = *(const float4 *)(Kt + (c * kPT + lane) * 4), q4 = *(const float4 *)(q + 4 * c);
+                s4[0] = fmaf(q4.x, k4.x, s4[0]), s4[1] = fmaf(q4.y, k4.y, s4[1]);
+                s4[2] = fmaf(q4.z, k4.z, s4[2]), s4[3] = fmaf(q4.w, k4.w, s4[3]);
+            }
+            const float sc = p0 + lane < jb.p1 ? ((s4[0] + s4[1]) + (s4[2] + s4[3])) * a.scale : -INFINITY;
+            const float mn = fmaxf(m[j], warp_max(sc));
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            const float corr = expf(m[j] - ref), e = expf(sc - ref);
+            l[j] = l[j] * corr + warp_sum(e);
+            m[j] = mn;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[j][g][i] *= corr;
+            for (int pp = 0; pp < kPT; pp++) {
+                const float ep = __shfl_sync(0xffffffffu, e, pp);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    if (128 * g + 4 * lane < hd4) {
+                        const float4 v4 = *(const float4 *)(Vs + pp * hd4 + 128 * g + 4 * lane);
+                        o[j][g][0] = fmaf(ep, v4.x, o[j][g][0]), o[j][g][1] = fmaf(ep, v4.y, o[j][g][1]);
+                        o[j][g][2] = fmaf(ep, v4.z, o[j][g][2]), o[j][g][3] = fmaf(ep, v4.w, o[j][g][3]);
+                    }
+                }
+            }
+        }
+    }
+    const int64_t all = (int64_t)a.n_seq * a.heads;
+#pragma unroll
+    for (int j = 0; j < TW; j++) {
+        const int r = warp * TW + j;
+        if (r >= jb.nr) break;
+        const int64_t at = jb.part * all + out_row(a, jb.h, jb.r0 + r);
+        if (lane == 0) a.ml[at] = make_float2(m[j], l[j]);
+        if (l[j] == 0.0f) continue;  // the join skips it
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = 128 * g + 4 * lane + i;
+                if (d < hd) a.po[at * hd + d] = o[j][g][i];
+            }
+    }
+}
+
+// joins the parts of a row, one warp each
+template <typename T>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int parts) {
+    const int lane = threadIdx.x & 31;
+    const int64_t all = (int64_t)a.n_seq * a.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= all) return;
+    const int b = (int)(row / a.heads), h = (int)(row % a.heads), n = a.lens[b];
+    if (lane == 0 && ((n != 0 && n < a.prefix) || n > (int64_t)a.ld_table * a.page_size)) raise_error(a.err, kErrBadIndex);
+    float M = -INFINITY;
+    if (n > 0)
+        for (int j = lane; j < parts; j += 32) M = fmaxf(M, a.ml[j * all + row].x);
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;  // dimension lane + 32 i
+    if (n > 0)
+        for (int j = 0; j < parts; j++) {
+            const float2 ml = a.ml[j * all + row];
+            if (ml.y == 0.0f) continue;
+            const float w = expf(ml.x - ref);
+            l = fmaf(w, ml.y, l);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (lane + 32 * i < a.hd) o[i] = fmaf(w, a.po[(j * all + row) * a.hd + lane + 32 * i], o[i]);
+        }
+    const float rl = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);  // an empty row gives zeros
+    T *out = (T *)a.out + b * a.ldo + (int64_t)h * a.hd;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (lane + 32 * i < a.hd) from_f32(o[i] * rl, &out[lane + 32 * i]);
+}
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+Plan plan_for(const qmc_paged_cache *c, int n_seq, int n_heads, int prefix, int ld_table, int sms) {
+    Plan p{};
+    const int group = n_heads / c->n_kv_heads;
+    const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix), want = 4 * sms;
+    p.rows = n_seq * group;
+    p.ptiles = ceil_div(p.rows, kQR);
+    p.gtiles = ceil_div(group, kQR);
+    p.psplit = prefix ? (int)std::min<int64_t>(ceil_div(want, (int64_t)c->n_kv_heads * p.ptiles), ceil_div(prefix, 2 * kPT)) : 0;
+    p.osplit = own ? (int)std::min<int64_t>(ceil_div(want, (int64_t)n_seq * c->n_kv_heads * p.gtiles), ceil_div(own, 2 * kPT)) : 0;
+    const int64_t parts = p.psplit + p.osplit, all = (int64_t)n_seq * n_heads;
+    p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;
+    p.bytes = p.ml_bytes + parts * all * c->head_dim * 4 + 256;
+    return p;
+}
+
+template <typename T, typename CT, int NG>
+int launch_rows(const AttnArgs &a, int64_t jobs, bool vec, cudaStream_t s) {
+    const int hd4 = (a.hd + 3) & ~3;
+    auto fn = attn_rows_kernel<T, CT, NG>;
+    const int smem = (2 * kPT + kQR) * hd4 * 4;
+    QMC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * kPT + kQR) * 256 * 4));
+    fn<<<(unsigned)jobs, 128, smem, s>>>(a, vec);
+    QMC_LAUNCH_CHECK();
+    return QMC_OK;
+}
+
+template <typename T, typename CT>
+int launch_attn(const AttnArgs &a, cudaStream_t s) {
+    const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
+    if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
+    if (jobs) {
+        const size_t al = 4 * sizeof(CT);
+        const bool vec = a.hd % 4 == 0 && (uintptr_t)a.kc % al == 0 && (uintptr_t)a.vc % al == 0;
+        const int rc = a.hd <= 128 ? launch_rows<T, CT, 1>(a, jobs, vec, s) : launch_rows<T, CT, 2>(a, jobs, vec, s);
+        if (rc) return rc;
+    }
+    const int64_t all = (int64_t)a.n_seq * a.heads;
+    attn_join_kernel<T><<<(unsigned)((all + 3) / 4), 128, 0, s>>>(a, a.psplit + a.osplit);
+    QMC_LAUNCH_CHECK();
+    return QMC_OK;
+}
+
+int check_attn(const char *op, int dtype, const qmc_paged_cache *c, int n_seq, int n_heads, int prefix, int ld_table) {
+    if (const int rc = check_cache(c, op)) return rc;
+    const bool ok = (dtype == QMC_F32 && (c->dtype == QMC_F32 || c->dtype == QMC_F16)) ||
+                    (dtype == c->dtype && (dtype == QMC_F16 || dtype == QMC_BF16));
+    if (!ok) return set_error(QMC_EINVAL, "%s: rows of dtype %d over a cache of dtype %d", op, dtype, c->dtype);
+    if (c->head_dim > 256) return set_error(QMC_EINVAL, "%s: head_dim %d is above 256", op, c->head_dim);
+    if (n_seq < 0 || n_heads < 1 || n_heads % c->n_kv_heads || prefix < 0 || ld_table < 1)
+        return set_error(QMC_EINVAL, "%s: %d sequences, %d heads over %d, prefix %d, table %d wide", op, n_seq, n_heads,
+                         c->n_kv_heads, prefix, ld_table);
+    if ((int64_t)ld_table * c->page_size > INT32_MAX || (int64_t)n_seq * n_heads > INT32_MAX)
+        return set_error(QMC_EINVAL, "%s: more than 2^31 - 1 positions or rows", op);
+    if (prefix > (int64_t)ld_table * c->page_size)
+        return set_error(QMC_EINVAL, "%s: prefix of %d past a table of %d pages of %d", op, prefix, ld_table, c->page_size);
+    return QMC_OK;
+}
+
+}  // namespace
+}  // namespace qmc
+
+using namespace qmc;
+
+extern "C" {
+
+int qmc_attn_prefix_workspace(int dtype, const qmc_paged_cache *cache, int32_t n_seq, int32_t n_heads,
+                              int32_t prefix_len, int32_t ld_table, size_t *bytes) {
+    if (!bytes) return set_error(QMC_EINVAL, "attn_prefix_workspace: null argument");
+    *bytes = 0;
+    if (const int rc = check_attn("attn_prefix_workspace", dtype, cache, n_seq, n_heads, prefix_len, ld_table)) return rc;
+    DevCtx *c = ctx();
+    if (!c) return QMC_ECUDA;
+    *bytes = (size_t)plan_for(cache, n_seq, n_heads, prefix_len, ld_table, c->num_sms).bytes;
+    return QMC_OK;
+}
+
+int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, const void *q, int64_t ldq, void *out,
+                    int64_t ldo, int32_t n_heads, int32_t n_seq, float scale, const int32_t *prefix_pages,
+                    int32_t prefix_len, const int32_t *page_table, int32_t ld_table, const int32_t *seq_lens,
+                    void *workspace, size_t workspace_bytes, void *stream) {
+    const char *op = "attn_prefix";
+    if (const int rc = check_attn(op, dtype, cache, n_seq, n_heads, prefix_len, ld_table)) return rc;
+    if (layer < 0 || layer >= cache->n_layers) return set_error(QMC_EINVAL, "%s: layer %d of %d", op, layer, cache->n_layers);
+    const int64_t n = (int64_t)n_heads * cache->head_dim;
+    if (ldq < n || ldo < n || ldq > (int64_t)1 << 40 || ldo > (int64_t)1 << 40)
+        return set_error(QMC_EINVAL, "%s: rows of %lld elements are %lld and %lld apart", op, (long long)n, (long long)ldq, (long long)ldo);
+    if (!(scale == scale) || scale - scale != 0.0f) return set_error(QMC_EINVAL, "%s: scale %g", op, scale);
+    if (n_seq == 0) return QMC_OK;
+    if (!q || !out || !page_table || !seq_lens || !workspace || (prefix_len && !prefix_pages))
+        return set_error(QMC_EINVAL, "%s: null argument", op);
+    if ((uintptr_t)q % dtype_size(dtype) || (uintptr_t)out % dtype_size(dtype))
+        return set_error(QMC_EINVAL, "%s: misaligned q or out", op);
+    DevCtx *c = ctx();
+    if (!c) return QMC_ECUDA;
+    const Plan p = plan_for(cache, n_seq, n_heads, prefix_len, ld_table, c->num_sms);
+    if (workspace_bytes < (size_t)p.bytes)
+        return set_error(QMC_EINVAL, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, (size_t)p.bytes);
+    AttnArgs a{};
+    a.q = q, a.out = out, a.ldq = ldq, a.ldo = ldo;
+    const int64_t off = layer * layer_elems(cache) * dtype_size(cache->dtype);
+    a.kc = (const uint8_t *)cache->k + off, a.vc = (const uint8_t *)cache->v + off;
+    a.prefix_pages = prefix_pages, a.table = page_table, a.lens = seq_lens, a.err = c->err;
+    uint8_t *w = (uint8_t *)(((uintptr_t)workspace + 255) / 256 * 256);
+    a.ml = (float2 *)w, a.po = (float *)(w + p.ml_bytes);
+    a.n_seq = n_seq, a.heads = n_heads, a.kv = cache->n_kv_heads, a.group = n_heads / cache->n_kv_heads;
+    a.hd = cache->head_dim, a.page_size = cache->page_size, a.n_pages = cache->n_pages, a.ld_table = ld_table;
+    a.prefix = prefix_len, a.rows = p.rows, a.ptiles = p.ptiles, a.psplit = p.psplit, a.gtiles = p.gtiles, a.osplit = p.osplit;
+    a.scale = scale;
+    cudaStream_t s = pick_stream(stream);
+    if (dtype == QMC_F32 && cache->dtype == QMC_F32) return launch_attn<float, float>(a, s);
+    if (dtype == QMC_F32) return launch_attn<float, __half>(a, s);
+    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, s);
+    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, s);
+}
+
+}  // extern "C"

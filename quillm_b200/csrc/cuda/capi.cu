@@ -170,6 +170,8 @@ int qmc_check_device_error(void) {
         QMC_CUDA(cudaMemset(c_->err, 0, sizeof(int)));
         if (v & kErrBadState)
             return set_error(QMC_EINVAL, "a decode step found its device position or token out of range (code %d)", v);
+        if (v == kErrBadIndex)  // a timeout beside it is what the caller has to know first
+            return set_error(QMC_EINVAL, "a batched-decoding operator met a page, position or index out of range (code %d)", v);
         return set_error(QMC_ETIMEOUT, "a device-side bounded wait expired (code %d)", v);
     }
     return QMC_OK;

@@ -1,0 +1,407 @@
+// Norms of queries and keys per head and the rotary rotation, over rows at positions of their own, into rows or
+// into a paged cache (qmc_qk_norm_rope, qmc_kv_append_paged).
+//
+// For every head x of a row:  y = x / sqrt(mean(x^2) + eps) * w  (optional), then each pair (a, b) of the first
+// rot dimensions becomes (a c - b s, a s + b c) with (c, s) = m (cos, sin)(pos f_i).  The angle is formed in turns in
+// double, t = pos * f_i / 2 pi, reduced by its nearest integer (exact) and only then rounded to float for sincospi: at
+// position 10^6 the product still carries 2^-33 turns, where a float angle would be off by a sixteenth of a radian.
+//
+// HBM bound: each element is read once and written once with ~10 operations between.  A lane group of 1 to 32 lanes
+// holds one head, each lane two chunks of C elements (16 bytes each where the layout allows it) that hold whole
+// pairs between them: in the half layout the chunks at t C and t C + rot / 2, in the interleaved one neighbours.  So a
+// rotation needs no exchange, a norm log2(lanes) shuffles, and every access is a full vector.  A block takes up to
+// 256 threads' worth of one row's heads and forms the row's (c, s) once in shared memory while its loads are in flight.
+#include <cmath>
+#include <new>
+
+#include "batch.cuh"
+
+struct qmc_rope_plan {
+    int head_dim, rot_dim, layout;
+    float mscale;
+    double turns[128];  // f_i / 2 pi
+};
+
+namespace qmc {
+
+int check_cache(const qmc_paged_cache *c, const char *op) {
+    if (!c || !c->k || !c->v) return set_error(QMC_EINVAL, "%s: null cache", op);
+    if (!is_row_dtype(c->dtype)) return set_error(QMC_EINVAL, "%s: bad cache dtype %d", op, c->dtype);
+    if (c->n_layers < 1 || c->n_pages < 1 || c->page_size < 1 || c->n_kv_heads < 1 || c->head_dim < 1)
+        return set_error(QMC_EINVAL, "%s: cache of %d layers, %d pages of %d, %d heads of %d", op, c->n_layers, c->n_pages,
+                         c->page_size, c->n_kv_heads, c->head_dim);
+    const int64_t sz = dtype_size(c->dtype);
+    if ((uintptr_t)c->k % sz || (uintptr_t)c->v % sz) return set_error(QMC_EINVAL, "%s: misaligned cache", op);
+    // slots of a layer are counted in 64 bits, elements of the pool must be too
+    const __int128 n = (__int128)c->n_layers * c->n_pages * c->page_size * c->n_kv_heads * c->head_dim * sz;
+    if (n > ((__int128)1 << 62)) return set_error(QMC_EINVAL, "%s: cache too large", op);
+    return QMC_OK;
+}
+
+namespace {
+
+struct RowsArgs {
+    const void *q, *k, *v;
+    void *qo, *ko;  // rows; ko: keys to rows (no cache)
+    int64_t ldq, ldk, ldv, ldqo, ldko;
+    void *kc, *vc;  // one layer of the pools, or null
+    const int *seq, *pos, *table;
+    const float *qw, *kw;
+    int *err;
+    int n_seq, ld_table, page_size, n_pages;
+    int heads, kv, hd, rot;
+    int shift;      // log2 of a head's lanes
+    bool half, rotate;
+    float eps, mscale;
+};
+struct Turns {
+    double t[128];
+};
+
+// the two chunks of lane item t: offsets ea, eb, the pair index of each chunk's first element, and whether element i
+// of one pairs with element i of the other (else pairs lie inside each chunk)
+template <int C>
+__device__ __forceinline__ void item_offsets(int t, bool half, int rot, int &ea, int &eb, int &pa, int &pb, bool &across,
+                                             bool &turn) {
+    if (half) {
+        const int P = (rot >> 1) / C;
+        turn = t < P;
+        across = true;
+        ea = turn ? t * C : rot + 2 * (t - P) * C;
+        eb = turn ? ea + (rot >> 1) : ea + C;
+        pa = pb = turn ? t * C : 0;
+    } else {
+        ea = 2 * t * C, eb = ea + C;
+        across = C == 1;
+        turn = true;  // pairs past rot / 2 hold (1, 0)
+        pa = ea >> 1, pb = eb >> 1;
+    }
+}
+
+// T rows, CT cache elements, C elements per chunk, NIT items per lane
+template <typename T, typename CT, int C, int NIT>
+__global__ void __launch_bounds__(256) rope_rows_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Turns f) {
+    __shared__ __align__(16) float2 cs[128];
+    __shared__ __align__(16) float w_s[2][256];
+    __shared__ int64_t slot_s;
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lph = 1 << a.shift, li = tid & (lph - 1), hd = a.hd;
+    const int head = (int)blockIdx.y * ((int)blockDim.x >> a.shift) + (tid >> a.shift);
+    const bool cache = a.kc != nullptr;
+    const int n_heads = a.heads + a.kv + (cache ? a.kv : 0);
+    const int kind = head < a.heads ? 0 : head < a.heads + a.kv ? 1 : 2;  // q, k, v
+    const bool live = head < n_heads;
+    const int h = kind == 0 ? head : kind == 1 ? head - a.heads : head - a.heads - a.kv;
+
+    const T *src = nullptr;
+    if (live)
+        src = (kind == 0 ? (const T *)a.q + row * a.ldq : kind == 1 ? (const T *)a.k + row * a.ldk : (const T *)a.v + row * a.ldv) +
+              (int64_t)h * hd;
+    float xa[NIT][C], xb[NIT][C];
+#pragma unroll
+    for (int j = 0; j < NIT; j++) {
+        int ea, eb, pa, pb;
+        bool across, turn;
+        item_offsets<C>(li + j * lph, a.half, a.rot, ea, eb, pa, pb, across, turn);
+#pragma unroll
+        for (int i = 0; i < C; i++) xa[j][i] = xb[j][i] = 0.0f;
+        if (live && ea < hd) load_chunk<T, C>(src + ea, xa[j]);
+        if (live && eb < hd) load_chunk<T, C>(src + eb, xb[j]);
+    }
+    const int pos = a.pos[row];
+    for (int i = tid; i < hd >> 1; i += blockDim.x) {
+        float s = 0.0f, c = 1.0f;
+        if (a.rotate && 2 * i < a.rot) {
+            const double t = (double)pos * f.t[i];
+            sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+            s *= a.mscale, c *= a.mscale;
+        }
+        cs[i] = make_float2(c, s);
+    }
+    if (a.qw)
+        for (int i = tid; i < hd; i += blockDim.x) w_s[0][i] = a.qw[i];
+    if (a.kw)
+        for (int i = tid; i < hd; i += blockDim.x) w_s[1][i] = a.kw[i];
+    if (cache && tid == (int)blockDim.x - 1) {
+        // -1: no slot; -2: padding
+        const int sq = a.seq ? a.seq[row] : (int)row;
+        int64_t slot = -2;
+        if (sq >= 0 && pos >= 0) {
+            slot = -1;
+            const int e = pos / a.page_size;
+            if (sq < a.n_seq && e < a.ld_table) {
+                const int page = a.table[(int64_t)sq * a.ld_table + e];
+                if (page >= 0 && page < a.n_pages) slot = (int64_t)page * a.page_size + pos % a.page_size;
+            }
+            if (slot < 0) raise_error(a.err, kErrBadIndex);
+        }
+        slot_s = slot;
+    }
+    __syncthreads();
+    const int64_t slot = cache ? slot_s : 0;
+    if (slot == -2) return;  // the whole row's blocks
+    const float *w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
+    if (w) {  // the same for a head's lanes; other heads of the warp may differ, so the shuffles are masked to the group
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NIT; j++)
+#pragma unroll
+            for (int i = 0; i < C; i++) ss = fmaf(xa[j][i], xa[j][i], fmaf(xb[j][i], xb[j][i], ss));
+        const unsigned group = (lph == 32 ? 0xffffffffu : ((1u << lph) - 1u)) << ((tid & 31) & ~(lph - 1));
+        for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+        const float r = 1.0f / sqrtf(ss / (float)hd + a.eps);
+        const float *ws = w_s[kind];
+#pragma unroll
+        for (int j = 0; j < NIT; j++) {
+            int ea, eb, pa, pb;
+            bool across, turn;
+            item_offsets<C>(li + j * lph, a.half, a.rot, ea, eb, pa, pb, across, turn);
+#pragma unroll
+            for (int i = 0; i < C; i++) {
+                if (ea < hd) xa[j][i] *= r * ws[ea + i];
+                if (eb < hd) xb[j][i] *= r * ws[eb + i];
+            }
+        }
+    }
+    if (!live || (kind != 0 && slot < 0)) return;
+    T *dst = kind == 0 ? (T *)a.qo + row * a.ldqo + (int64_t)h * hd : (T *)a.ko + (cache ? 0 : row * a.ldko + (int64_t)h * hd);
+    CT *cdst = (kind == 1 ? (CT *)a.kc : (CT *)a.vc) + (cache ? (slot * a.kv + h) * hd : 0);
+#pragma unroll
+    for (int j = 0; j < NIT; j++) {
+        int ea, eb, pa, pb;
+        bool across, turn;
+        item_offsets<C>(li + j * lph, a.half, a.rot, ea, eb, pa, pb, across, turn);
+        if (ea >= hd) continue;
+        if (kind != 2 && turn) {
+            if (across) {
+#pragma unroll
+                for (int i = 0; i < C; i++) {
+                    const float2 r = cs[pa + i];
+                    const float u = xa[j][i], v = xb[j][i];
+                    xa[j][i] = u * r.x - v * r.y;
+                    xb[j][i] = u * r.y + v * r.x;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i + 1 < C; i += 2) {
+                    const float2 r = cs[pa + i / 2];
+                    const float u = xa[j][i], v = xa[j][i + 1];
+                    xa[j][i] = u * r.x - v * r.y;
+                    xa[j][i + 1] = u * r.y + v * r.x;
+                    if (eb < hd) {
+                        const float2 r2 = cs[pb + i / 2];
+                        const float u2 = xb[j][i], v2 = xb[j][i + 1];
+                        xb[j][i] = u2 * r2.x - v2 * r2.y;
+                        xb[j][i + 1] = u2 * r2.y + v2 * r2.x;
+                    }
+                }
+            }
+        }
+        if (kind == 0 || !cache) {
+            store_chunk<T, C>(dst + ea, xa[j]);
+            if (eb < hd) store_chunk<T, C>(dst + eb, xb[j]);
+        } else {
+            store_chunk<CT, C>(cdst + ea, xa[j]);
+            if (eb < hd) store_chunk<CT, C>(cdst + eb, xb[j]);
+        }
+    }
+}
+
+template <typename T, typename CT, int C, int NIT>
+int launch_t(RowsArgs &a, const Turns &f, int64_t rows, cudaStream_t s) {
+    const int P = a.half ? (a.rot >> 1) / C : 0;
+    const int chunks = a.half ? (a.hd - a.rot) / C : a.hd / C;
+    const int items = P + (chunks + 1) / 2;
+    a.shift = 0;
+    while ((NIT << a.shift) < items) a.shift++;
+    const int heads = a.heads + a.kv + (a.kc ? a.kv : 0);
+    const int lanes = heads << a.shift, warps = (lanes + 31) / 32;
+    const int parts = (warps + 7) / 8, wpb = (warps + parts - 1) / parts;  // even blocks of at most 8 warps
+    if (parts > 65535) return set_error(QMC_EINVAL, "rope rows: %d heads are too many", heads);
+    rope_rows_kernel<T, CT, C, NIT><<<dim3((unsigned)rows, parts), wpb * 32, 0, s>>>(a, f);
+    QMC_LAUNCH_CHECK();
+    return QMC_OK;
+}
+
+// the widest chunk that divides the head, the rotated half, the strides and every address; hd <= 256, so a lane needs at most
+// 4 items of one element (128 lanes' worth of pairs), 2 of two and 1 of four or eight
+template <typename T, typename CT>
+int launch_c(RowsArgs &a, const Turns &f, int64_t rows, cudaStream_t s) {
+    constexpr int CM = 16 / sizeof(T);
+    auto fits = [&](int c) {
+        auto addr = [&](const void *p, size_t elem) {
+            const size_t b = c * elem < 16 ? c * elem : 16;
+            return !p || (uintptr_t)p % b == 0;
+        };
+        const int64_t lds[5] = {a.q ? a.ldq : 0, a.k ? a.ldk : 0, a.v ? a.ldv : 0, a.q ? a.ldqo : 0, a.ko ? a.ldko : 0};
+        for (int64_t ld : lds)
+            if (ld % c) return false;
+        return a.hd % c == 0 && (!a.half || (a.rot / 2 % c == 0 && a.rot % c == 0)) && addr(a.q, sizeof(T)) &&
+               addr(a.k, sizeof(T)) && addr(a.v, sizeof(T)) && addr(a.qo, sizeof(T)) && addr(a.ko, sizeof(T)) &&
+               addr(a.kc, sizeof(CT)) && addr(a.vc, sizeof(CT));
+    };
+    if (fits(CM)) return launch_t<T, CT, CM, 1>(a, f, rows, s);
+    if (fits(2)) return launch_t<T, CT, 2, 2>(a, f, rows, s);
+    return launch_t<T, CT, 1, 4>(a, f, rows, s);
+}
+
+template <typename T>
+int launch_ct(RowsArgs &a, const Turns &f, int cdt, int64_t rows, cudaStream_t s) {
+    if (!a.kc) return launch_c<T, T>(a, f, rows, s);
+    if (cdt == QMC_F32) return launch_c<T, float>(a, f, rows, s);
+    if (cdt == QMC_F16) return launch_c<T, __half>(a, f, rows, s);
+    return launch_c<T, __nv_bfloat16>(a, f, rows, s);
+}
+
+int launch_rows(RowsArgs &a, const qmc_rope_plan *p, int dtype, int cdt, int64_t rows, cudaStream_t s) {
+    static const Turns none{};
+    Turns f = none;
+    a.rotate = p != nullptr;
+    a.half = p && p->layout == QMC_ROPE_HALF;
+    a.rot = p ? p->rot_dim : 0;
+    a.mscale = p ? p->mscale : 1.0f;
+    if (p)
+        for (int i = 0; i < p->rot_dim / 2; i++) f.t[i] = p->turns[i];
+    if (dtype == QMC_F32) return launch_ct<float>(a, f, cdt, rows, s);
+    if (dtype == QMC_F16) return launch_ct<__half>(a, f, cdt, rows, s);
+    return launch_ct<__nv_bfloat16>(a, f, cdt, rows, s);
+}
+
+// rows of `n` heads `ld` elements apart
+int check_rows(const char *op, const char *name, const void *p, int64_t ld, int64_t n, int hd, int dtype) {
+    if (!p) return set_error(QMC_EINVAL, "%s: null %s", op, name);
+    if (ld < n * hd) return set_error(QMC_EINVAL, "%s: %s rows of %lld elements are %lld apart", op, name, (long long)(n * hd), (long long)ld);
+    if (ld > (int64_t)1 << 40) return set_error(QMC_EINVAL, "%s: ld of %s too large", op, name);
+    if ((uintptr_t)p % dtype_size(dtype)) return set_error(QMC_EINVAL, "%s: misaligned %s", op, name);
+    return QMC_OK;
+}
+
+}  // namespace
+}  // namespace qmc
+
+using namespace qmc;
+
+extern "C" {
+
+int qmc_rope_plan_create(const qmc_rope_config *c, qmc_rope_plan **out) {
+    if (!c || !out) return set_error(QMC_EINVAL, "rope_plan_create: null argument");
+    *out = nullptr;
+    const int rot = c->rot_dim;
+    if (c->head_dim < 2 || c->head_dim > 256 || (c->head_dim & 1) || rot < 2 || rot > c->head_dim || (rot & 1))
+        return set_error(QMC_EINVAL, "rope_plan_create: head_dim %d, rot_dim %d", c->head_dim, rot);
+    if (c->layout != QMC_ROPE_INTERLEAVED && c->layout != QMC_ROPE_HALF)
+        return set_error(QMC_EINVAL, "rope_plan_create: bad layout %d", c->layout);
+    if (c->scaling < QMC_ROPE_PLAIN || c->scaling > QMC_ROPE_YARN)
+        return set_error(QMC_EINVAL, "rope_plan_create: bad scaling %d", c->scaling);
+    if (!(c->theta > 0) || !std::isfinite(c->theta)) return set_error(QMC_EINVAL, "rope_plan_create: theta %g", c->theta);
+    const bool scaled = c->scaling != QMC_ROPE_PLAIN;
+    if (scaled && (!(c->factor > 0) || !std::isfinite(c->factor)))
+        return set_error(QMC_EINVAL, "rope_plan_create: factor %g", c->factor);
+    if (c->scaling == QMC_ROPE_BANDS && (!(c->low > 0) || !(c->high > c->low) || !std::isfinite(c->high) || c->orig_ctx < 1))
+        return set_error(QMC_EINVAL, "rope_plan_create: bands %g .. %g of %d", c->low, c->high, c->orig_ctx);
+    if (c->scaling == QMC_ROPE_YARN &&
+        (!(c->low > 0) || !(c->high >= c->low) || !std::isfinite(c->high) || c->orig_ctx < 1 || c->theta == 1.0))
+        return set_error(QMC_EINVAL, "rope_plan_create: ramp %g .. %g of %d, theta %g", c->low, c->high, c->orig_ctx, c->theta);
+    qmc_rope_plan *p = new (std::nothrow) qmc_rope_plan();
+    if (!p) return set_error(QMC_ENOMEM, "rope_plan_create: out of memory");
+    p->head_dim = c->head_dim, p->rot_dim = rot, p->layout = c->layout;
+    const double two_pi = 6.283185307179586476925286766559;
+    double lo = 0, hi = 0;
+    p->mscale = 1.0f;
+    if (c->scaling == QMC_ROPE_YARN) {
+        auto d = [&](double turns) { return rot * log(c->orig_ctx / (two_pi * turns)) / (2.0 * log(c->theta)); };
+        lo = fmin(fmax(floor(d(c->high)), 0.0), rot - 1.0);
+        hi = fmin(fmax(ceil(d(c->low)), 0.0), rot - 1.0);
+        p->mscale = (float)(0.1 * log(c->factor) + 1.0);
+    }
+    for (int i = 0; i < rot / 2; i++) {
+        double f = pow(c->theta, -2.0 * i / rot);
+        if (c->scaling == QMC_ROPE_LINEAR) {
+            f /= c->factor;
+        } else if (c->scaling == QMC_ROPE_BANDS) {
+            const double t = c->orig_ctx * f / two_pi;
+            const double s = fmin(fmax((t - c->low) / (c->high - c->low), 0.0), 1.0);
+            f = f * s + f / c->factor * (1.0 - s);
+        } else if (c->scaling == QMC_ROPE_YARN) {
+            const double r = fmin(fmax((i - lo) / fmax(hi - lo, 0.001), 0.0), 1.0);
+            f = f / c->factor * r + f * (1.0 - r);
+        }
+        p->turns[i] = f / two_pi;
+    }
+    *out = p;
+    return QMC_OK;
+}
+
+int qmc_rope_plan_free(qmc_rope_plan *p) {
+    delete p;
+    return QMC_OK;
+}
+
+int qmc_qk_norm_rope(const qmc_rope_plan *plan, int dtype, const void *q, int64_t ldq, void *q_out, int64_t ldqo,
+                     int32_t n_heads, const void *k, int64_t ldk, void *k_out, int64_t ldko, int32_t n_kv_heads,
+                     const float *q_weight, const float *k_weight, float eps, const int32_t *positions, int64_t rows,
+                     void *stream) {
+    const char *op = "qk_norm_rope";
+    if (!plan) return set_error(QMC_EINVAL, "%s: null plan", op);
+    if (!is_row_dtype(dtype)) return set_error(QMC_EINVAL, "%s: bad dtype %d", op, dtype);
+    if (n_heads < 0 || n_kv_heads < 0 || rows < 0 || rows > INT32_MAX)
+        return set_error(QMC_EINVAL, "%s: %d + %d heads, %lld rows", op, n_heads, n_kv_heads, (long long)rows);
+    if (!(eps >= 0)) return set_error(QMC_EINVAL, "%s: eps %g", op, eps);
+    if (rows == 0 || (int64_t)n_heads + n_kv_heads == 0) return QMC_OK;
+    const int hd = plan->head_dim;
+    int rc;
+    if (n_heads && ((rc = check_rows(op, "q", q, ldq, n_heads, hd, dtype)) || (rc = check_rows(op, "q_out", q_out, ldqo, n_heads, hd, dtype))))
+        return rc;
+    if (n_kv_heads && ((rc = check_rows(op, "k", k, ldk, n_kv_heads, hd, dtype)) || (rc = check_rows(op, "k_out", k_out, ldko, n_kv_heads, hd, dtype))))
+        return rc;
+    if (!positions) return set_error(QMC_EINVAL, "%s: null positions", op);
+    DevCtx *c = ctx();
+    if (!c) return QMC_ECUDA;
+    RowsArgs a{};
+    if (n_heads) a.q = q, a.qo = q_out, a.ldq = ldq, a.ldqo = ldqo;
+    if (n_kv_heads) a.k = k, a.ko = k_out, a.ldk = ldk, a.ldko = ldko;
+    a.heads = n_heads, a.kv = n_kv_heads, a.hd = hd;
+    a.qw = q_weight, a.kw = k_weight, a.eps = eps;
+    a.pos = positions, a.err = c->err;
+    return launch_rows(a, plan, dtype, dtype, rows, pick_stream(stream));
+}
+
+int qmc_kv_append_paged(const qmc_rope_plan *plan, const qmc_paged_cache *cache, int32_t layer, int dtype,
+                        const void *q, int64_t ldq, void *q_out, int64_t ldqo, int32_t n_heads, const void *k,
+                        int64_t ldk, const void *v, int64_t ldv, const float *q_weight, const float *k_weight, float eps,
+                        const int32_t *seq, const int32_t *positions, const int32_t *page_table, int32_t n_seq,
+                        int32_t ld_table, int64_t rows, void *stream) {
+    const char *op = "kv_append_paged";
+    int rc = check_cache(cache, op);
+    if (rc) return rc;
+    const int hd = cache->head_dim, kv = cache->n_kv_heads;
+    if (hd > 256 || (hd & 1)) return set_error(QMC_EINVAL, "%s: head_dim %d is odd or above 256", op, hd);
+    if (plan && plan->head_dim != hd) return set_error(QMC_EINVAL, "%s: plan for head_dim %d, cache of %d", op, plan->head_dim, hd);
+    if (layer < 0 || layer >= cache->n_layers) return set_error(QMC_EINVAL, "%s: layer %d of %d", op, layer, cache->n_layers);
+    if (!is_row_dtype(dtype)) return set_error(QMC_EINVAL, "%s: bad dtype %d", op, dtype);
+    if (n_heads < 0 || rows < 0 || rows > INT32_MAX || n_seq < 0 || ld_table < 1)
+        return set_error(QMC_EINVAL, "%s: %d heads, %lld rows, table of %d x %d", op, n_heads, (long long)rows, n_seq, ld_table);
+    if (!(eps >= 0)) return set_error(QMC_EINVAL, "%s: eps %g", op, eps);
+    if (!q != !n_heads) return set_error(QMC_EINVAL, "%s: %d query heads with%s q", op, n_heads, q ? "" : "out");
+    if (rows == 0) return QMC_OK;
+    if (n_heads && ((rc = check_rows(op, "q", q, ldq, n_heads, hd, dtype)) || (rc = check_rows(op, "q_out", q_out, ldqo, n_heads, hd, dtype))))
+        return rc;
+    if ((rc = check_rows(op, "k", k, ldk, kv, hd, dtype)) || (rc = check_rows(op, "v", v, ldv, kv, hd, dtype))) return rc;
+    if (!positions || !page_table) return set_error(QMC_EINVAL, "%s: null positions or page table", op);
+    if (!seq && rows > n_seq) return set_error(QMC_EINVAL, "%s: %lld rows for %d sequences", op, (long long)rows, n_seq);
+    DevCtx *c = ctx();
+    if (!c) return QMC_ECUDA;
+    RowsArgs a{};
+    if (n_heads) a.q = q, a.qo = q_out, a.ldq = ldq, a.ldqo = ldqo;
+    a.k = k, a.v = v, a.ldk = ldk, a.ldv = ldv;
+    const int64_t off = layer * layer_elems(cache) * dtype_size(cache->dtype);
+    a.kc = (uint8_t *)cache->k + off, a.vc = (uint8_t *)cache->v + off;
+    a.seq = seq, a.pos = positions, a.table = page_table;
+    a.n_seq = n_seq, a.ld_table = ld_table, a.page_size = cache->page_size, a.n_pages = cache->n_pages;
+    a.heads = n_heads, a.kv = kv, a.hd = hd;
+    a.qw = q_weight, a.kw = k_weight, a.eps = eps;
+    a.err = c->err;
+    return launch_rows(a, plan, dtype, cache->dtype, rows, pick_stream(stream));
+}
+
+}  // extern "C"
