@@ -9,7 +9,7 @@
 // o = sum_j e^(m_j - M) o_j / sum_j e^(m_j - M) l_j.
 #include <algorithm>
 
-#include "batch.cuh"
+#include "attn_prefix.cuh"
 
 namespace qmc {
 namespace {
@@ -18,73 +18,12 @@ struct Plan {
     int rows;                 // query rows of a KV head over the whole batch: n_seq * group
     int ptiles, psplit;       // prefix: row tiles and position ranges
     int gtiles, osplit;       // own positions: row tiles of a group and position ranges
+    bool mma;
     int64_t ml_bytes, bytes;  // workspace: [parts][n_seq * n_heads] float2 (m, l), then [parts][...][hd] floats
-};
-
-struct AttnArgs {
-    const void *q, *kc, *vc;  // kc, vc: the layer's pools
-    void *out;
-    int64_t ldq, ldo;
-    const int *prefix_pages, *table, *lens;
-    int *err;
-    float2 *ml;
-    float *po;
-    int n_seq, heads, kv, group, hd, page_size, n_pages, ld_table, prefix;
-    int rows, ptiles, psplit, gtiles, osplit;
-    float scale;
 };
 
 constexpr int kQR = 16;  // query rows per block (4 per warp)
 constexpr int kPT = 32;  // positions per staged tile (one per lane)
-
-// the part of one job: rows [r0, r0 + nr) of KV head h, positions [p0, p1), and where its results go
-struct Job {
-    int h, r0, nr, p0, p1, part, b;  // b: the sequence of an own job, -1 for the prefix
-};
-
-__device__ __forceinline__ int own_len(const AttnArgs &a, int b) {
-    const int n = a.lens[b];
-    return min(max(n - a.prefix, 0), a.ld_table * a.page_size - a.prefix);
-}
-
-// jobs: prefix [h][tile][split], then own [b][h][group tile][split]
-__device__ __forceinline__ Job job_of(const AttnArgs &a, int64_t i, int tile, int quantum) {
-    Job j;
-    const int64_t np = (int64_t)a.kv * a.ptiles * a.psplit;
-    if (i < np) {
-        const int sp = (int)(i % a.psplit), t = (int)(i / a.psplit % a.ptiles);
-        j.h = (int)(i / a.psplit / a.ptiles);
-        j.r0 = t * tile, j.nr = min(tile, a.rows - j.r0);
-        const int64_t chunk = (((int64_t)a.prefix + a.psplit - 1) / a.psplit + quantum - 1) / quantum * quantum;
-        j.p0 = (int)min((int64_t)a.prefix, sp * chunk), j.p1 = (int)min((int64_t)a.prefix, j.p0 + chunk);
-        j.part = sp, j.b = -1;
-        return j;
-    }
-    i -= np;
-    const int sp = (int)(i % a.osplit), t = (int)(i / a.osplit % a.gtiles);
-    j.h = (int)(i / a.osplit / a.gtiles % a.kv);
-    j.b = (int)(i / a.osplit / a.gtiles / a.kv);
-    j.r0 = j.b * a.group + t * tile, j.nr = min(tile, a.group - t * tile);
-    const int64_t n = own_len(a, j.b), chunk = ((n + a.osplit - 1) / a.osplit + quantum - 1) / quantum * quantum;
-    j.p0 = a.prefix + (int)min(n, sp * chunk), j.p1 = a.prefix + (int)min(n, sp * chunk + chunk);
-    j.part = a.psplit + sp;
-    return j;
-}
-
-// slot of position p, -1 (and the error word) for a page outside the pool
-__device__ __forceinline__ int64_t slot_of(const AttnArgs &a, int b, int p) {
-    const int e = p / a.page_size, page = b < 0 ? a.prefix_pages[e] : a.table[(int64_t)b * a.ld_table + e];
-    if (page < 0 || page >= a.n_pages) {
-        raise_error(a.err, kErrBadIndex);
-        return -1;
-    }
-    return (int64_t)page * a.page_size + p % a.page_size;
-}
-
-// row r of a KV head: sequence r / group, query head h * group + r % group; its place among all batch * heads rows
-__device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
-    return (int64_t)(r / a.group) * a.heads + h * a.group + r % a.group;
-}
 
 // The general kernel, in float on the CUDA cores: any head_dim up to 256, any types, strides and alignments.  Per row and tile of
 // 32 positions lane p scores position p, the warp updates the row's maximum and sum once, and each lane
@@ -98,7 +37,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
     float *Qs = Vs + kPT * hd4;    // [kQR][hd4]
     __shared__ int64_t slot_s[kPT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const Job jb = job_of(a, blockIdx.x, kQR, kPT);
+    const Job jb = job_of(a, blockIdx.x, kQR, kQR, kPT);
     for (int i = tid; i < kQR * hd4; i += 128) {
         const int r = i / hd4, d = i % hd4, rr = jb.r0 + r;
         Qs[i] = (r < jb.nr && d < hd)
@@ -157,7 +96,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
             const float sc = p0 + lane < jb.p1 ? ((s4[0] + s4[1]) + (s4[2] + s4[3])) * a.scale : -INFINITY;
             const float mn = fmaxf(m[j], warp_max(sc));
             const float ref = mn == -INFINITY ? 0.0f : mn;
-            const float corr = expf(m[j] - ref), e = expf(sc - ref);
+            const float corr = exp2f(m[j] - ref), e = exp2f(sc - ref);
             l[j] = l[j] * corr + warp_sum(e);
             m[j] = mn;
 #pragma unroll
@@ -213,7 +152,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int pa
         for (int j = 0; j < parts; j++) {
             const float2 ml = a.ml[j * all + row];
             if (ml.y == 0.0f) continue;
-            const float w = expf(ml.x - ref);
+            const float w = exp2f(ml.x - ref);
             l = fmaf(w, ml.y, l);
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -228,15 +167,22 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int pa
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// 16-bit rows of whole 16-byte chunks go to the matrix instructions
+bool takes_mma(const qmc_paged_cache *c) {
+    return c->dtype != QMC_F32 && c->head_dim % 8 == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0;
+}
+
 Plan plan_for(const qmc_paged_cache *c, int n_seq, int n_heads, int prefix, int ld_table, int sms) {
     Plan p{};
+    p.mma = takes_mma(c);
+    const int tile = p.mma ? 64 : kPT;
     const int group = n_heads / c->n_kv_heads;
     const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix), want = 4 * sms;
     p.rows = n_seq * group;
-    p.ptiles = ceil_div(p.rows, kQR);
+    p.ptiles = ceil_div(p.rows, p.mma ? attn_mma_tile(p.rows) : kQR);
     p.gtiles = ceil_div(group, kQR);
-    p.psplit = prefix ? (int)std::min<int64_t>(ceil_div(want, (int64_t)c->n_kv_heads * p.ptiles), ceil_div(prefix, 2 * kPT)) : 0;
-    p.osplit = own ? (int)std::min<int64_t>(ceil_div(want, (int64_t)n_seq * c->n_kv_heads * p.gtiles), ceil_div(own, 2 * kPT)) : 0;
+    p.psplit = prefix ? (int)std::min<int64_t>(ceil_div(want, (int64_t)c->n_kv_heads * p.ptiles), ceil_div(prefix, 2 * tile)) : 0;
+    p.osplit = own ? (int)std::min<int64_t>(ceil_div(want, (int64_t)n_seq * c->n_kv_heads * p.gtiles), ceil_div(own, 2 * tile)) : 0;
     const int64_t parts = p.psplit + p.osplit, all = (int64_t)n_seq * n_heads;
     p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;
     p.bytes = p.ml_bytes + parts * all * c->head_dim * 4 + 256;
@@ -255,15 +201,18 @@ int launch_rows(const AttnArgs &a, int64_t jobs, bool vec, cudaStream_t s) {
 }
 
 template <typename T, typename CT>
-int launch_attn(const AttnArgs &a, cudaStream_t s) {
+int launch_attn(const AttnArgs &a, bool mma, int dtype, int cdt, cudaStream_t s) {
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
-    if (jobs) {
+    int rc = QMC_OK;
+    if (jobs && mma) {
+        rc = launch_attn_mma(a, dtype, cdt, s);
+    } else if (jobs) {
         const size_t al = 4 * sizeof(CT);
         const bool vec = a.hd % 4 == 0 && (uintptr_t)a.kc % al == 0 && (uintptr_t)a.vc % al == 0;
-        const int rc = a.hd <= 128 ? launch_rows<T, CT, 1>(a, jobs, vec, s) : launch_rows<T, CT, 2>(a, jobs, vec, s);
-        if (rc) return rc;
+        rc = a.hd <= 128 ? launch_rows<T, CT, 1>(a, jobs, vec, s) : launch_rows<T, CT, 2>(a, jobs, vec, s);
     }
+    if (rc) return rc;
     const int64_t all = (int64_t)a.n_seq * a.heads;
     attn_join_kernel<T><<<(unsigned)((all + 3) / 4), 128, 0, s>>>(a, a.psplit + a.osplit);
     QMC_LAUNCH_CHECK();
@@ -335,12 +284,13 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
     a.n_seq = n_seq, a.heads = n_heads, a.kv = cache->n_kv_heads, a.group = n_heads / cache->n_kv_heads;
     a.hd = cache->head_dim, a.page_size = cache->page_size, a.n_pages = cache->n_pages, a.ld_table = ld_table;
     a.prefix = prefix_len, a.rows = p.rows, a.ptiles = p.ptiles, a.psplit = p.psplit, a.gtiles = p.gtiles, a.osplit = p.osplit;
-    a.scale = scale;
+    a.scale = scale * 1.4426950408889634f;
     cudaStream_t s = pick_stream(stream);
-    if (dtype == QMC_F32 && cache->dtype == QMC_F32) return launch_attn<float, float>(a, s);
-    if (dtype == QMC_F32) return launch_attn<float, __half>(a, s);
-    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, s);
-    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, s);
+    const int cdt = cache->dtype;
+    if (dtype == QMC_F32 && cdt == QMC_F32) return launch_attn<float, float>(a, p.mma, dtype, cdt, s);
+    if (dtype == QMC_F32) return launch_attn<float, __half>(a, p.mma, dtype, cdt, s);
+    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, p.mma, dtype, cdt, s);
+    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, p.mma, dtype, cdt, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,74 @@
+// Work of the shared-prefix attention (attn_prefix.cu), for its kernels: the jobs of a launch and where their parts go.
+#pragma once
+
+#include "batch.cuh"
+
+namespace qmc {
+
+struct AttnArgs {
+    const void *q, *kc, *vc;  // kc, vc: the layer's pools
+    void *out;
+    int64_t ldq, ldo;
+    const int *prefix_pages, *table, *lens;
+    int *err;
+    float2 *ml;
+    float *po;
+    int n_seq, heads, kv, group, hd, page_size, n_pages, ld_table, prefix;
+    int rows, ptiles, psplit, gtiles, osplit;
+    float scale;  // times log2(e): scores and maxima are exponents of two
+};
+
+// the part of one job: rows [r0, r0 + nr) of KV head h, positions [p0, p1), and where its results go
+struct Job {
+    int h, r0, nr, p0, p1, part, b;  // b: the sequence of an own job, -1 for the prefix
+};
+
+__device__ __forceinline__ int own_len(const AttnArgs &a, int b) {
+    const int n = a.lens[b];
+    return min(max(n - a.prefix, 0), a.ld_table * a.page_size - a.prefix);
+}
+
+// jobs: prefix [h][tile][split], then own [b][h][group tile][split]; ranges of positions are multiples of `quantum`
+__device__ __forceinline__ Job job_of(const AttnArgs &a, unsigned i, int ptile, int otile, int quantum) {
+    Job j;
+    const unsigned np = (unsigned)(a.kv * a.ptiles * a.psplit);
+    if (i < np) {
+        const int sp = i % a.psplit, t = i / a.psplit % a.ptiles;
+        j.h = i / a.psplit / a.ptiles;
+        j.r0 = t * ptile, j.nr = min(ptile, a.rows - j.r0);
+        const int64_t chunk = (((int64_t)a.prefix + a.psplit - 1) / a.psplit + quantum - 1) / quantum * quantum;
+        j.p0 = (int)min((int64_t)a.prefix, sp * chunk), j.p1 = (int)min((int64_t)a.prefix, sp * chunk + chunk);
+        j.part = sp, j.b = -1;
+        return j;
+    }
+    i -= np;
+    const int sp = i % a.osplit, t = i / a.osplit % a.gtiles;
+    j.h = i / a.osplit / a.gtiles % a.kv;
+    j.b = i / a.osplit / a.gtiles / a.kv;
+    j.r0 = j.b * a.group + t * otile, j.nr = min(otile, a.group - t * otile);
+    const int64_t n = own_len(a, j.b), chunk = ((n + a.osplit - 1) / a.osplit + quantum - 1) / quantum * quantum;
+    j.p0 = a.prefix + (int)min(n, sp * chunk), j.p1 = a.prefix + (int)min(n, sp * chunk + chunk);
+    j.part = a.psplit + sp;
+    return j;
+}
+
+// slot of position p, -1 (and the error word) for a page outside the pool
+__device__ __forceinline__ int64_t slot_of(const AttnArgs &a, int b, int p) {
+    const int e = p / a.page_size, page = b < 0 ? a.prefix_pages[e] : a.table[(int64_t)b * a.ld_table + e];
+    if (page < 0 || page >= a.n_pages) {
+        raise_error(a.err, kErrBadIndex);
+        return -1;
+    }
+    return (int64_t)page * a.page_size + p % a.page_size;
+}
+
+// row r of a KV head: sequence r / group, query head h * group + r % group; its place among all batch * heads rows
+__device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
+    return (int64_t)(r / a.group) * a.heads + h * a.group + r % a.group;
+}
+
+// the matrix-instruction kernel (attn_mma.cu), for 16-bit caches whose rows are whole 16-byte chunks
+int attn_mma_tile(int rows);  // query rows of a prefix job, for `rows` of them per KV head; own jobs take 16
+int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, cudaStream_t s);
+
+}  // namespace qmc
