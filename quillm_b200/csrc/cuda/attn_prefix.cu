@@ -18,7 +18,8 @@ struct Plan {
     int rows;                 // query rows of a KV head over the whole batch: n_seq * group
     int ptiles, psplit;       // prefix: row tiles and position ranges
     int gtiles, osplit;       // own positions: row tiles of a group and position ranges
-    bool mma;
+    bool mma, tc;             // matrix instructions; tensor memory for the prefix
+    int pparts;
     int64_t ml_bytes, bytes;  // workspace: [parts][n_seq * n_heads] float2 (m, l), then [parts][...][hd] floats
 };
 
@@ -172,18 +173,35 @@ bool takes_mma(const qmc_paged_cache *c) {
     return c->dtype != QMC_F32 && c->head_dim % 8 == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0;
 }
 
-Plan plan_for(const qmc_paged_cache *c, int n_seq, int n_heads, int prefix, int ld_table, int sms) {
+// position ranges for each of `units` row tiles over `tiles` position tiles, `slots` blocks running at once: the number with
+// the fewest rounds of tiles, a block costing kBlockTiles more for its start, its end and its parts' way through memory
+constexpr int kBlockTiles = 3, kMostSplits = 64, kTcRows = 64;
+int split_for(int64_t units, int tiles, int slots) {
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int n = 1; n <= std::min(kMostSplits, tiles); n++) {
+        const int64_t cost = (units * n + slots - 1) / slots * (ceil_div(tiles, n) + kBlockTiles);
+        if (cost < least) least = cost, best = n;
+    }
+    return best;
+}
+
+Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int prefix, int ld_table, int sms) {
     Plan p{};
-    p.mma = takes_mma(c);
-    const int tile = p.mma ? 64 : kPT;
-    const int group = n_heads / c->n_kv_heads;
-    const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix), want = 4 * sms;
+    const int group = n_heads / c->n_kv_heads, kv = c->n_kv_heads;
+    const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix);
     p.rows = n_seq * group;
-    p.ptiles = ceil_div(p.rows, p.mma ? attn_mma_tile(p.rows) : kQR);
-    p.gtiles = ceil_div(group, kQR);
-    p.psplit = prefix ? (int)std::min<int64_t>(ceil_div(want, (int64_t)c->n_kv_heads * p.ptiles), ceil_div(prefix, 2 * tile)) : 0;
-    p.osplit = own ? (int)std::min<int64_t>(ceil_div(want, (int64_t)n_seq * c->n_kv_heads * p.gtiles), ceil_div(own, 2 * tile)) : 0;
-    const int64_t parts = p.psplit + p.osplit, all = (int64_t)n_seq * n_heads;
+    p.mma = takes_mma(c);
+    p.tc = p.mma && dtype == c->dtype && c->head_dim <= 128 && p.rows > kTcRows && prefix;
+    const int tile = p.mma ? 64 : kPT;                 // positions
+    const int slots = (p.mma ? 2 : 4) * sms;           // blocks that run at once
+    p.gtiles = ceil_div(group, p.mma ? 16 : kQR);
+    p.ptiles = ceil_div(p.rows, p.tc ? attn_tc_tile(p.rows) : p.mma ? attn_mma_tile(p.rows) : kQR);
+    if (p.tc) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, 128), sms);
+    else if (prefix) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, tile), slots);
+    if (own) p.osplit = split_for((int64_t)n_seq * kv * p.gtiles, ceil_div(own, tile), slots);
+    p.pparts = p.psplit * (p.tc ? attn_tc_parts(p.rows) : 1);
+    const int64_t parts = p.pparts + p.osplit, all = (int64_t)n_seq * n_heads;
     p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;
     p.bytes = p.ml_bytes + parts * all * c->head_dim * 4 + 256;
     return p;
@@ -201,11 +219,15 @@ int launch_rows(const AttnArgs &a, int64_t jobs, bool vec, cudaStream_t s) {
 }
 
 template <typename T, typename CT>
-int launch_attn(const AttnArgs &a, bool mma, int dtype, int cdt, cudaStream_t s) {
+int launch_attn(const AttnArgs &a, const Plan &p, int dtype, int cdt, cudaStream_t s) {
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
     int rc = QMC_OK;
-    if (jobs && mma) {
+    if (p.tc) {
+        AttnArgs own = a;
+        own.psplit = 0;  // own positions only
+        if (!(rc = launch_attn_tc(a, cdt, s)) && a.osplit) rc = launch_attn_mma(own, dtype, cdt, s);
+    } else if (jobs && p.mma) {
         rc = launch_attn_mma(a, dtype, cdt, s);
     } else if (jobs) {
         const size_t al = 4 * sizeof(CT);
@@ -214,7 +236,7 @@ int launch_attn(const AttnArgs &a, bool mma, int dtype, int cdt, cudaStream_t s)
     }
     if (rc) return rc;
     const int64_t all = (int64_t)a.n_seq * a.heads;
-    attn_join_kernel<T><<<(unsigned)((all + 3) / 4), 128, 0, s>>>(a, a.psplit + a.osplit);
+    attn_join_kernel<T><<<(unsigned)((all + 3) / 4), 128, 0, s>>>(a, a.pparts + a.osplit);
     QMC_LAUNCH_CHECK();
     return QMC_OK;
 }
@@ -249,7 +271,7 @@ int qmc_attn_prefix_workspace(int dtype, const qmc_paged_cache *cache, int32_t n
     if (const int rc = check_attn("attn_prefix_workspace", dtype, cache, n_seq, n_heads, prefix_len, ld_table)) return rc;
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;
-    *bytes = (size_t)plan_for(cache, n_seq, n_heads, prefix_len, ld_table, c->num_sms).bytes;
+    *bytes = (size_t)plan_for(cache, dtype, n_seq, n_heads, prefix_len, ld_table, c->num_sms).bytes;
     return QMC_OK;
 }
 
@@ -271,7 +293,7 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
         return set_error(QMC_EINVAL, "%s: misaligned q or out", op);
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;
-    const Plan p = plan_for(cache, n_seq, n_heads, prefix_len, ld_table, c->num_sms);
+    const Plan p = plan_for(cache, dtype, n_seq, n_heads, prefix_len, ld_table, c->num_sms);
     if (workspace_bytes < (size_t)p.bytes)
         return set_error(QMC_EINVAL, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, (size_t)p.bytes);
     AttnArgs a{};
@@ -283,14 +305,14 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
     a.ml = (float2 *)w, a.po = (float *)(w + p.ml_bytes);
     a.n_seq = n_seq, a.heads = n_heads, a.kv = cache->n_kv_heads, a.group = n_heads / cache->n_kv_heads;
     a.hd = cache->head_dim, a.page_size = cache->page_size, a.n_pages = cache->n_pages, a.ld_table = ld_table;
-    a.prefix = prefix_len, a.rows = p.rows, a.ptiles = p.ptiles, a.psplit = p.psplit, a.gtiles = p.gtiles, a.osplit = p.osplit;
+    a.prefix = prefix_len, a.rows = p.rows, a.ptiles = p.ptiles, a.psplit = p.psplit, a.gtiles = p.gtiles, a.osplit = p.osplit, a.pparts = p.pparts;
     a.scale = scale * 1.4426950408889634f;
     cudaStream_t s = pick_stream(stream);
     const int cdt = cache->dtype;
-    if (dtype == QMC_F32 && cdt == QMC_F32) return launch_attn<float, float>(a, p.mma, dtype, cdt, s);
-    if (dtype == QMC_F32) return launch_attn<float, __half>(a, p.mma, dtype, cdt, s);
-    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, p.mma, dtype, cdt, s);
-    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, p.mma, dtype, cdt, s);
+    if (dtype == QMC_F32 && cdt == QMC_F32) return launch_attn<float, float>(a, p, dtype, cdt, s);
+    if (dtype == QMC_F32) return launch_attn<float, __half>(a, p, dtype, cdt, s);
+    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, p, dtype, cdt, s);
+    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, p, dtype, cdt, s);
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@ struct AttnArgs {
     float *po;
     int n_seq, heads, kv, group, hd, page_size, n_pages, ld_table, prefix;
     int rows, ptiles, psplit, gtiles, osplit;
+    int pparts;   // parts that the prefix leaves of each row; the own ones follow
     float scale;  // times log2(e): scores and maxima are exponents of two
 };
 
@@ -48,7 +49,7 @@ __device__ __forceinline__ Job job_of(const AttnArgs &a, unsigned i, int ptile, 
     j.r0 = j.b * a.group + t * otile, j.nr = min(otile, a.group - t * otile);
     const int64_t n = own_len(a, j.b), chunk = ((n + a.osplit - 1) / a.osplit + quantum - 1) / quantum * quantum;
     j.p0 = a.prefix + (int)min(n, sp * chunk), j.p1 = a.prefix + (int)min(n, sp * chunk + chunk);
-    j.part = a.psplit + sp;
+    j.part = a.pparts + sp;
     return j;
 }
 
@@ -70,5 +71,11 @@ __device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
 // the matrix-instruction kernel (attn_mma.cu), for 16-bit caches whose rows are whole 16-byte chunks
 int attn_mma_tile(int rows);  // query rows of a prefix job, for `rows` of them per KV head; own jobs take 16
 int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, cudaStream_t s);
+
+// the tensor-core kernel (attn_tc.cu): the prefix jobs of such a cache with rows of its own type and head_dim <= 128, for many
+// rows; a job of up to 128 rows leaves two parts
+int attn_tc_tile(int rows);
+int attn_tc_parts(int rows);
+int launch_attn_tc(const AttnArgs &a, int cdt, cudaStream_t s);
 
 }  // namespace qmc
