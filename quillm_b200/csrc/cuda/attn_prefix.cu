@@ -192,7 +192,8 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
     const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix);
     p.rows = n_seq * group;
     p.mma = takes_mma(c);
-    p.tc = p.mma && dtype == c->dtype && c->head_dim <= 128 && p.rows > kTcRows && prefix;
+    p.tc = p.mma && dtype == c->dtype && c->head_dim <= 128 && p.rows > kTcRows && prefix &&
+           layer_elems(c) < ((int64_t)1 << 35);
     const int tile = p.mma ? 64 : kPT;                 // positions
     const int slots = (p.mma ? 2 : 4) * sms;           // blocks that run at once
     p.gtiles = ceil_div(group, p.mma ? 16 : kQR);
@@ -285,7 +286,7 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
     const int64_t n = (int64_t)n_heads * cache->head_dim;
     if (ldq < n || ldo < n || ldq > (int64_t)1 << 40 || ldo > (int64_t)1 << 40)
         return set_error(QMC_EINVAL, "%s: rows of %lld elements are %lld and %lld apart", op, (long long)n, (long long)ldq, (long long)ldo);
-    if (!(scale == scale) || scale - scale != 0.0f) return set_error(QMC_EINVAL, "%s: scale %g", op, scale);
+    if (!(scale >= 0.0f) || scale - scale != 0.0f) return set_error(QMC_EINVAL, "%s: scale %g", op, scale);
     if (n_seq == 0) return QMC_OK;
     if (!q || !out || !page_table || !seq_lens || !workspace || (prefix_len && !prefix_pages))
         return set_error(QMC_EINVAL, "%s: null argument", op);

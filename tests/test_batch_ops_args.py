@@ -109,7 +109,7 @@ def test_attn_refuses_caches(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(layer=2), dict(layer=-1), dict(dtype=2), dict(dtype=4), dict(q=None), dict(out=None), dict(ldq=255), dict(ldo=255),
-    dict(heads=3), dict(heads=0), dict(n_seq=-1), dict(scale=math.nan), dict(scale=math.inf), dict(pages=None),
+    dict(heads=3), dict(heads=0), dict(n_seq=-1), dict(scale=math.nan), dict(scale=math.inf), dict(scale=-0.5), dict(pages=None),
     dict(prefix=-1), dict(prefix=17), dict(table=None), dict(ld=0), dict(ld=1 << 30), dict(lens=None), dict(ws=None), dict(q=A + 1)])
 def test_attn_refusals(bad):
     refused(attn(cache(), **bad), "attn_prefix")
