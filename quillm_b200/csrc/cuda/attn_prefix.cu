@@ -193,7 +193,8 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
     p.rows = n_seq * group;
     p.mma = takes_mma(c);
     p.tc = p.mma && dtype == c->dtype && c->head_dim <= 128 && p.rows > kTcRows && prefix &&
-           layer_elems(c) < ((int64_t)1 << 35);
+           c->page_size % 8 == 0 &&
+           (int64_t)c->n_pages * c->page_size <= INT32_MAX;
     const int tile = p.mma ? 64 : kPT;                 // positions
     const int slots = (p.mma ? 2 : 4) * sms;           // blocks that run at once
     p.gtiles = ceil_div(group, p.mma ? 16 : kQR);

@@ -72,8 +72,9 @@ __device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
 int attn_mma_tile(int rows);  // query rows of a prefix job, for `rows` of them per KV head; own jobs take 16
 int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, cudaStream_t s);
 
-// the tensor-core kernel (attn_tc.cu): the prefix jobs of such a cache with rows of its own type and head_dim <= 128, for many
-// rows; a job of up to 128 rows leaves two parts
+// the tensor-core kernel (attn_tc.cu): the prefix jobs of such a cache with rows of its own type, head_dim <= 128, pages of a
+// multiple of 8 positions and under 2^31 slots, for many rows; a job of up to 128 rows leaves two parts
+int attn_tc_box(int page_size);  // positions of one copy
 int attn_tc_tile(int rows);
 int attn_tc_parts(int rows);
 int launch_attn_tc(const AttnArgs &a, int cdt, cudaStream_t s);

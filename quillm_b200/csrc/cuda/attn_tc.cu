@@ -1,30 +1,35 @@
 // The prefix part of the shared-prefix attention on the 5th-generation tensor cores, for many query rows per KV head:
 // tcgen05.mma with scores and accumulators in tensor memory (TMEM).
 //
-// Per 128 query rows and 128 positions: S = Q K^T (M = 128 rows, N = 128 positions) into 128 TMEM columns; a warpgroup,
-// one thread per row, turns S into weights P = 2^(scale S - m) and writes them over S as 16-bit pairs; O += P V with P
+// Per 128 query rows and 128 positions: S = Q K^T (M = 128 rows, N = 128 positions) into 128 TMEM columns; eight warps,
+// two threads per row, turn S into weights P = 2^(scale S - m) and write them over S as 16-bit pairs; O += P V with P
 // read from TMEM as the A operand and V from shared memory as it lies in the cache ([position][dim], an MN-major
 // operand).  A row's reference m moves only when a score passes it by more than 8 (weights stay below 2^8, exact
-// in the split of l and O): then the warp rescales its O rows in TMEM and takes the tile again, which after a row's first
+// in the split of l and O): then the row's warps rescale their O rows in TMEM and take the tile again, which after a row's first
 // tile is rare, so O normally stays where it is until the end.
 //
-// A block runs two streams of such tiles, so that the tensor cores work on one while the other's warpgroup takes its
+// A block runs two streams of such tiles, so that the tensor cores work on one while the other's warps take its
 // exponentials (16384 of them per tile at 16 a cycle are as long as the tile's two products).  PAIR: the streams are
 // two row tiles over the same positions (each K and V tile is read once for 256 rows).  Otherwise, with at most 128 rows, they
 // take the range's position tiles in turn and leave a part each.
 //
-// Warps 0-3 and 4-7: the streams' weights (warp w may access TMEM lanes 32 (w % 4) .. + 31); 8-11: copies, 16 bytes a thread at
-// a time, each position's row found through its page, into a ring of K and V tiles in the 128-byte swizzle (chunk c of
-// row r at c ^ (r & 7), a panel of 128 rows for each 64 dimensions); 12: one lane issues the MMAs.  Every wait is bounded: after a
-// timeout a role raises the error word and falls through to the end, where the copies and MMAs in flight are waited for
-// (bounded) and the TMEM is freed.
+// Warps 0-7 and 8-15: the streams' weights, two threads a row with half of the positions each; 16: TMA, a lane for each box of
+// a K or V tile; 17: one lane issues the MMAs.  A box is a run of rows within a page (the largest power of two that divides the
+// page size, 8 to 128 of them) and 64 dimensions wide, the 128-byte swizzle's row.  Dimensions past the head are the next
+// head's, or zeros: for the scores Q has zeros there, in O they are not stored.  Rows past the range, which a box may bring along, are
+// masked in the scores and overwritten with zeros in the last V tile, since what lies there need not be finite.
+// Every wait is bounded: after a timeout a role raises the error word and falls through to the end, where the copies and MMAs in
+// flight are waited for (bounded) and the TMEM is freed.  A role that has stopped leaves the others to their own timeouts.
+#include <algorithm>
+
 #include "attn_prefix.cuh"
+#include "matmul_tc.cuh"
 
 namespace qmc {
 namespace {
 
 constexpr int kM = 128, kN = 128;  // rows and positions of a tile
-constexpr int kCopyWarps = 4, kMmaWarp = 8 + kCopyWarps, kThreads = (kMmaWarp + 1) * 32;
+constexpr int kCopyWarp = 16, kMmaWarp = 17, kThreads = 18 * 32;  // warps 0-15: weights
 constexpr float kLift = 8.0f;      // how far a score may pass its row's reference, in powers of two
 
 template <int HDP>
@@ -54,14 +59,12 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *(const uint32_t *)&h;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
 }
-// this thread's arrival on a barrier once its copies so far have landed
-__device__ __forceinline__ void copies_arrive(uint64_t *bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // shared-memory operand descriptors, 128-byte swizzle.  K-major (rows of 64 elements, eight-row groups 1024 bytes apart); MN-major
 // (64 elements of M or N a row, eight-row groups of K 1024 bytes apart, the next 64 elements a panel further)
@@ -75,6 +78,11 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
 __device__ __forceinline__ constexpr uint32_t idesc(int n, bool bmn, bool bf16) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((bmn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(kM >> 4) << 24);
+}
+__device__ __forceinline__ bool elect_one() {  // true for one lane of a converged warp
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t acc) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
@@ -140,56 +148,94 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ uint32_t live_bits(int left, int at) {
     return left >= at + 32 ? 0xffffffffu : left <= at ? 0u : (1u << (left - at)) - 1u;
 }
-// one row of a tile, read in halves of 64 scores: the largest, and 2^(scale s - m) as 16-bit pairs over the scores (a half's pairs
-// lie on the first quarter or second quarter of the columns, which have been read by then) with their sum, before rounding.
-// MASK: only the first `left` positions exist
-template <bool MASK>
-__device__ __forceinline__ float row_max(uint32_t ts, int left) {
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        uint32_t x[64];
-        tmem_ld64(ts + 64 * h, x);
-#pragma unroll
-        for (int k = 0; k < 64; k++) {
-            const float s = __uint_as_float(x[k]);
-            if (!MASK || (live_bits(left, 64 * h + (k & 32)) >> (k & 31) & 1u)) mx[k & 3] = fmaxf(mx[k & 3], s);
-        }
-    }
-    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+// pairs of floats, one instruction each
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
 }
-template <typename CT, bool MASK>
-__device__ __forceinline__ float row_weights(uint32_t ts, float scale, float m, int left) {
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        uint32_t x[64];
-        tmem_ld64(ts + 64 * h, x);
-#pragma unroll
-        for (int k = 0; k < 64; k += 2) {
-            float t0 = fmaf(__uint_as_float(x[k]), scale, -m), t1 = fmaf(__uint_as_float(x[k + 1]), scale, -m);
-            if (MASK) {
-                const uint32_t live = live_bits(left, 64 * h + (k & 32)) >> (k & 31);
-                t0 = live & 1u ? t0 : -INFINITY;
-                t1 = live & 2u ? t1 : -INFINITY;
-            }
-            const float p0 = ex2(t0), p1 = ex2(t1);
-            sum[k & 2] += p0, sum[(k & 2) + 1] += p1;
-            x[k / 2] = pack2(CT(), p0, p1);
-        }
-        tmem_st32(ts + 32 * h, x);
+__device__ __forceinline__ void of_pair(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^t of a pair without the special-function unit, t in [-126, 127]: n = t rounded to an integer (as the low bits of t +
+// 1.5 * 2^23), 2^(t - n) by the minimax polynomial of the relative error on [-1/2, 1/2] (degree 3: 2^-13.7, under a bf16 step's
+// 1/50; degree 4: 2^-18.5, for fp16), n added to its exponent
+template <bool BF>
+__device__ __forceinline__ void ex2_pair(uint64_t t, float &p0, float &p1) {
+    const float kRnd = 12582912.0f;
+    const uint64_t up = add2(t, pair_of(kRnd, kRnd)), n = add2(up, pair_of(-kRnd, -kRnd));
+    const uint64_t f = fma2(n, pair_of(-1.0f, -1.0f), t);
+    uint64_t v;
+    if (BF) {
+        v = fma2(f, pair_of(0.05517166852951f, 0.05517166852951f), pair_of(0.24261112511158f, 0.24261112511158f));
+        v = fma2(f, v, pair_of(0.69326096773148f, 0.69326096773148f));
+        v = fma2(f, v, pair_of(0.99992805719376f, 0.99992805719376f));
+    } else {
+        v = fma2(f, pair_of(0.00957010220736f, 0.00957010220736f), pair_of(0.05591785907745f, 0.05591785907745f));
+        v = fma2(f, v, pair_of(0.24024744331837f, 0.24024744331837f));
+        v = fma2(f, v, pair_of(0.69312179088593f, 0.69312179088593f));
+        v = fma2(f, v, pair_of(0.99999928474426f, 0.99999928474426f));
     }
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    float u0, u1, v0, v1;
+    of_pair(up, u0, u1);
+    of_pair(v, v0, v1);
+    p0 = __int_as_float(__float_as_int(v0) + (__float_as_int(u0) << 23));
+    p1 = __int_as_float(__float_as_int(v1) + (__float_as_int(u1) << 23));
+}
+// 64 of a row's scores: 2^(scale s - m) as 16-bit pairs over the first 32 registers, their sum before rounding added to `sum`, the
+// largest exponent to `mx`.  The special-function unit gives 16 results a cycle and SM, the products take 4096 flops:
+// three of every eight pairs, spread among the others, go to the FMA pipe instead.  MASK: only the first `left` positions exist
+template <typename CT, bool MASK>
+__device__ __forceinline__ void half_weights(uint32_t (&x)[64], float scale, float m, int left, float (&mx)[2], uint64_t (&sum)[2]) {
+    constexpr bool BF = __is_same(CT, __nv_bfloat16);
+    const uint64_t sc = pair_of(scale, scale), mm = pair_of(-m, -m);
+#pragma unroll
+    for (int k = 0; k < 64; k += 2) {
+        uint64_t t = fma2(pair_of(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sc, mm);
+        float t0, t1, p0, p1;
+        of_pair(t, t0, t1);
+        if (MASK) {
+            const uint32_t live = live_bits(left, k & 32) >> (k & 31);
+            t0 = live & 1u ? t0 : -INFINITY;
+            t1 = live & 2u ? t1 : -INFINITY;
+        }
+        mx[(k >> 1) & 1] = fmaxf(mx[(k >> 1) & 1], fmaxf(t0, t1));
+        if (!MASK && (k >> 1) % 8 % 3 == 1) {
+            ex2_pair<BF>(pair_of(fmaxf(t0, -126.0f), fmaxf(t1, -126.0f)), p0, p1);
+        } else {
+            p0 = ex2(t0), p1 = ex2(t1);
+        }
+        sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(p0, p1));
+        x[k / 2] = pack2(CT(), p0, p1);
+    }
+}
+// barrier `id` of two warps: the or of their verdicts
+__device__ __forceinline__ bool pair_any(int id, bool v) {
+    int r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 64, p;\n selp.s32 %0, 1, 0, q;\n}\n"
+        : "=r"(r)
+        : "r"((int)v), "r"(id)
+        : "memory");
+    return r != 0;
 }
 
 struct Shared {
-    uint64_t full[6], empty[6], sfull[2], pfull[2], ofin[2], drain;
+    uint64_t full[6], empty[6], sfull[2], pfull[2], ofin[2], vlast, drain;
+    float top[2][kM];  // what a row's two threads exchange
     uint32_t tmem;
-    int dead;
 };
 
 template <typename CT, int HDP, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a, int box) {
     extern __shared__ __align__(128) uint8_t sm_raw[];
     __shared__ Shared sh;
     constexpr int NS = ring<HDP, PAIR>(), TB = tile_bytes<HDP>(), CH = HDP / 8, PANEL = 128 * 128;  // chunks of a row; bytes of 64 dimensions
@@ -205,25 +251,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a) 
 
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
-            mbar_init(&sh.full[i], 32 * kCopyWarps);  // the copying threads
-            mbar_init(&sh.empty[i], 1);               // a commit
+            mbar_init(&sh.full[i], 1);   // the expected bytes
+            mbar_init(&sh.empty[i], 1);  // a commit
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.pfull[i], 4);    // the stream's warps
+            mbar_init(&sh.pfull[i], 8);    // the stream's warps
             mbar_init(&sh.ofin[i], 1);
         }
+        mbar_init(&sh.vlast, 1);
         mbar_init(&sh.drain, 1);
-        sh.dead = 0;
         fence_mbar_init();
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp < 8) {  // the query tiles; rows past the last and chunks past the head are zeros
+    if (warp < kCopyWarp) {  // the query tiles; rows past the last and chunks past the head are zeros
         const bool vec = a.ldq % 8 == 0 && (uintptr_t)a.q % 16 == 0;
-        for (int i = tid; i < (PAIR ? 2 : 1) * kM * CH; i += 256) {
+        for (int i = tid; i < (PAIR ? 2 : 1) * kM * CH; i += 32 * kCopyWarp) {
             const int r = i / CH, c = i % CH, rr = jb.r0 + r;
             alignas(16) CT e[8];
             *(uint4 *)e = make_uint4(0, 0, 0, 0);
@@ -235,208 +281,260 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a) 
             }
             *(uint4 *)(base + (r / kM) * TB + place(r % kM, c)) = *(const uint4 *)e;
         }
-    } else if (nch < CH) {  // K and V: chunks past the head, in the whole ring, never written again
-        for (int i = tid - 256; i < NS * kN * (CH - nch); i += kThreads - 256) {
-            const int r = i / (CH - nch), c = nch + i % (CH - nch);
-            *(uint4 *)(base + (smk - smq) + (r / kN) * TB + place(r % kN, c)) = make_uint4(0, 0, 0, 0);
-        }
     }
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;  // S (and P) of stream w at columns 128 w, O at 256 + HDP w
-    volatile int *dead = &sh.dead;
+    // all 512 columns are this block's, so they start at 0: S (and P) of stream w at 128 w, O at 256 + HDP w
+    constexpr uint32_t tmem = 0;
 
-    if (warp >= 8 && warp < 8 + kCopyWarps) {  // ---------------------------------------------------------------- copies
-        // warp wl copies rows 32 wl .. + 31 of every tile; its lane i knows where row 32 wl + i lies, in 16-byte units from
-        // the pool's start (a layer's pool is under 2^36 bytes)
-        const int wl = warp - 8, c = lane % CH, rl = lane / CH;
-        constexpr int RPI = 32 / CH;  // rows an instruction covers
-        constexpr uint32_t kNone = 0xffffffffu;
-        auto find = [&](int j) {
-            const int p = jb.p0 + j * kN + 32 * wl + lane;
-            const int64_t s = p < jb.p1 ? slot_of(a, -1, p) : (int64_t)-1;
-            return s >= 0 ? (uint32_t)((s * a.kv + jb.h) * nch) : kNone;
-        };
-        uint32_t put[8 / RPI];  // this lane's place in rows rl, rl + RPI, ... of an eight-row group
-#pragma unroll
-        for (int i = 0; i < 8 / RPI; i++) put[i] = place(32 * wl + i * RPI + rl, c);
-        auto issue = [&](uint32_t slot, int u, const uint8_t *pool) {  // tile u of the sequence K0 V0 K1 V1 ...
-            const int at = u % NS;
-            if (u >= NS && __any_sync(0xffffffffu, !mbar_wait(&sh.empty[at], (u / NS - 1) & 1) || *dead)) {
-                if (lane == 0 && !*dead) raise_error(a.err, kErrMbarTimeout);
-                *dead = 1;
+    if (warp == kCopyWarp) {  // ---------------------------------------------------------------- TMA
+        // lane i: box i % groups of the tile's rows, panel i / groups of 64 dimensions
+        const int groups = kN / box, g = lane % groups, panel = lane / groups;
+        const bool mine = panel < HDP / 64;
+        int issued = 0;
+        auto issue = [&](int row, int left, int u, const CUtensorMap *map) {  // tile u of the sequence K0 V0 K1 V1 ...
+            const int at = u % NS, here = min(groups, (left + box - 1) / box);
+            if (u >= NS && __any_sync(0xffffffffu, !mbar_wait(&sh.empty[at], (u / NS - 1) & 1))) {
+                if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 return false;
             }
-            const uint32_t st = smk + at * TB;
-            const uint8_t *src = pool + 16 * c;
-#pragma unroll
-            for (int i = 0; i < 32 / RPI; i++) {
-                const uint32_t s = __shfl_sync(0xffffffffu, slot, i * RPI + rl);
-                const uint32_t to = st + put[i % (8 / RPI)] + (i * RPI / 8 * 8) * 128;
-                if (c < nch) copy16(to, src + (s != kNone ? (uint64_t)s * 16 : 0), s != kNone);
-            }
-            copies_arrive(&sh.full[at]);
+            if (lane == 0) mbar_arrive_tx(&sh.full[at], here * (HDP / 64) * box * 128);
+            __syncwarp();
+            if (mine && g < here) tma_2d(smk + at * TB + panel * PANEL + g * box * 128, map, jb.h * hd + 64 * panel, row, &sh.full[at]);
+            issued = u + 1;
             return true;
         };
-        uint32_t slot = ntile > 0 ? find(0) : kNone;
         for (int j = 0; j < ntile; j++) {
-            const uint32_t next = j + 1 < ntile ? find(j + 1) : kNone;
-            if (!issue(slot, 2 * j, (const uint8_t *)a.kc) || !issue(slot, 2 * j + 1, (const uint8_t *)a.vc)) break;
-            slot = next;
-        }
-        copy_wait_all();
-    } else if (warp == kMmaWarp) {  // ---------------------------------------------------------------- MMA issuer
-        if (lane == 0) {
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t parity) {
-                if (ok && (!mbar_wait(bar, parity) || *dead)) {
-                    if (!*dead) raise_error(a.err, kErrMbarTimeout);
-                    *dead = 1;
-                    ok = false;
+            const int p = jb.p0 + j * kN + g * box, left = jb.p1 - jb.p0 - j * kN;
+            int row = -kN;  // a page outside the pool: rows that do not exist read as zeros
+            if (p < jb.p1) {
+                const int64_t slot = slot_of(a, -1, p);
+                if (slot >= 0) row = (int)slot;
+            }
+            if (!issue(row, left, 2 * j, &kmap) || !issue(row, left, 2 * j + 1, &vmap)) break;
+            if (left < kN) {  // the last V tile: zeros behind the range, once its copies have landed
+                const int u = 2 * j + 1, at = u % NS;
+                if (__any_sync(0xffffffffu, !mbar_wait(&sh.full[at], (u / NS) & 1))) {
+                    if (lane == 0) raise_error(a.err, kErrMbarTimeout);
+                    break;
                 }
-                return ok;
-            };
-            auto tile = [&](int u) {  // has landed; the copies are ordered before the tensor core's reads of them
-                if (!wait(&sh.full[u % NS], (u / NS) & 1)) return false;
+                for (int i = lane; i < (kN - left) * CH; i += 32)
+                    *(uint4 *)(base + (smk - smq) + at * TB + place(left + i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
-                return true;
-            };
-            auto scores = [&](int w, int j) {  // S_w = Q_w K_j^T
-                if (!tile(2 * j)) return;
-                tc_fence_after();
-                const uint32_t q = smq + (PAIR ? w : 0) * TB, k = smk + (2 * j) % NS * TB;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.vlast);
+            }
+        }
+        // no copy may still be landing when the block exits
+        const long long t0 = clock64();
+        for (int u = max(0, issued - NS); u < issued; u++)
+            if (!mbar_wait_since(&sh.full[u % NS], (u / NS) & 1, t0)) {
+                if (lane == 0) raise_error(a.err, kErrMbarTimeout);
+                break;
+            }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {  // ---------------------------------------------------------------- MMA issuer
+        // the whole warp runs this, one lane issues: addresses and descriptors stay uniform, where a lone lane would move each
+        // of them to the uniform registers that the instruction takes
+        const bool lead = elect_one();
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+            if (!ok && lane == 0) raise_error(a.err, kErrMbarTimeout);
+            return ok;
+        };
+        auto tile = [&](int u) {  // has landed
+            if ((u & 1) && jb.p1 - jb.p0 < (u / 2 + 1) * kN && !wait(&sh.vlast, 0)) return false;
+            return wait(&sh.full[u % NS], (u / NS) & 1);
+        };
+        auto scores = [&](int w, int j) {  // S_w = Q_w K_j^T
+            const uint32_t q = smq + (PAIR ? w : 0) * TB, k = smk + (2 * j) % NS * TB;
+            if (lead) {
 #pragma unroll
                 for (int i = 0; i < HDP / 16; i++) {
                     const uint32_t off = (i >> 2) * PANEL + (i & 3) * 32;
-                    mma_ss(tmem + 128 * w, desc_k(q + off), desc_k(k + off), idesc(kN, false, BF), i > 0);
+                    mma_ss(128 * w, desc_k(q + off), desc_k(k + off), idesc(kN, false, BF), i > 0);
                 }
                 mma_commit(&sh.sfull[w]);
                 if (!PAIR || w == 1) mma_commit(&sh.empty[(2 * j) % NS]);
-            };
-            auto weigh = [&](int w, int j, int i) {  // O_w += P_w V_j, the stream's i-th tile
-                if (!tile(2 * j + 1) || !wait(&sh.pfull[w], i & 1u)) return;
-                tc_fence_after();
-                const uint32_t v = smk + (2 * j + 1) % NS * TB;
+            }
+        };
+        auto weigh = [&](int w, int j, bool first) {  // O_w += P_w V_j
+            const uint32_t v = smk + (2 * j + 1) % NS * TB;
+            if (lead) {
 #pragma unroll
                 for (int k = 0; k < kN / 16; k++)
-                    mma_ts(tmem + 256 + HDP * w, tmem + 128 * w + 8 * k, desc_mn(v + k * 16 * 128), idesc(HDP, true, BF),
-                           i > 0 || k > 0);
+                    mma_ts(256 + HDP * w, 128 * w + 8 * k, desc_mn(v + k * 16 * 128), idesc(HDP, true, BF), !first || k > 0);
                 if (!PAIR || w == 1) mma_commit(&sh.empty[(2 * j + 1) % NS]);
-            };
-            constexpr int step = PAIR ? 1 : 2;  // tiles from one of a stream's to its next
-            for (int w = 0; w < 2; w++) {
-                const int j = PAIR ? 0 : w;
-                if (j < ntile) scores(w, j);
             }
-            for (int i = 0; i * step < ntile && ok; i++)
-                for (int w = 0; w < 2 && ok; w++) {
-                    const int j = PAIR ? i : 2 * i + w;
-                    if (j >= ntile) continue;
-                    weigh(w, j, i);
-                    if (!ok) break;
-                    if (j + step < ntile) scores(w, j + step);
-                    else mma_commit(&sh.ofin[w]);
-                }
-            // nothing may be in flight when the TMEM is freed
-            mma_commit(&sh.drain);
-            if (!mbar_wait(&sh.drain, 0)) raise_error(a.err, kErrMbarTimeout);
+        };
+        constexpr int step = PAIR ? 1 : 2;  // tiles from one of a stream's to its next
+        bool ok = true;
+        for (int w = 0; w < 2 && ok; w++) {
+            const int j = PAIR ? 0 : w;
+            if (j < ntile && (ok = tile(2 * j))) scores(w, j);
         }
+        for (int i = 0; i * step < ntile && ok; i++)
+            for (int w = 0; w < 2 && ok; w++) {
+                const int j = PAIR ? i : 2 * i + w;
+                if (j >= ntile) continue;
+                // the tiles of both products first (PAIR: of both streams), while the tensor cores work on the other stream, so that
+                // nothing but the issue follows the weights
+                if (!PAIR || w == 0) ok = tile(2 * j + 1) && (j + step >= ntile || tile(2 * (j + step)));
+                ok = ok && wait(&sh.pfull[w], i & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                weigh(w, j, i == 0);
+                if (j + step < ntile) scores(w, j + step);
+                else if (lead) mma_commit(&sh.ofin[w]);
+            }
+        // nothing may be in flight when the TMEM is freed
+        if (lead) mma_commit(&sh.drain);
+        if (!mbar_wait(&sh.drain, 0) && lane == 0) raise_error(a.err, kErrMbarTimeout);
         __syncwarp();
     } else {  // ---------------------------------------------------------------- weights
-        const int w = warp >> 2, row = 32 * (warp & 3) + lane, r = (PAIR ? w * kM : 0) + row;
-        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), ts = lanes + 128 * w, to = lanes + 256 + HDP * w;
+        // warps 8 w + 4 half + q: stream w, rows 32 q .. + 31 (the TMEM lanes a warp may access), half of the columns.  The two
+        // warps of a row meet once a tile: before either writes weights over scores that the other reads, and to
+        // agree on the row's reference.  A warp whose wait has expired goes on through the barriers without touching TMEM.
+        const int w = warp >> 3, half = (warp >> 2) & 1, row = 32 * (warp & 3) + lane, r = (PAIR ? w * kM : 0) + row;
+        const int id = 1 + 4 * w + (warp & 3);
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = lanes + 128 * w, to = lanes + 256 + HDP * w;
         const int mine = PAIR ? ntile : (ntile - w + 1) / 2;
+        auto larger = [&](float v) {  // of the row's two values, in both threads
+            if (half) sh.top[w][row] = v;
+            pair_any(id, false);
+            if (!half) sh.top[w][row] = v = fmaxf(v, sh.top[w][row]);
+            pair_any(id, false);
+            return half ? sh.top[w][row] : v;
+        };
         float m = 0.0f, l = 0.0f;
         bool ok = true;
         for (int i = 0; i < mine; i++) {
-            const int j = PAIR ? i : 2 * i + w, left = jb.p1 - jb.p0 - j * kN;
-            if (__any_sync(0xffffffffu, !mbar_wait(&sh.sfull[w], i & 1u) || *dead)) {
-                if (lane == 0 && !*dead) raise_error(a.err, kErrMbarTimeout);
-                *dead = 1;
+            const int j = PAIR ? i : 2 * i + w, left = jb.p1 - jb.p0 - j * kN - 64 * half;  // of this warp's columns
+            if (ok && __any_sync(0xffffffffu, !mbar_wait(&sh.sfull[w], i & 1u))) {
+                if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 ok = false;
-                break;
             }
             tc_fence_after();
-            const bool whole = left >= kN;
-            const float top = whole ? row_max<false>(ts, left) : row_max<true>(ts, left), mx = top * a.scale;
-            if (i == 0) {
-                m = mx == -INFINITY ? 0.0f : mx;
-            } else if (__any_sync(0xffffffffu, mx > m + kLift)) {
-                // lift the references of the warp's rows; O holds the tiles before this one, whose product is complete (this
-                // tile's scores were committed after it)
-                const float to_m = fmaxf(m, mx), down = ex2(m - to_m);
-                m = to_m, l *= down;
-                for (int c = 0; c < HDP / 32; c++) {
-                    uint32_t x[32];
-                    tmem_ld32(to + 32 * c, x);
+            uint32_t x[64];
+            if (i == 0) {  // the first reference: the row's largest score
+                float mx = -INFINITY;
+                if (ok) {
+                    tmem_ld64(ts + 64 * half, x);
+                    const uint32_t lo = live_bits(left, 0), hi = live_bits(left, 32);
 #pragma unroll
-                    for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * down);
-                    tmem_st32(to + 32 * c, x);
+                    for (int k = 0; k < 64; k++)
+                        mx = fmaxf(mx, (k < 32 ? lo : hi) >> (k & 31) & 1u ? __uint_as_float(x[k]) : -INFINITY);
                 }
+                mx = larger(mx);
+                m = mx == -INFINITY ? 0.0f : mx * a.scale;
             }
-            l += whole ? row_weights<CT, false>(ts, a.scale, m, left) : row_weights<CT, true>(ts, a.scale, m, left);
-            tmem_wait_st();
+            float mx[2] = {-INFINITY, -INFINITY};
+            uint64_t sum[2] = {0, 0};
+            auto weigh = [&]() {
+                if (!ok) return;
+                tmem_ld64(ts + 64 * half, x);
+                if (left >= 64) half_weights<CT, false>(x, a.scale, m, left, mx, sum);
+                else half_weights<CT, true>(x, a.scale, m, left, mx, sum);
+            };
+            weigh();
+            if (pair_any(id, fmaxf(mx[0], mx[1]) > kLift)) {
+                // lift the references of the two warps' rows and take the scores again; O (half of its columns each) holds
+                // the tiles before this one, whose product is complete (this tile's scores were committed after it)
+                const float up = fmaxf(0.0f, larger(fmaxf(mx[0], mx[1]))), down = ex2(-up);
+                m += up, l *= down;
+                if (ok && i > 0)
+                    for (int c = 0; c < HDP / 64; c++) {
+                        uint32_t z[32];
+                        tmem_ld32(to + HDP / 2 * half + 32 * c, z);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) z[k] = __float_as_uint(__uint_as_float(z[k]) * down);
+                        tmem_st32(to + HDP / 2 * half + 32 * c, z);
+                    }
+                sum[0] = sum[1] = 0;
+                weigh();
+                pair_any(id, false);  // both have read the scores
+            }
+            float s0, s1;
+            of_pair(add2(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
+            if (ok) {
+                tmem_st32(ts + 32 * half, x);
+                tmem_wait_st();
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.pfull[w]);
         }
-        if (ok && mine > 0 && __any_sync(0xffffffffu, !mbar_wait(&sh.ofin[w], 0) || *dead)) {
-            if (lane == 0 && !*dead) raise_error(a.err, kErrMbarTimeout);
-            *dead = 1;
+        if (ok && mine > 0 && __any_sync(0xffffffffu, !mbar_wait(&sh.ofin[w], 0))) {
+            if (lane == 0) raise_error(a.err, kErrMbarTimeout);
             ok = false;
         }
         tc_fence_after();
+        if (half) sh.top[w][row] = l;
+        pair_any(id, false);
         const int64_t all = (int64_t)a.n_seq * a.heads, part = PAIR ? jb.part : 2 * jb.part + w;
         const bool real = r < jb.nr;
         const int64_t at = part * all + (real ? out_row(a, jb.h, jb.r0 + r) : 0);
-        if (real) a.ml[at] = mine > 0 && ok ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+        if (real && half == 0)
+            a.ml[at] = mine > 0 && ok ? make_float2(m, l + sh.top[w][row]) : make_float2(-INFINITY, 0.0f);
         if (ok && mine > 0)
-            for (int c = 0; c < HDP / 32; c++) {
+            for (int c = 0; c < HDP / 64; c++) {
                 uint32_t x[32];
-                tmem_ld32(to + 32 * c, x);
+                const int d = HDP / 2 * half + 32 * c;
+                tmem_ld32(to + d, x);
                 if (real)
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
-                        if (32 * c + k < hd)
-                            *(float4 *)(a.po + at * hd + 32 * c + k) = make_float4(__uint_as_float(x[k]), __uint_as_float(x[k + 1]),
-                                                                               __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+                        if (d + k < hd)
+                            *(float4 *)(a.po + at * hd + d + k) = make_float4(__uint_as_float(x[k]), __uint_as_float(x[k + 1]),
+                                                                              __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
             }
         tc_fence_before();
     }
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "r"(512) : "memory");
     }
 }
 
 template <typename CT, int HDP, bool PAIR>
-int launch_t(const AttnArgs &a, cudaStream_t s) {
+int launch_t(const AttnArgs &a, const CUtensorMap &kmap, const CUtensorMap &vmap, int box, cudaStream_t s) {
     auto fn = attn_tc_kernel<CT, HDP, PAIR>;
     constexpr int smem = smem_bytes<HDP, PAIR>();
+    static_assert(smem + sizeof(Shared) <= 232448, "shared memory of a block");
     QMC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
-    fn<<<(unsigned)jobs, kThreads, smem, s>>>(a);
+    fn<<<(unsigned)jobs, kThreads, smem, s>>>(kmap, vmap, a, box);
     QMC_LAUNCH_CHECK();
     return QMC_OK;
 }
 template <typename CT>
-int launch_h(const AttnArgs &a, cudaStream_t s) {
+int launch_h(const AttnArgs &a, CUtensorMapDataType type, cudaStream_t s) {
+    const int box = attn_tc_box(a.page_size);
+    const int64_t slots = (int64_t)a.n_pages * a.page_size, row = (int64_t)a.kv * a.hd;
+    CUtensorMap kmap, vmap;
+    int rc;
+    if ((rc = make_tensor_map(&kmap, a.kc, type, row, slots, row * 2, 64, box, true)) ||
+        (rc = make_tensor_map(&vmap, a.vc, type, row, slots, row * 2, 64, box, true)))
+        return rc;
     const bool pair = a.rows > kM;
-    if (a.hd <= 64) return pair ? launch_t<CT, 64, true>(a, s) : launch_t<CT, 64, false>(a, s);
-    return pair ? launch_t<CT, 128, true>(a, s) : launch_t<CT, 128, false>(a, s);
+    if (a.hd <= 64) return pair ? launch_t<CT, 64, true>(a, kmap, vmap, box, s) : launch_t<CT, 64, false>(a, kmap, vmap, box, s);
+    return pair ? launch_t<CT, 128, true>(a, kmap, vmap, box, s) : launch_t<CT, 128, false>(a, kmap, vmap, box, s);
 }
 
 }  // namespace
 
+int attn_tc_box(int page_size) { return std::min(kN, page_size & -page_size); }
 int attn_tc_tile(int rows) { return rows > kM ? 2 * kM : kM; }
 int attn_tc_parts(int rows) { return rows > kM ? 1 : 2; }
 
 int launch_attn_tc(const AttnArgs &a, int cdt, cudaStream_t s) {
-    return cdt == QMC_F16 ? launch_h<__half>(a, s) : launch_h<__nv_bfloat16>(a, s);
+    return cdt == QMC_F16 ? launch_h<__half>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s)
+                          : launch_h<__nv_bfloat16>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s);
 }
 
 }  // namespace qmc

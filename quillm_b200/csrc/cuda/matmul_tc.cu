@@ -331,21 +331,6 @@ EncodeTiled encode_fn() {
     });
     return fn;
 }
-// 2-D row-major map: `cols` elements per row, `rows` rows `pitch` bytes apart; boxes of box_cols x
-// box_rows elements, optionally 128-byte swizzled; elements outside the matrix read as zero
-int make_map(CUtensorMap *m, const void *base, CUtensorMapDataType type, int64_t cols, int64_t rows, int64_t pitch,
-             int box_cols, int box_rows, bool swizzle = false) {
-    EncodeTiled fn = encode_fn();
-    if (!fn) return set_error(QMC_ECUDA, "cuTensorMapEncodeTiled is unavailable");
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = fn(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return set_error(QMC_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return QMC_OK;
-}
-
 template <int DT>
 int launch_t(const CUtensorMap &wmap, const CUtensorMap &dwmap, const CUtensorMap &amap, const CUtensorMap &smap,
              const TcParams &p, cudaStream_t s) {
@@ -365,6 +350,21 @@ int launch_t(const CUtensorMap &wmap, const CUtensorMap &dwmap, const CUtensorMa
 
 }  // namespace
 
+// 2-D row-major map: `cols` elements per row, `rows` rows `pitch` bytes apart; boxes of box_cols x
+// box_rows elements, optionally 128-byte swizzled; elements outside the matrix read as zero
+int make_tensor_map(CUtensorMap *m, const void *base, CUtensorMapDataType type, int64_t cols, int64_t rows, int64_t pitch,
+             int box_cols, int box_rows, bool swizzle) {
+    EncodeTiled fn = encode_fn();
+    if (!fn) return set_error(QMC_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = fn(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(QMC_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return QMC_OK;
+}
+
 int64_t matmul_tc_scale_ld(int64_t T) { return (T + 3) / 4 * 4; }
 
 int launch_matmul_q_tc(int dtype, const void *Wsplit, int64_t wstride, const int8_t *aq, const float *adT, float *C,
@@ -382,10 +382,10 @@ int launch_matmul_q_tc(int dtype, const void *Wsplit, int64_t wstride, const int
     CUtensorMap wmap, dwmap, amap, smap;
     const bool q8 = dtype == QMC_Q8_0;
     int rc;
-    if ((rc = make_map(&wmap, Wsplit, CU_TENSOR_MAP_DATA_TYPE_UINT8, wstride, N, wstride, q8 ? 128 : KS * 16, MT, q8)) ||
-        (rc = make_map(&dwmap, Wsplit, CU_TENSOR_MAP_DATA_TYPE_UINT8, wstride, N, wstride, 16, MT)) ||
-        (rc = make_map(&amap, aq, CU_TENSOR_MAP_DATA_TYPE_UINT8, nb * 32, T, nb * 32, 128, NT, true)) ||
-        (rc = make_map(&smap, adT, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, T, nb, matmul_tc_scale_ld(T) * 4, NT, KS)))
+    if ((rc = make_tensor_map(&wmap, Wsplit, CU_TENSOR_MAP_DATA_TYPE_UINT8, wstride, N, wstride, q8 ? 128 : KS * 16, MT, q8)) ||
+        (rc = make_tensor_map(&dwmap, Wsplit, CU_TENSOR_MAP_DATA_TYPE_UINT8, wstride, N, wstride, 16, MT)) ||
+        (rc = make_tensor_map(&amap, aq, CU_TENSOR_MAP_DATA_TYPE_UINT8, nb * 32, T, nb * 32, 128, NT, true)) ||
+        (rc = make_tensor_map(&smap, adT, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, T, nb, matmul_tc_scale_ld(T) * 4, NT, KS)))
         return rc;
     return q8 ? launch_t<QMC_Q8_0>(wmap, dwmap, amap, smap, p, s) : launch_t<QMC_Q4_0>(wmap, dwmap, amap, smap, p, s);
 }
