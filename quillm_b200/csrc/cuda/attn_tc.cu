@@ -59,6 +59,22 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *(const uint32_t *)&h;
 }
+// bounded wait without a suspend-time hint: with one (20 us) waiters here woke up to microseconds late
+__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
+    if (bar_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity))
+        if (clock64() - t0 > kWaitCycles) return false;
+    return true;
+}
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -66,14 +82,16 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int
         : "memory");
 }
 
-// shared-memory operand descriptors, 128-byte swizzle.  K-major (rows of 64 elements, eight-row groups 1024 bytes apart); MN-major
-// (64 elements of M or N a row, eight-row groups of K 1024 bytes apart, the next 64 elements a panel further)
-__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3fffu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// shared-memory operand descriptors, 128-byte swizzle, from the address in 16-byte units.  K-major (rows of 64 elements, eight-row
+// groups 1024 bytes apart); MN-major (64 elements of M or N a row, eight-row groups of K 1024 bytes apart, the next 64
+// elements a panel further).  Only the low word holds an address, so the next operand is an addition to it.
+__device__ __forceinline__ uint64_t desc(uint32_t low) {
+    constexpr uint32_t kHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "n"(kHigh));
+    return d;
 }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3fffu) | ((uint64_t)(128 * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+constexpr uint32_t kLowK = 1u << 16, kLowMN = (uint32_t)(128 * 128 >> 4) << 16;
 // float accumulator, A and B of one 16-bit type; bmn: B is MN-major
 __device__ __forceinline__ constexpr uint32_t idesc(int n, bool bmn, bool bf16) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((bmn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
@@ -100,7 +118,7 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// 32 or 64 consecutive TMEM columns of this thread's lane; the load and its wait are one statement, so that nothing reads the
+// 32 or 16 consecutive TMEM columns of this thread's lane; the load and its wait are one statement, so that nothing reads the
 // registers between the two
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -114,21 +132,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
 }
@@ -190,20 +199,21 @@ __device__ __forceinline__ void ex2_pair(uint64_t t, float &p0, float &p1) {
     p0 = __int_as_float(__float_as_int(v0) + (__float_as_int(u0) << 23));
     p1 = __int_as_float(__float_as_int(v1) + (__float_as_int(u1) << 23));
 }
-// 64 of a row's scores: 2^(scale s - m) as 16-bit pairs over the first 32 registers, their sum before rounding added to `sum`, the
+// 16 of a row's scores: 2^(scale s - m) as 16-bit pairs in pk, their sum before rounding added to `sum`, the
 // largest exponent to `mx`.  The special-function unit gives 16 results a cycle and SM, the products take 4096 flops:
 // three of every eight pairs, spread among the others, go to the FMA pipe instead.  MASK: only the first `left` positions exist
 template <typename CT, bool MASK>
-__device__ __forceinline__ void half_weights(uint32_t (&x)[64], float scale, float m, int left, float (&mx)[2], uint64_t (&sum)[2]) {
+__device__ __forceinline__ void some_weights(const uint32_t (&x)[16], uint32_t *pk, float scale, float m, int left, float (&mx)[2],
+                                             uint64_t (&sum)[2]) {
     constexpr bool BF = __is_same(CT, __nv_bfloat16);
     const uint64_t sc = pair_of(scale, scale), mm = pair_of(-m, -m);
 #pragma unroll
-    for (int k = 0; k < 64; k += 2) {
+    for (int k = 0; k < 16; k += 2) {
         uint64_t t = fma2(pair_of(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sc, mm);
         float t0, t1, p0, p1;
         of_pair(t, t0, t1);
         if (MASK) {
-            const uint32_t live = live_bits(left, k & 32) >> (k & 31);
+            const uint32_t live = live_bits(left, 0) >> k;
             t0 = live & 1u ? t0 : -INFINITY;
             t1 = live & 2u ? t1 : -INFINITY;
         }
@@ -214,7 +224,7 @@ __device__ __forceinline__ void half_weights(uint32_t (&x)[64], float scale, flo
             p0 = ex2(t0), p1 = ex2(t1);
         }
         sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(p0, p1));
-        x[k / 2] = pack2(CT(), p0, p1);
+        pk[k / 2] = pack2(CT(), p0, p1);
     }
 }
 // barrier `id` of two warps: the or of their verdicts
@@ -287,7 +297,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     // all 512 columns are this block's, so they start at 0: S (and P) of stream w at 128 w, O at 256 + HDP w
-    constexpr uint32_t tmem = 0;
 
     if (warp == kCopyWarp) {  // ---------------------------------------------------------------- TMA
         // lane i: box i % groups of the tile's rows, panel i / groups of 64 dimensions
@@ -296,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         int issued = 0;
         auto issue = [&](int row, int left, int u, const CUtensorMap *map) {  // tile u of the sequence K0 V0 K1 V1 ...
             const int at = u % NS, here = min(groups, (left + box - 1) / box);
-            if (u >= NS && __any_sync(0xffffffffu, !mbar_wait(&sh.empty[at], (u / NS - 1) & 1))) {
+            if (u >= NS && __any_sync(0xffffffffu, !bar_wait(&sh.empty[at], (u / NS - 1) & 1))) {
                 if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 return false;
             }
@@ -316,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (!issue(row, left, 2 * j, &kmap) || !issue(row, left, 2 * j + 1, &vmap)) break;
             if (left < kN) {  // the last V tile: zeros behind the range, once its copies have landed
                 const int u = 2 * j + 1, at = u % NS;
-                if (__any_sync(0xffffffffu, !mbar_wait(&sh.full[at], (u / NS) & 1))) {
+                if (__any_sync(0xffffffffu, !bar_wait(&sh.full[at], (u / NS) & 1))) {
                     if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                     break;
                 }
@@ -340,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // of them to the uniform registers that the instruction takes
         const bool lead = elect_one();
         auto wait = [&](uint64_t *bar, uint32_t parity) {
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+            const bool ok = __all_sync(0xffffffffu, bar_wait(bar, parity));
             if (!ok && lane == 0) raise_error(a.err, kErrMbarTimeout);
             return ok;
         };
@@ -349,23 +358,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             return wait(&sh.full[u % NS], (u / NS) & 1);
         };
         auto scores = [&](int w, int j) {  // S_w = Q_w K_j^T
-            const uint32_t q = smq + (PAIR ? w : 0) * TB, k = smk + (2 * j) % NS * TB;
+            const uint32_t q = (smq + (PAIR ? w : 0) * TB) / 16 | kLowK, k = (smk + (2 * j) % NS * TB) / 16 | kLowK;
             if (lead) {
 #pragma unroll
                 for (int i = 0; i < HDP / 16; i++) {
-                    const uint32_t off = (i >> 2) * PANEL + (i & 3) * 32;
-                    mma_ss(128 * w, desc_k(q + off), desc_k(k + off), idesc(kN, false, BF), i > 0);
+                    const uint32_t off = ((i >> 2) * PANEL + (i & 3) * 32) / 16;
+                    mma_ss(128 * w, desc(q + off), desc(k + off), idesc(kN, false, BF), i > 0);
                 }
                 mma_commit(&sh.sfull[w]);
                 if (!PAIR || w == 1) mma_commit(&sh.empty[(2 * j) % NS]);
             }
         };
         auto weigh = [&](int w, int j, bool first) {  // O_w += P_w V_j
-            const uint32_t v = smk + (2 * j + 1) % NS * TB;
+            const uint32_t v = (smk + (2 * j + 1) % NS * TB) / 16 | kLowMN;
             if (lead) {
 #pragma unroll
                 for (int k = 0; k < kN / 16; k++)
-                    mma_ts(256 + HDP * w, 128 * w + 8 * k, desc_mn(v + k * 16 * 128), idesc(HDP, true, BF), !first || k > 0);
+                    mma_ts(256 + HDP * w, 128 * w + 8 * k, desc(v + k * (16 * 128 / 16)), idesc(HDP, true, BF), !first || k > 0);
                 if (!PAIR || w == 1) mma_commit(&sh.empty[(2 * j + 1) % NS]);
             }
         };
@@ -391,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
         // nothing may be in flight when the TMEM is freed
         if (lead) mma_commit(&sh.drain);
-        if (!mbar_wait(&sh.drain, 0) && lane == 0) raise_error(a.err, kErrMbarTimeout);
+        if (!bar_wait(&sh.drain, 0) && lane == 0) raise_error(a.err, kErrMbarTimeout);
         __syncwarp();
     } else {  // ---------------------------------------------------------------- weights
         // warps 8 w + 4 half + q: stream w, rows 32 q .. + 31 (the TMEM lanes a warp may access), half of the columns.  The two
@@ -412,62 +421,68 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         bool ok = true;
         for (int i = 0; i < mine; i++) {
             const int j = PAIR ? i : 2 * i + w, left = jb.p1 - jb.p0 - j * kN - 64 * half;  // of this warp's columns
-            if (ok && __any_sync(0xffffffffu, !mbar_wait(&sh.sfull[w], i & 1u))) {
+            if (ok && __any_sync(0xffffffffu, !bar_wait(&sh.sfull[w], i & 1u))) {
                 if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 ok = false;
             }
             tc_fence_after();
-            uint32_t x[64];
+            uint32_t pk[32];
             if (i == 0) {  // the first reference: the row's largest score
                 float mx = -INFINITY;
                 if (ok) {
-                    tmem_ld64(ts + 64 * half, x);
-                    const uint32_t lo = live_bits(left, 0), hi = live_bits(left, 32);
+#pragma unroll 1
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(ts + 64 * half + 32 * c, x);
+                        const uint32_t live = live_bits(left, 32 * c);
 #pragma unroll
-                    for (int k = 0; k < 64; k++)
-                        mx = fmaxf(mx, (k < 32 ? lo : hi) >> (k & 31) & 1u ? __uint_as_float(x[k]) : -INFINITY);
+                        for (int k = 0; k < 32; k++) mx = fmaxf(mx, live >> k & 1u ? __uint_as_float(x[k]) : -INFINITY);
+                    }
                 }
                 mx = larger(mx);
                 m = mx == -INFINITY ? 0.0f : mx * a.scale;
             }
-            float mx[2] = {-INFINITY, -INFINITY};
-            uint64_t sum[2] = {0, 0};
-            auto weigh = [&]() {
-                if (!ok) return;
-                tmem_ld64(ts + 64 * half, x);
-                if (left >= 64) half_weights<CT, false>(x, a.scale, m, left, mx, sum);
-                else half_weights<CT, true>(x, a.scale, m, left, mx, sum);
-            };
-            weigh();
-            if (pair_any(id, fmaxf(mx[0], mx[1]) > kLift)) {
+            float mx[2];
+            uint64_t sum[2];
+            for (int again = 0;; again++) {
+                mx[0] = mx[1] = -INFINITY, sum[0] = sum[1] = 0;
+                if (ok) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t x[16];
+                        tmem_ld16(ts + 64 * half + 16 * c, x);
+                        if (left >= 64) some_weights<CT, false>(x, pk + 8 * c, a.scale, m, left, mx, sum);
+                        else some_weights<CT, true>(x, pk + 8 * c, a.scale, m, left - 16 * c, mx, sum);
+                    }
+                }
+                // both have read the scores; does a row pass its reference?  After a lift none does
+                if (!pair_any(id, again == 0 && fmaxf(mx[0], mx[1]) > kLift)) break;
                 // lift the references of the two warps' rows and take the scores again; O (half of its columns each) holds
                 // the tiles before this one, whose product is complete (this tile's scores were committed after it)
                 const float up = fmaxf(0.0f, larger(fmaxf(mx[0], mx[1]))), down = ex2(-up);
                 m += up, l *= down;
                 if (ok && i > 0)
+#pragma unroll 1
                     for (int c = 0; c < HDP / 64; c++) {
-                        uint32_t z[32];
-                        tmem_ld32(to + HDP / 2 * half + 32 * c, z);
+                        uint32_t x[32];
+                        tmem_ld32(to + HDP / 2 * half + 32 * c, x);
 #pragma unroll
-                        for (int k = 0; k < 32; k++) z[k] = __float_as_uint(__uint_as_float(z[k]) * down);
-                        tmem_st32(to + HDP / 2 * half + 32 * c, z);
+                        for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * down);
+                        tmem_st32(to + HDP / 2 * half + 32 * c, x);
                     }
-                sum[0] = sum[1] = 0;
-                weigh();
-                pair_any(id, false);  // both have read the scores
             }
             float s0, s1;
             of_pair(add2(sum[0], sum[1]), s0, s1);
             l += s0 + s1;
             if (ok) {
-                tmem_st32(ts + 32 * half, x);
+                tmem_st32(ts + 32 * half, pk);
                 tmem_wait_st();
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.pfull[w]);
         }
-        if (ok && mine > 0 && __any_sync(0xffffffffu, !mbar_wait(&sh.ofin[w], 0))) {
+        if (ok && mine > 0 && __any_sync(0xffffffffu, !bar_wait(&sh.ofin[w], 0))) {
             if (lane == 0) raise_error(a.err, kErrMbarTimeout);
             ok = false;
         }
@@ -480,6 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (real && half == 0)
             a.ml[at] = mine > 0 && ok ? make_float2(m, l + sh.top[w][row]) : make_float2(-INFINITY, 0.0f);
         if (ok && mine > 0)
+#pragma unroll 1
             for (int c = 0; c < HDP / 64; c++) {
                 uint32_t x[32];
                 const int d = HDP / 2 * half + 32 * c;
