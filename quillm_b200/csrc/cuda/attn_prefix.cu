@@ -202,7 +202,7 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
     if (p.tc) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, 128), sms);
     else if (prefix) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, tile), slots);
     if (own) p.osplit = split_for((int64_t)n_seq * kv * p.gtiles, ceil_div(own, tile), slots);
-    p.pparts = p.psplit * (p.tc ? attn_tc_parts(p.rows) : 1);
+    p.pparts = p.psplit;
     const int64_t parts = p.pparts + p.osplit, all = (int64_t)n_seq * n_heads;
     p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;
     p.bytes = p.ml_bytes + parts * all * c->head_dim * 4 + 256;

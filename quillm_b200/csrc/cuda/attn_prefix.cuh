@@ -15,7 +15,7 @@ struct AttnArgs {
     float *po;
     int n_seq, heads, kv, group, hd, page_size, n_pages, ld_table, prefix;
     int rows, ptiles, psplit, gtiles, osplit;
-    int pparts;   // parts that the prefix leaves of each row; the own ones follow
+    int pparts;   // parts that the prefix leaves of each row (psplit of its own launch); the own ones follow
     float scale;  // times log2(e): scores and maxima are exponents of two
 };
 
@@ -73,10 +73,9 @@ int attn_mma_tile(int rows);  // query rows of a prefix job, for `rows` of them 
 int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, cudaStream_t s);
 
 // the tensor-core kernel (attn_tc.cu): the prefix jobs of such a cache with rows of its own type, head_dim <= 128, pages of a
-// multiple of 8 positions and under 2^31 slots, for many rows; a job of up to 128 rows leaves two parts
+// multiple of 8 positions and under 2^31 slots, for many rows
 int attn_tc_box(int page_size);  // positions of one copy
 int attn_tc_tile(int rows);
-int attn_tc_parts(int rows);
 int launch_attn_tc(const AttnArgs &a, int cdt, cudaStream_t s);
 
 }  // namespace qmc

@@ -1,20 +1,18 @@
 // The prefix part of the shared-prefix attention on the 5th-generation tensor cores, for many query rows per KV head:
 // tcgen05.mma with scores and accumulators in tensor memory (TMEM).
 //
-// Per 128 query rows and 128 positions: S = Q K^T (M = 128 rows, N = 128 positions) into 128 TMEM columns; eight warps,
-// two threads per row, turn S into weights P = 2^(scale S - m) and write them over S as 16-bit pairs; O += P V with P
-// read from TMEM as the A operand and V from shared memory as it lies in the cache ([position][dim], an MN-major
-// operand).  A row's reference m moves only when a score passes it by more than 8 (weights stay below 2^8, exact
-// in the split of l and O): then the row's warps rescale their O rows in TMEM and take the tile again, which after a row's first
-// tile is rare, so O normally stays where it is until the end.
+// Per 128 query rows and 128 positions: S = Q K^T (M = 128 rows, N = 128 positions) into 128 TMEM columns; eight warps, two
+// threads per row with 64 positions each, turn S into weights P = 2^(scale S - m) and write them over S as 16-bit pairs;
+// O += P V with P read from TMEM as the A operand and V from shared memory as it lies in the cache ([position][dim], an
+// MN-major operand).  A row's reference m moves only when a thread's weights add up to more than kMost (so each stays below
+// that, exact in the split of l and O): then the row's two warps rescale its O in TMEM and take the tile again, which after
+// a row's first tile is rare, so O normally stays where it is until the end.
 //
-// A block runs two streams of such tiles, so that the tensor cores work on one while the other's warps take its
-// exponentials (16384 of them per tile at 16 a cycle are as long as the tile's two products).  PAIR: the streams are
-// two row tiles over the same positions (each K and V tile is read once for 256 rows).  Otherwise, with at most 128 rows, they
-// take the range's position tiles in turn and leave a part each.
+// A block runs two streams of such tiles, so that the tensor cores work on one while the other's warps take its exponentials.
+// PAIR: the streams are two row tiles over the same positions (each K and V tile is read once for 256 rows).  Otherwise, with
+// at most 128 rows, they take the range's position tiles in turn and are joined at the end.
 //
-// Warps 0-7 and 8-15: the streams' weights, two threads a row with half of the positions each; 16: TMA, a lane for each box of
-// a K or V tile; 17: one lane issues the MMAs.  A box is a run of rows within a page (the largest power of two that divides the
+// Warps 0-15: weights; 16: TMA, a lane for each box of a K or V tile; 17: one lane issues the MMAs.  A box is a run of rows within a page (the largest power of two that divides the
 // page size, 8 to 128 of them) and 64 dimensions wide, the 128-byte swizzle's row.  Dimensions past the head are the next
 // head's, or zeros: for the scores Q has zeros there, in O they are not stored.  Rows past the range, which a box may bring along, are
 // masked in the scores and overwritten with zeros in the last V tile, since what lies there need not be finite.
@@ -30,7 +28,7 @@ namespace {
 
 constexpr int kM = 128, kN = 128;  // rows and positions of a tile
 constexpr int kCopyWarp = 16, kMmaWarp = 17, kThreads = 18 * 32;  // warps 0-15: weights
-constexpr float kLift = 8.0f;      // how far a score may pass its row's reference, in powers of two
+constexpr float kMost = 256.0f;    // that a thread's weights of a tile may add up to
 
 template <int HDP>
 __host__ __device__ constexpr int tile_bytes() {  // of Q, K or V
@@ -58,22 +56,6 @@ __device__ __forceinline__ uint32_t pack2(__half, float x, float y) {
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *(const uint32_t *)&h;
-}
-// bounded wait without a suspend-time hint: with one (20 us) waiters here woke up to microseconds late
-__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok)
-                 : "r"(smem_u32(bar)), "r"(parity)
-                 : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
-    if (bar_try(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!bar_try(bar, parity))
-        if (clock64() - t0 > kWaitCycles) return false;
-    return true;
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile(
@@ -118,7 +100,7 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// 32 or 16 consecutive TMEM columns of this thread's lane; the load and its wait are one statement, so that nothing reads the
+// 32 consecutive TMEM columns of this thread's lane; the load and its wait are one statement, so that nothing reads the
 // registers between the two
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -129,15 +111,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
 }
@@ -199,25 +172,24 @@ __device__ __forceinline__ void ex2_pair(uint64_t t, float &p0, float &p1) {
     p0 = __int_as_float(__float_as_int(v0) + (__float_as_int(u0) << 23));
     p1 = __int_as_float(__float_as_int(v1) + (__float_as_int(u1) << 23));
 }
-// 16 of a row's scores: 2^(scale s - m) as 16-bit pairs in pk, their sum before rounding added to `sum`, the
-// largest exponent to `mx`.  The special-function unit gives 16 results a cycle and SM, the products take 4096 flops:
-// three of every eight pairs, spread among the others, go to the FMA pipe instead.  MASK: only the first `left` positions exist
+// a thread's 32 scores of a row: 2^(scale s - m) as 16-bit pairs in pk, and their sum before rounding.  The special-function unit gives
+// 16 results a cycle and SM: three of every eight pairs, spread among the others, go to the FMA pipe instead.
+// MASK: only the first `left` positions exist
 template <typename CT, bool MASK>
-__device__ __forceinline__ void some_weights(const uint32_t (&x)[16], uint32_t *pk, float scale, float m, int left, float (&mx)[2],
-                                             uint64_t (&sum)[2]) {
+__device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *pk, float scale, float m, int left) {
     constexpr bool BF = __is_same(CT, __nv_bfloat16);
     const uint64_t sc = pair_of(scale, scale), mm = pair_of(-m, -m);
+    const uint32_t live = MASK ? live_bits(left, 0) : 0xffffffffu;
+    uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 16; k += 2) {
-        uint64_t t = fma2(pair_of(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sc, mm);
+    for (int k = 0; k < 32; k += 2) {
+        const uint64_t t = fma2(pair_of(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sc, mm);
         float t0, t1, p0, p1;
         of_pair(t, t0, t1);
         if (MASK) {
-            const uint32_t live = live_bits(left, 0) >> k;
-            t0 = live & 1u ? t0 : -INFINITY;
-            t1 = live & 2u ? t1 : -INFINITY;
+            t0 = live >> k & 1u ? t0 : -INFINITY;
+            t1 = live >> (k + 1) & 1u ? t1 : -INFINITY;
         }
-        mx[(k >> 1) & 1] = fmaxf(mx[(k >> 1) & 1], fmaxf(t0, t1));
         if (!MASK && (k >> 1) % 8 % 3 == 1) {
             ex2_pair<BF>(pair_of(fmaxf(t0, -126.0f), fmaxf(t1, -126.0f)), p0, p1);
         } else {
@@ -226,9 +198,12 @@ __device__ __forceinline__ void some_weights(const uint32_t (&x)[16], uint32_t *
         sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(p0, p1));
         pk[k / 2] = pack2(CT(), p0, p1);
     }
+    float s0, s1;
+    of_pair(add2(sum[0], sum[1]), s0, s1);
+    return s0 + s1;
 }
-// barrier `id` of two warps: the or of their verdicts
-__device__ __forceinline__ bool pair_any(int id, bool v) {
+// barrier `id` of the two warps of 32 rows: the or of their verdicts
+__device__ __forceinline__ bool rows_any(int id, bool v) {
     int r;
     asm volatile(
         "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 64, p;\n selp.s32 %0, 1, 0, q;\n}\n"
@@ -237,10 +212,9 @@ __device__ __forceinline__ bool pair_any(int id, bool v) {
         : "memory");
     return r != 0;
 }
-
 struct Shared {
-    uint64_t full[6], empty[6], sfull[2], pfull[2], ofin[2], vlast, drain;
-    float top[2][kM];  // what a row's two threads exchange
+    uint64_t full[6], empty[6], sfull[2], pfull[2], ofin[2], qready, vlast, drain;
+    float top[2][kM];  // the larger of a row's two threads
     uint32_t tmem;
 };
 
@@ -266,9 +240,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.pfull[i], 8);    // the stream's warps
+            mbar_init(&sh.pfull[i], 8);  // the stream's warps
             mbar_init(&sh.ofin[i], 1);
         }
+        mbar_init(&sh.qready, 32 * kCopyWarp);
         mbar_init(&sh.vlast, 1);
         mbar_init(&sh.drain, 1);
         fence_mbar_init();
@@ -277,25 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp < kCopyWarp) {  // the query tiles; rows past the last and chunks past the head are zeros
-        const bool vec = a.ldq % 8 == 0 && (uintptr_t)a.q % 16 == 0;
-        for (int i = tid; i < (PAIR ? 2 : 1) * kM * CH; i += 32 * kCopyWarp) {
-            const int r = i / CH, c = i % CH, rr = jb.r0 + r;
-            alignas(16) CT e[8];
-            *(uint4 *)e = make_uint4(0, 0, 0, 0);
-            if (r < jb.nr && c < nch) {
-                const CT *src = (const CT *)a.q + (rr / a.group) * a.ldq + (int64_t)(jb.h * a.group + rr % a.group) * hd + 8 * c;
-                if (vec) *(uint4 *)e = *(const uint4 *)src;
-                else
-                    for (int k = 0; k < 8; k++) e[k] = src[k];
-            }
-            *(uint4 *)(base + (r / kM) * TB + place(r % kM, c)) = *(const uint4 *)e;
-        }
-    }
-    fence_proxy_async();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    __syncthreads();  // the barriers
     // all 512 columns are this block's, so they start at 0: S (and P) of stream w at 128 w, O at 256 + HDP w
 
     if (warp == kCopyWarp) {  // ---------------------------------------------------------------- TMA
@@ -305,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         int issued = 0;
         auto issue = [&](int row, int left, int u, const CUtensorMap *map) {  // tile u of the sequence K0 V0 K1 V1 ...
             const int at = u % NS, here = min(groups, (left + box - 1) / box);
-            if (u >= NS && __any_sync(0xffffffffu, !bar_wait(&sh.empty[at], (u / NS - 1) & 1))) {
+            if (u >= NS && __any_sync(0xffffffffu, !mbar_wait(&sh.empty[at], (u / NS - 1) & 1))) {
                 if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 return false;
             }
@@ -325,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (!issue(row, left, 2 * j, &kmap) || !issue(row, left, 2 * j + 1, &vmap)) break;
             if (left < kN) {  // the last V tile: zeros behind the range, once its copies have landed
                 const int u = 2 * j + 1, at = u % NS;
-                if (__any_sync(0xffffffffu, !bar_wait(&sh.full[at], (u / NS) & 1))) {
+                if (__any_sync(0xffffffffu, !mbar_wait(&sh.full[at], (u / NS) & 1))) {
                     if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                     break;
                 }
@@ -349,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // of them to the uniform registers that the instruction takes
         const bool lead = elect_one();
         auto wait = [&](uint64_t *bar, uint32_t parity) {
-            const bool ok = __all_sync(0xffffffffu, bar_wait(bar, parity));
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
             if (!ok && lane == 0) raise_error(a.err, kErrMbarTimeout);
             return ok;
         };
@@ -379,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
         };
         constexpr int step = PAIR ? 1 : 2;  // tiles from one of a stream's to its next
-        bool ok = true;
+        bool ok = wait(&sh.qready, 0);
         for (int w = 0; w < 2 && ok; w++) {
             const int j = PAIR ? 0 : w;
             if (j < ntile && (ok = tile(2 * j))) scores(w, j);
@@ -400,80 +357,95 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
         // nothing may be in flight when the TMEM is freed
         if (lead) mma_commit(&sh.drain);
-        if (!bar_wait(&sh.drain, 0) && lane == 0) raise_error(a.err, kErrMbarTimeout);
+        if (!mbar_wait(&sh.drain, 0) && lane == 0) raise_error(a.err, kErrMbarTimeout);
         __syncwarp();
     } else {  // ---------------------------------------------------------------- weights
-        // warps 8 w + 4 half + q: stream w, rows 32 q .. + 31 (the TMEM lanes a warp may access), half of the columns.  The two
-        // warps of a row meet once a tile: before either writes weights over scores that the other reads, and to
+        // the query tiles first; rows past the last and chunks past the head are zeros
+        const bool vec = a.ldq % 8 == 0 && (uintptr_t)a.q % 16 == 0;
+        for (int i = tid; i < (PAIR ? 2 : 1) * kM * CH; i += 32 * kCopyWarp) {
+            const int r = i / CH, c = i % CH, rr = jb.r0 + r;
+            alignas(16) CT e[8];
+            *(uint4 *)e = make_uint4(0, 0, 0, 0);
+            if (r < jb.nr && c < nch) {
+                const CT *src = (const CT *)a.q + (rr / a.group) * a.ldq + (int64_t)(jb.h * a.group + rr % a.group) * hd + 8 * c;
+                if (vec) *(uint4 *)e = *(const uint4 *)src;
+                else
+                    for (int k = 0; k < 8; k++) e[k] = src[k];
+            }
+            *(uint4 *)(base + (r / kM) * TB + place(r % kM, c)) = *(const uint4 *)e;
+        }
+        fence_proxy_async();
+        mbar_arrive(&sh.qready);
+
+        // warp 8 w + 4 half + q: stream w, rows 32 q .. + 31 (the TMEM lanes it may access), half of the positions of each tile.
+        // The two warps of a row meet once a tile: before either writes weights over scores that the other reads, and to
         // agree on the row's reference.  A warp whose wait has expired goes on through the barriers without touching TMEM.
-        const int w = warp >> 3, half = (warp >> 2) & 1, row = 32 * (warp & 3) + lane, r = (PAIR ? w * kM : 0) + row;
-        const int id = 1 + 4 * w + (warp & 3);
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = lanes + 128 * w, to = lanes + 256 + HDP * w;
+        const int w = warp >> 3, half = (warp >> 2) & 1, row = 32 * (warp & 3) + lane, id = 1 + 4 * w + (warp & 3);
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = lanes + 128 * w, to = lanes + 256 + HDP * w + HDP / 2 * half;
         const int mine = PAIR ? ntile : (ntile - w + 1) / 2;
-        auto larger = [&](float v) {  // of the row's two values, in both threads
-            if (half) sh.top[w][row] = v;
-            pair_any(id, false);
-            if (!half) sh.top[w][row] = v = fmaxf(v, sh.top[w][row]);
-            pair_any(id, false);
-            return half ? sh.top[w][row] : v;
+        auto largest = [&](float v) {
+            rows_any(id, false);  // both have read what it held
+            if (half == 0) sh.top[w][row] = v;
+            rows_any(id, false);
+            if (half == 1) sh.top[w][row] = v = fmaxf(v, sh.top[w][row]);
+            rows_any(id, false);
+            return sh.top[w][row];
         };
         float m = 0.0f, l = 0.0f;
         bool ok = true;
         for (int i = 0; i < mine; i++) {
-            const int j = PAIR ? i : 2 * i + w, left = jb.p1 - jb.p0 - j * kN - 64 * half;  // of this warp's columns
-            if (ok && __any_sync(0xffffffffu, !bar_wait(&sh.sfull[w], i & 1u))) {
+            const int j = PAIR ? i : 2 * i + w, left = jb.p1 - jb.p0 - j * kN - 64 * half;  // of this thread's positions
+            if (ok && __any_sync(0xffffffffu, !mbar_wait(&sh.sfull[w], i & 1u))) {
                 if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 ok = false;
             }
             tc_fence_after();
             uint32_t pk[32];
-            if (i == 0) {  // the first reference: the row's largest score
-                float mx = -INFINITY;
-                if (ok) {
+            float sum = 0.0f;
+            for (int again = i == 0 ? -1 : 0;; again++) {  // -1: no reference yet
+                if (ok && again >= 0) {
+                    sum = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t x[32];
+                        tmem_ld32(ts + 64 * half + 32 * c, x);
+                        sum += left >= 64 ? row_weights<CT, false>(x, pk + 16 * c, a.scale, m, left)
+                                          : row_weights<CT, true>(x, pk + 16 * c, a.scale, m, left - 32 * c);
+                    }
+                }
+                // both have read the scores; does a row pass its reference?  After a lift none does
+                if (!rows_any(id, again < 0 || (again == 0 && i > 0 && !(sum <= kMost)))) break;
+                // the reference becomes the row's largest score, if that is above it
+                float top = -INFINITY;
+                if (ok)
 #pragma unroll 1
                     for (int c = 0; c < 2; c++) {
                         uint32_t x[32];
                         tmem_ld32(ts + 64 * half + 32 * c, x);
                         const uint32_t live = live_bits(left, 32 * c);
 #pragma unroll
-                        for (int k = 0; k < 32; k++) mx = fmaxf(mx, live >> k & 1u ? __uint_as_float(x[k]) : -INFINITY);
+                        for (int k = 0; k < 32; k++) top = fmaxf(top, live >> k & 1u ? __uint_as_float(x[k]) : -INFINITY);
                     }
+                top = largest(top) * a.scale;
+                if (again < 0) {
+                    m = top == -INFINITY ? 0.0f : top;
+                    continue;
                 }
-                mx = larger(mx);
-                m = mx == -INFINITY ? 0.0f : mx * a.scale;
-            }
-            float mx[2];
-            uint64_t sum[2];
-            for (int again = 0;; again++) {
-                mx[0] = mx[1] = -INFINITY, sum[0] = sum[1] = 0;
-                if (ok) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t x[16];
-                        tmem_ld16(ts + 64 * half + 16 * c, x);
-                        if (left >= 64) some_weights<CT, false>(x, pk + 8 * c, a.scale, m, left, mx, sum);
-                        else some_weights<CT, true>(x, pk + 8 * c, a.scale, m, left - 16 * c, mx, sum);
-                    }
-                }
-                // both have read the scores; does a row pass its reference?  After a lift none does
-                if (!pair_any(id, again == 0 && fmaxf(mx[0], mx[1]) > kLift)) break;
-                // lift the references of the two warps' rows and take the scores again; O (half of its columns each) holds
-                // the tiles before this one, whose product is complete (this tile's scores were committed after it)
-                const float up = fmaxf(0.0f, larger(fmaxf(mx[0], mx[1]))), down = ex2(-up);
-                m += up, l *= down;
-                if (ok && i > 0)
+                // O (half of its columns each) holds the tiles before this one, whose product is complete (this tile's scores
+                // were committed after it)
+                const float to_m = fmaxf(m, top), down = ex2(m - to_m);
+                m = to_m, l *= down;
+                if (ok)
 #pragma unroll 1
                     for (int c = 0; c < HDP / 64; c++) {
                         uint32_t x[32];
-                        tmem_ld32(to + HDP / 2 * half + 32 * c, x);
+                        tmem_ld32(to + 32 * c, x);
 #pragma unroll
                         for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * down);
-                        tmem_st32(to + HDP / 2 * half + 32 * c, x);
+                        tmem_st32(to + 32 * c, x);
                     }
             }
-            float s0, s1;
-            of_pair(add2(sum[0], sum[1]), s0, s1);
-            l += s0 + s1;
+            l += sum;
             if (ok) {
                 tmem_st32(ts + 32 * half, pk);
                 tmem_wait_st();
@@ -482,31 +454,58 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.pfull[w]);
         }
-        if (ok && mine > 0 && __any_sync(0xffffffffu, !bar_wait(&sh.ofin[w], 0))) {
+        if (ok && mine > 0 && __any_sync(0xffffffffu, !mbar_wait(&sh.ofin[w], 0))) {
             if (lane == 0) raise_error(a.err, kErrMbarTimeout);
             ok = false;
         }
         tc_fence_after();
-        if (half) sh.top[w][row] = l;
-        pair_any(id, false);
-        const int64_t all = (int64_t)a.n_seq * a.heads, part = PAIR ? jb.part : 2 * jb.part + w;
-        const bool real = r < jb.nr;
-        const int64_t at = part * all + (real ? out_row(a, jb.h, jb.r0 + r) : 0);
-        if (real && half == 0)
-            a.ml[at] = mine > 0 && ok ? make_float2(m, l + sh.top[w][row]) : make_float2(-INFINITY, 0.0f);
-        if (ok && mine > 0)
+        // The last products of both streams are complete, so the ring is free: m and l of the rows, and O, so that it leaves in
+        // whole lines.  16-byte chunk c of row r lies at c ^ (r & 7).
+        asm volatile("bar.sync 9, 512;" ::: "memory");
+        float *const ml = (float *)(base + (smk - smq));  // [stream][m, l of either half][row]
+        uint8_t *const rows = (uint8_t *)(ml + 2 * 3 * kM), *const own = rows + w * (kM * HDP * 4);
+        if (half == 0) ml[3 * w * kM + row] = mine > 0 && ok ? m : -INFINITY;
+        ml[(3 * w + 1 + half) * kM + row] = mine > 0 && ok ? l : 0.0f;
 #pragma unroll 1
-            for (int c = 0; c < HDP / 64; c++) {
-                uint32_t x[32];
-                const int d = HDP / 2 * half + 32 * c;
-                tmem_ld32(to + d, x);
-                if (real)
+        for (int c = 0; c < HDP / 64; c++) {
+            uint32_t x[32];
+            if (ok && mine > 0) {
+                tmem_ld32(to + 32 * c, x);
+            } else {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        if (d + k < hd)
-                            *(float4 *)(a.po + at * hd + d + k) = make_float4(__uint_as_float(x[k]), __uint_as_float(x[k + 1]),
-                                                                              __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+                for (int k = 0; k < 32; k++) x[k] = 0;
             }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                *(uint4 *)(own + row * (HDP * 4) + (((HDP / 8 * half + 8 * c + k) ^ (row & 7)) << 4)) =
+                    make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        }
+        asm volatile("bar.sync 9, 512;" ::: "memory");
+        const int64_t all = (int64_t)a.n_seq * a.heads;
+        constexpr int RW = (PAIR ? 2 : 1) * kM / 16;  // rows a warp stores
+        for (int k = 0; k < RW; k++) {
+            const int r = RW * warp + k, rr = r % kM, s = PAIR ? r / kM : 0;
+            if (r >= jb.nr) break;
+            const int64_t at = jb.part * all + out_row(a, jb.h, jb.r0 + r);
+            const float *h = ml + 3 * s * kM + rr;
+            float M = h[0], L = h[kM] + h[2 * kM], c0 = 1.0f, c1 = 0.0f;
+            if (!PAIR) {  // the two streams' parts of the row as one
+                const float m0 = M, m1 = h[3 * kM];
+                M = fmaxf(m0, m1);
+                if (M > -INFINITY) c0 = ex2(m0 - M), c1 = ex2(m1 - M);
+                L = L * c0 + (h[4 * kM] + h[5 * kM]) * c1;
+            }
+            if (lane == 0) a.ml[at] = make_float2(M, L);
+            if (4 * lane < hd) {
+                const int o = rr * (HDP * 4) + ((lane ^ (rr & 7)) << 4);
+                float4 v = *(const float4 *)(rows + s * (kM * HDP * 4) + o);
+                if (!PAIR) {
+                    const float4 u = *(const float4 *)(rows + kM * HDP * 4 + o);
+                    v = make_float4(v.x * c0 + u.x * c1, v.y * c0 + u.y * c1, v.z * c0 + u.z * c1, v.w * c0 + u.w * c1);
+                }
+                *(float4 *)(a.po + at * hd + 4 * lane) = v;
+            }
+        }
         tc_fence_before();
     }
     __syncthreads();
@@ -546,7 +545,6 @@ int launch_h(const AttnArgs &a, CUtensorMapDataType type, cudaStream_t s) {
 
 int attn_tc_box(int page_size) { return std::min(kN, page_size & -page_size); }
 int attn_tc_tile(int rows) { return rows > kM ? 2 * kM : kM; }
-int attn_tc_parts(int rows) { return rows > kM ? 1 : 2; }
 
 int launch_attn_tc(const AttnArgs &a, int cdt, cudaStream_t s) {
     return cdt == QMC_F16 ? launch_h<__half>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s)
