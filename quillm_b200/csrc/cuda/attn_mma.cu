@@ -339,44 +339,44 @@ __global__ void __launch_bounds__(128) attn_mma_kernel(const AttnArgs a) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ Scratch sc;
     const Job jb = job_of(a, blockIdx.x, 16 * WM, 16, kTP);
+    pdl_launch_dependents();
     if (WM > 1 && jb.b < 0) mma_job<T, CT, HDP, WM>(a, jb, sm, sc);
     else mma_job<T, CT, HDP, 1>(a, jb, sm, sc);
+    pdl_wait();  // launched beside the prefix's kernel, this one ends after it: the join waits for this one
 }
 
 template <typename T, typename CT, int HDP, int WM>
-int launch_t(const AttnArgs &a, cudaStream_t s) {
+int launch_t(const AttnArgs &a, bool after, cudaStream_t s) {
     auto fn = attn_mma_kernel<T, CT, HDP, WM>;
     constexpr int smem = smem_bytes<HDP, 16 * WM, sizeof(T) == 4>();
     static_assert(4 * 16 * HDP * 4 <= stages<HDP>() * stage_bytes<HDP>(), "the join fits the ring");
     QMC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
-    if (jobs) fn<<<(unsigned)jobs, 128, smem, s>>>(a);
-    QMC_LAUNCH_CHECK();
-    return QMC_OK;
+    return jobs ? launch_after(fn, dim3((unsigned)jobs), 128, smem, s, after, a) : QMC_OK;
 }
 template <typename T, typename CT, int HDP>
-int launch_m(const AttnArgs &a, cudaStream_t s) {
+int launch_m(const AttnArgs &a, bool after, cudaStream_t s) {
     switch (attn_mma_tile(a.rows)) {
-        case 16: return launch_t<T, CT, HDP, 1>(a, s);
-        case 32: return launch_t<T, CT, HDP, 2>(a, s);
-        default: return launch_t<T, CT, HDP, 4>(a, s);
+        case 16: return launch_t<T, CT, HDP, 1>(a, after, s);
+        case 32: return launch_t<T, CT, HDP, 2>(a, after, s);
+        default: return launch_t<T, CT, HDP, 4>(a, after, s);
     }
 }
 template <typename T, typename CT>
-int launch_h(const AttnArgs &a, cudaStream_t s) {
-    if (a.hd <= 64) return launch_m<T, CT, 64>(a, s);
-    if (a.hd <= 128) return launch_m<T, CT, 128>(a, s);
-    return launch_m<T, CT, 256>(a, s);
+int launch_h(const AttnArgs &a, bool after, cudaStream_t s) {
+    if (a.hd <= 64) return launch_m<T, CT, 64>(a, after, s);
+    if (a.hd <= 128) return launch_m<T, CT, 128>(a, after, s);
+    return launch_m<T, CT, 256>(a, after, s);
 }
 
 }  // namespace
 
 int attn_mma_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, cudaStream_t s) {
-    if (dtype == QMC_F32) return launch_h<float, __half>(a, s);
-    return cdt == QMC_F16 ? launch_h<__half, __half>(a, s) : launch_h<__nv_bfloat16, __nv_bfloat16>(a, s);
+int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, bool after, cudaStream_t s) {
+    if (dtype == QMC_F32) return launch_h<float, __half>(a, after, s);
+    return cdt == QMC_F16 ? launch_h<__half, __half>(a, after, s) : launch_h<__nv_bfloat16, __nv_bfloat16>(a, after, s);
 }
 
 }  // namespace qmc

@@ -14,11 +14,13 @@
 namespace qmc {
 namespace {
 
+enum { kRowsKernel, kWarpKernel, kMmaKernel, kTcKernel };
+
 struct Plan {
     int rows;                 // query rows of a KV head over the whole batch: n_seq * group
     int ptiles, psplit;       // prefix: row tiles and position ranges
     int gtiles, osplit;       // own positions: row tiles of a group and position ranges
-    bool mma, tc;             // matrix instructions; tensor memory for the prefix
+    int pkind, okind;         // the kernels of the prefix and of own positions
     int pparts;
     int64_t ml_bytes, bytes;  // workspace: [parts][n_seq * n_heads] float2 (m, l), then [parts][...][hd] floats
 };
@@ -39,6 +41,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
     __shared__ int64_t slot_s[kPT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Job jb = job_of(a, blockIdx.x, kQR, kQR, kPT);
+    pdl_launch_dependents();
     for (int i = tid; i < kQR * hd4; i += 128) {
         const int r = i / hd4, d = i % hd4, rr = jb.r0 + r;
         Qs[i] = (r < jb.nr && d < hd)
@@ -135,35 +138,61 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
     }
 }
 
-// joins the parts of a row, one warp each
-template <typename T>
+// joins the parts of a row, one warp each: lane j takes part j's factor 2^(m_j - M), then every lane V of the row's dimensions (twice
+// above 128, as many times as needed one by one) over the parts, whose loads do not wait for one another
+template <typename T, int V>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int parts) {
     const int lane = threadIdx.x & 31;
     const int64_t all = (int64_t)a.n_seq * a.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    pdl_wait();
     if (row >= all) return;
     const int b = (int)(row / a.heads), h = (int)(row % a.heads), n = a.lens[b];
     if (lane == 0 && ((n != 0 && n < a.prefix) || n > (int64_t)a.ld_table * a.page_size)) raise_error(a.err, kErrBadIndex);
-    float M = -INFINITY;
-    if (n > 0)
-        for (int j = lane; j < parts; j += 32) M = fmaxf(M, a.ml[j * all + row].x);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;  // dimension lane + 32 i
-    if (n > 0)
-        for (int j = 0; j < parts; j++) {
-            const float2 ml = a.ml[j * all + row];
-            if (ml.y == 0.0f) continue;
-            const float w = exp2f(ml.x - ref);
-            l = fmaf(w, ml.y, l);
+    constexpr int NV = 256 / 32 / V;
+    float o[NV][V], l = 0.0f, M = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (lane + 32 * i < a.hd) o[i] = fmaf(w, a.po[(j * all + row) * a.hd + lane + 32 * i], o[i]);
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) o[i][k] = 0.0f;
+    if (n > 0) {
+        for (int j = lane; j < parts; j += 32) M = fmaxf(M, a.ml[j * all + row].x);
+        M = warp_max(M);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        for (int j0 = 0; j0 < parts; j0 += 32) {
+            float w = 0.0f;  // of part j0 + lane; one without weights is not read
+            if (j0 + lane < parts) {
+                const float2 ml = a.ml[(j0 + lane) * all + row];
+                if (ml.y != 0.0f) w = exp2f(ml.x - ref), l = fmaf(w, ml.y, l);
+            }
+            const int here = min(32, parts - j0);
+#pragma unroll 8
+            for (int j = 0; j < here; j++) {
+                const float wj = __shfl_sync(0xffffffffu, w, j);
+                const bool live = wj != 0.0f;  // NaN included
+                const float *src = a.po + ((j0 + j) * all + row) * a.hd;
+#pragma unroll
+                for (int i = 0; i < NV; i++) {
+                    const int d = V * (lane + 32 * i);
+                    float v[V];
+#pragma unroll
+                    for (int k = 0; k < V; k++) v[k] = 0.0f;
+                    if (live && d < a.hd) load_chunk<float, V>(src + d, v);
+#pragma unroll
+                    for (int k = 0; k < V; k++) o[i][k] = fmaf(wj, v[k], o[i][k]);
+                }
+            }
         }
+        l = warp_sum(l);
+    }
     const float rl = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);  // an empty row gives zeros
     T *out = (T *)a.out + b * a.ldo + (int64_t)h * a.hd;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (lane + 32 * i < a.hd) from_f32(o[i] * rl, &out[lane + 32 * i]);
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int d = V * (lane + 32 * i) + k;
+            if (d < a.hd) from_f32(o[i][k] * rl, &out[d]);
+        }
 }
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -175,7 +204,7 @@ bool takes_mma(const qmc_paged_cache *c) {
 
 // position ranges for each of `units` row tiles over `tiles` position tiles, `slots` blocks running at once: the number with
 // the fewest rounds of tiles, a block costing kBlockTiles more for its start, its end and its parts' way through memory
-constexpr int kBlockTiles = 3, kMostSplits = 64, kTcRows = 64;
+constexpr int kBlockTiles = 3, kMostSplits = 64;
 int split_for(int64_t units, int tiles, int slots) {
     int best = 1;
     int64_t least = INT64_MAX;
@@ -191,17 +220,21 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
     const int group = n_heads / c->n_kv_heads, kv = c->n_kv_heads;
     const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix);
     p.rows = n_seq * group;
-    p.mma = takes_mma(c);
-    p.tc = p.mma && dtype == c->dtype && c->head_dim <= 128 && p.rows > kTcRows && prefix &&
-           c->page_size % 8 == 0 &&
-           (int64_t)c->n_pages * c->page_size <= INT32_MAX;
-    const int tile = p.mma ? 64 : kPT;                 // positions
-    const int slots = (p.mma ? 2 : 4) * sms;           // blocks that run at once
-    p.gtiles = ceil_div(group, p.mma ? 16 : kQR);
-    p.ptiles = ceil_div(p.rows, p.tc ? attn_tc_tile(p.rows) : p.mma ? attn_mma_tile(p.rows) : kQR);
-    if (p.tc) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, 128), sms);
-    else if (prefix) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, tile), slots);
-    if (own) p.osplit = split_for((int64_t)n_seq * kv * p.gtiles, ceil_div(own, tile), slots);
+    const bool mma = takes_mma(c), narrow = mma && c->head_dim <= 128;
+    p.okind = narrow ? kWarpKernel : mma ? kMmaKernel : kRowsKernel;
+    p.pkind = p.okind;
+    if (narrow && p.rows > kWarpRows)
+        p.pkind = dtype == c->dtype && c->page_size % 8 == 0 && (int64_t)c->n_pages * c->page_size <= INT32_MAX ? kTcKernel : kMmaKernel;
+    struct Shape {
+        int ptile, otile, quantum, blocks;  // rows of a prefix and of an own job, positions of a tile, blocks an SM runs at once
+    };
+    const Shape shape[4] = {{kQR, kQR, kPT, 4}, {kWarpRows, kWarpRows, 64, 2}, {attn_mma_tile(p.rows), 16, 64, 2},
+                            {attn_tc_tile(p.rows), 0, 128, 1}};
+    const Shape &ps = shape[p.pkind], &os = shape[p.okind];
+    p.ptiles = ceil_div(p.rows, ps.ptile);
+    p.gtiles = ceil_div(group, os.otile);
+    if (prefix) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, ps.quantum), ps.blocks * sms);
+    if (own) p.osplit = split_for((int64_t)n_seq * kv * p.gtiles, ceil_div(own, os.quantum), os.blocks * sms);
     p.pparts = p.psplit;
     const int64_t parts = p.pparts + p.osplit, all = (int64_t)n_seq * n_heads;
     p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;
@@ -224,23 +257,30 @@ template <typename T, typename CT>
 int launch_attn(const AttnArgs &a, const Plan &p, int dtype, int cdt, cudaStream_t s) {
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
-    int rc = QMC_OK;
-    if (p.tc) {
-        AttnArgs own = a;
-        own.psplit = 0;  // own positions only
-        if (!(rc = launch_attn_tc(a, cdt, s)) && a.osplit) rc = launch_attn_mma(own, dtype, cdt, s);
-    } else if (jobs && p.mma) {
-        rc = launch_attn_mma(a, dtype, cdt, s);
-    } else if (jobs) {
+    auto launch = [&](int kind, const AttnArgs &x, bool after) {
+        if (kind == kTcKernel) return launch_attn_tc(x, cdt, s);
+        if (kind == kMmaKernel) return launch_attn_mma(x, dtype, cdt, after, s);
+        if (kind == kWarpKernel) return launch_attn_warp(x, dtype, cdt, after, s);
+        const int64_t n = (int64_t)x.kv * x.ptiles * x.psplit + (int64_t)x.n_seq * x.kv * x.gtiles * x.osplit;
         const size_t al = 4 * sizeof(CT);
-        const bool vec = a.hd % 4 == 0 && (uintptr_t)a.kc % al == 0 && (uintptr_t)a.vc % al == 0;
-        rc = a.hd <= 128 ? launch_rows<T, CT, 1>(a, jobs, vec, s) : launch_rows<T, CT, 2>(a, jobs, vec, s);
+        const bool vec = x.hd % 4 == 0 && (uintptr_t)x.kc % al == 0 && (uintptr_t)x.vc % al == 0;
+        return x.hd <= 128 ? launch_rows<T, CT, 1>(x, n, vec, s) : launch_rows<T, CT, 2>(x, n, vec, s);
+    };
+    int rc = QMC_OK;
+    if (jobs && p.pkind == p.okind) {
+        rc = launch(p.okind, a, false);
+    } else if (jobs) {  // own positions beside the prefix: their blocks take the SMs that the other's leave
+        AttnArgs first = a, second = a;
+        first.osplit = 0, second.psplit = 0;
+        if (a.psplit) rc = launch(p.pkind, first, false);
+        if (!rc && a.osplit) rc = launch(p.okind, second, a.psplit > 0);
     }
     if (rc) return rc;
+    // the join may start while the last parts are written; it waits for them before it reads
     const int64_t all = (int64_t)a.n_seq * a.heads;
-    attn_join_kernel<T><<<(unsigned)((all + 3) / 4), 128, 0, s>>>(a, a.pparts + a.osplit);
-    QMC_LAUNCH_CHECK();
-    return QMC_OK;
+    const dim3 grid((unsigned)((all + 3) / 4));
+    if (a.hd % 4 == 0) return launch_after(attn_join_kernel<T, 4>, grid, 128, 0, s, jobs > 0, a, a.pparts + a.osplit);
+    return launch_after(attn_join_kernel<T, 1>, grid, 128, 0, s, jobs > 0, a, a.pparts + a.osplit);
 }
 
 int check_attn(const char *op, int dtype, const qmc_paged_cache *c, int n_seq, int n_heads, int prefix, int ld_table) {

@@ -68,9 +68,27 @@ __device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
     return (int64_t)(r / a.group) * a.heads + h * a.group + r % a.group;
 }
 
+// a launch that may start before the kernel before it in the stream has ended (`after`); the kernel calls pdl_wait
+template <typename... A>
+int launch_after(void (*fn)(A...), dim3 grid, int threads, int smem, cudaStream_t s, bool after, A... args) {
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = s;
+    c.attrs = attr, c.numAttrs = after ? 1 : 0;
+    QMC_CUDA(cudaLaunchKernelEx(&c, fn, args...));
+    return QMC_OK;
+}
+
 // the matrix-instruction kernel (attn_mma.cu), for 16-bit caches whose rows are whole 16-byte chunks
 int attn_mma_tile(int rows);  // query rows of a prefix job, for `rows` of them per KV head; own jobs take 16
-int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, cudaStream_t s);
+// after: the kernel may start before the one before it in the stream has ended, and ends after it
+int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, bool after, cudaStream_t s);
+
+// up to 16 rows a tile, straight from global memory into the matrix instructions (attn_warp.cu): such caches with head_dim <= 128
+constexpr int kWarpRows = 16;
+int launch_attn_warp(const AttnArgs &a, int dtype, int cdt, bool after, cudaStream_t s);
 
 // the tensor-core kernel (attn_tc.cu): the prefix jobs of such a cache with rows of its own type, head_dim <= 128, pages of a
 // multiple of 8 positions and under 2^31 slots, for many rows

@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     __syncthreads();  // the barriers
+    pdl_launch_dependents();
     // all 512 columns are this block's, so they start at 0: S (and P) of stream w at 128 w, O at 256 + HDP w
 
     if (warp == kCopyWarp) {  // ---------------------------------------------------------------- TMA
