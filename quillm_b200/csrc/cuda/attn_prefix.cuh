@@ -68,6 +68,19 @@ __device__ __forceinline__ int64_t out_row(const AttnArgs &a, int h, int r) {
     return (int64_t)(r / a.group) * a.heads + h * a.group + r % a.group;
 }
 
+// the kernel's dynamic shared memory limit, raised once per device
+template <typename F>
+int raise_smem(F fn, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    QMC_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return set_error(QMC_EINVAL, "attn_prefix: device %d out of range", dev);
+    if (!done[dev]) {
+        QMC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done[dev] = true;
+    }
+    return QMC_OK;
+}
+
 // a launch that may start before the kernel before it in the stream has ended (`after`); the kernel calls pdl_wait
 template <typename... A>
 int launch_after(void (*fn)(A...), dim3 grid, int threads, int smem, cudaStream_t s, bool after, A... args) {
