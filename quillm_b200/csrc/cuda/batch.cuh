@@ -16,40 +16,65 @@ __device__ __forceinline__ void from_f32(float v, float *o) { *o = v; }
 __device__ __forceinline__ void from_f32(float v, __half *o) { *o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16 *o) { *o = __float2bfloat16_rn(v); }
 
-// C consecutive elements, moved in pieces of up to 16 bytes; p is aligned to min(16, C * sizeof(T)) bytes
+// two elements at once
+__device__ __forceinline__ float2 to_f32x2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 to_f32x2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ float2 to_f32x2(float2 v) { return v; }
+__device__ __forceinline__ void from_f32x2(float x, float y, __half2 *o) { *o = __floats2half2_rn(x, y); }
+__device__ __forceinline__ void from_f32x2(float x, float y, __nv_bfloat162 *o) { *o = __floats2bfloat162_rn(x, y); }
+__device__ __forceinline__ void from_f32x2(float x, float y, float2 *o) { *o = make_float2(x, y); }
+template <typename T>
+struct Two;
+template <>
+struct Two<float> {
+    using type = float2;
+};
+template <>
+struct Two<__half> {
+    using type = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+};
+
+// C consecutive elements as they lie in memory, moved in pieces of up to 16 bytes: an address is aligned to
+// min(16, C * sizeof(T)) bytes
+template <typename T, int C>
+struct alignas(C * sizeof(T) >= 16 ? 16 : C * sizeof(T)) Chunk {
+    T e[C];
+};
+template <typename T, int C>
+__device__ __forceinline__ void widen(const Chunk<T, C> &c, float (&v)[C]) {
+    if constexpr (C % 2 == 0) {
+        using T2 = typename Two<T>::type;
+#pragma unroll
+        for (int i = 0; i < C; i += 2) {
+            const float2 f = to_f32x2(*(const T2 *)&c.e[i]);
+            v[i] = f.x, v[i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i++) v[i] = to_f32(c.e[i]);
+    }
+}
 template <typename T, int C>
 __device__ __forceinline__ void load_chunk(const T *p, float (&v)[C]) {
-    constexpr int B = C * (int)sizeof(T);
-    alignas(16) T e[C];
-    if constexpr (B >= 16) {
-#pragma unroll
-        for (int i = 0; i < B / 16; i++) ((uint4 *)e)[i] = ((const uint4 *)p)[i];
-    } else if constexpr (B == 8) {
-        *(uint2 *)e = *(const uint2 *)p;
-    } else if constexpr (B == 4) {
-        *(uint32_t *)e = *(const uint32_t *)p;
-    } else {
-        e[0] = p[0];
-    }
-#pragma unroll
-    for (int i = 0; i < C; i++) v[i] = to_f32(e[i]);
+    const Chunk<T, C> c = *(const Chunk<T, C> *)p;
+    widen(c, v);
 }
 template <typename T, int C>
 __device__ __forceinline__ void store_chunk(T *p, const float (&v)[C]) {
-    constexpr int B = C * (int)sizeof(T);
-    alignas(16) T e[C];
+    Chunk<T, C> c;
+    if constexpr (C % 2 == 0) {
+        using T2 = typename Two<T>::type;
 #pragma unroll
-    for (int i = 0; i < C; i++) from_f32(v[i], &e[i]);
-    if constexpr (B >= 16) {
-#pragma unroll
-        for (int i = 0; i < B / 16; i++) ((uint4 *)p)[i] = ((const uint4 *)e)[i];
-    } else if constexpr (B == 8) {
-        *(uint2 *)p = *(const uint2 *)e;
-    } else if constexpr (B == 4) {
-        *(uint32_t *)p = *(const uint32_t *)e;
+        for (int i = 0; i < C; i += 2) from_f32x2(v[i], v[i + 1], (T2 *)&c.e[i]);
     } else {
-        p[0] = e[0];
+#pragma unroll
+        for (int i = 0; i < C; i++) from_f32(v[i], &c.e[i]);
     }
+    *(Chunk<T, C> *)p = c;
 }
 
 inline bool is_row_dtype(int d) { return d == QMC_F32 || d == QMC_F16 || d == QMC_BF16; }

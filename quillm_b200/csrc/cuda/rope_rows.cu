@@ -2,15 +2,17 @@
 // into a paged cache (qmc_qk_norm_rope, qmc_kv_append_paged).
 //
 // For every head x of a row:  y = x / sqrt(mean(x^2) + eps) * w  (optional), then each pair (a, b) of the first
-// rot dimensions becomes (a c - b s, a s + b c) with (c, s) = m (cos, sin)(pos f_i).  The angle is formed in turns in
-// double, t = pos * f_i / 2 pi, reduced by its nearest integer (exact) and only then rounded to float for sincospi: at
-// position 10^6 the product still carries 2^-33 turns, where a float angle would be off by a sixteenth of a radian.
+// rot dimensions becomes (a c - b s, a s + b c) with (c, s) = m (cos, sin)(pos f_i).  The angle is formed in turns in fixed point:
+// f_i / 2 pi is kept as a fraction of 2^64, and pos times it modulo 2^64 is the fraction of a turn, off by pos times the double's
+// rounding of f_i (2^-36 turns at position 10^6, where a float angle would be off by a sixteenth of a radian); its upper half,
+// rounded to float, goes to sincospi.
 //
 // HBM bound: each element is read once and written once with ~10 operations between.  A lane group of 1 to 32 lanes
 // holds one head, each lane two chunks of C elements (16 bytes each where the layout allows it) that hold whole
 // pairs between them: in the half layout the chunks at t C and t C + rot / 2, in the interleaved one neighbours.  So a
-// rotation needs no exchange, a norm log2(lanes) shuffles, and every access is a full vector.  A block takes up to
-// 256 threads' worth of one row's heads and forms the row's (c, s) once in shared memory while its loads are in flight.
+// rotation needs no exchange, a norm log2(lanes) shuffles, and every access is a full vector.  A row's (c, s) are formed once
+// per block, in shared memory, while its elements are in flight.
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -19,7 +21,7 @@
 struct qmc_rope_plan {
     int head_dim, rot_dim, layout;
     float mscale;
-    double turns[128];  // f_i / 2 pi
+    uint64_t turns[128];  // f_i / 2 pi without its whole turns, times 2^64
 };
 
 namespace qmc {
@@ -43,7 +45,7 @@ namespace {
 struct RowsArgs {
     const void *q, *k, *v;
     void *qo, *ko;  // rows; ko: keys to rows (no cache)
-    int64_t ldq, ldk, ldv, ldqo, ldko;
+    int64_t ldq, ldk, ldv, ldqo, ldko, rows;
     void *kc, *vc;  // one layer of the pools, or null
     const int *seq, *pos, *table;
     const float *qw, *kw;
@@ -51,81 +53,97 @@ struct RowsArgs {
     int n_seq, ld_table, page_size, n_pages;
     int heads, kv, hd, rot;
     int shift;      // log2 of a head's lanes
-    bool half, rotate;
-    float eps, mscale;
+    bool half;
+    float eps, mscale, inv_hd;
 };
+constexpr int kRows = 4;  // rows of a block, of many
 struct Turns {
-    double t[128];
+    uint64_t t[128];
 };
 
-// the two chunks of lane item t: offsets ea, eb, the pair index of each chunk's first element, and whether element i
-// of one pairs with element i of the other (else pairs lie inside each chunk)
-template <int C>
-__device__ __forceinline__ void item_offsets(int t, bool half, int rot, int &ea, int &eb, int &pa, int &pb, bool &across,
-                                             bool &turn) {
-    if (half) {
-        const int P = (rot >> 1) / C;
-        turn = t < P;
-        across = true;
-        ea = turn ? t * C : rot + 2 * (t - P) * C;
-        eb = turn ? ea + (rot >> 1) : ea + C;
-        pa = pb = turn ? t * C : 0;
+// N consecutive (c, s), an even number of them from a 16-byte boundary (one: 8)
+template <int N>
+__device__ __forceinline__ void load_turns(const float2 *p, float2 (&r)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float4 v = *(const float4 *)(p + i);
+            r[i] = make_float2(v.x, v.y), r[i + 1] = make_float2(v.z, v.w);
+        }
     } else {
-        ea = 2 * t * C, eb = ea + C;
-        across = C == 1;
-        turn = true;  // pairs past rot / 2 hold (1, 0)
-        pa = ea >> 1, pb = eb >> 1;
+        r[0] = p[0];
     }
 }
+__device__ __forceinline__ void rotate(float &a, float &b, float2 r) {
+    const float u = a, v = b;
+    a = u * r.x - v * r.y;
+    b = u * r.y + v * r.x;
+}
 
-// T rows, CT cache elements, C elements per chunk, NIT items per lane
-template <typename T, typename CT, int C, int NIT>
-__global__ void __launch_bounds__(256) rope_rows_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Turns f) {
-    __shared__ __align__(16) float2 cs[128];
-    __shared__ __align__(16) float w_s[2][256];
-    __shared__ int64_t slot_s;
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, lph = 1 << a.shift, li = tid & (lph - 1), hd = a.hd;
+// T rows, CT cache elements, C elements per chunk, NIT items per lane, R rows a block: their elements are all on their way before
+// the rows' (c, s) and slots are formed, each by a thread of its own.  FULL: every lane has both its chunks, and a head's lanes
+// and pairs are powers of two.
+template <typename T, typename CT, int C, int NIT, int R, bool HALF, bool FULL>
+__global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Turns f) {
+    __shared__ __align__(16) float2 cs[R][128];
+    __shared__ int64_t slot_s[R];
+    const int tid = threadIdx.x, lph = 1 << a.shift, li = tid & (lph - 1), hd = a.hd, half_hd = hd >> 1;
     const int head = (int)blockIdx.y * ((int)blockDim.x >> a.shift) + (tid >> a.shift);
     const bool cache = a.kc != nullptr;
-    const int n_heads = a.heads + a.kv + (cache ? a.kv : 0);
     const int kind = head < a.heads ? 0 : head < a.heads + a.kv ? 1 : 2;  // q, k, v
-    const bool live = head < n_heads;
+    const bool live = kind < 2 || (cache && head < a.heads + 2 * a.kv);
     const int h = kind == 0 ? head : kind == 1 ? head - a.heads : head - a.heads - a.kv;
+    const int64_t row0 = (int64_t)blockIdx.x * R, ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
+    const int n = (int)(a.rows - row0 < R ? a.rows - row0 : R);
 
-    const T *src = nullptr;
-    if (live)
-        src = (kind == 0 ? (const T *)a.q + row * a.ldq : kind == 1 ? (const T *)a.k + row * a.ldk : (const T *)a.v + row * a.ldv) +
-              (int64_t)h * hd;
-    float xa[NIT][C], xb[NIT][C];
+    // this lane's items: chunks at ea and eb (hd: none), in whose pairs the turns of pa, ... (and pb, ...) apply.  HALF: element i of one
+    // chunk pairs with element i of the other, the dimensions past the rotated ones stay; else pairs lie within a chunk, or,
+    // of one element, in the two neighbours
+    int ea[NIT], eb[NIT], pa[NIT];
+    bool turn[NIT];
 #pragma unroll
     for (int j = 0; j < NIT; j++) {
-        int ea, eb, pa, pb;
-        bool across, turn;
-        item_offsets<C>(li + j * lph, a.half, a.rot, ea, eb, pa, pb, across, turn);
-#pragma unroll
-        for (int i = 0; i < C; i++) xa[j][i] = xb[j][i] = 0.0f;
-        if (live && ea < hd) load_chunk<T, C>(src + ea, xa[j]);
-        if (live && eb < hd) load_chunk<T, C>(src + eb, xb[j]);
+        const int t = li + j * lph, P = (a.rot >> 1) / C;
+        if (HALF) {
+            turn[j] = t < P;
+            ea[j] = turn[j] ? t * C : a.rot + 2 * (t - P) * C;
+            eb[j] = turn[j] ? ea[j] + (a.rot >> 1) : ea[j] + C;
+            pa[j] = t * C;
+        } else {
+            ea[j] = 2 * t * C, eb[j] = ea[j] + C, pa[j] = t * C;
+            turn[j] = ea[j] < a.rot;  // pairs past the rotated ones hold (1, 0)
+        }
+        if (!FULL && (!live || ea[j] > hd)) ea[j] = hd;
+        if (!FULL && (!live || eb[j] > hd)) eb[j] = hd;
+        turn[j] = turn[j] && kind != 2 && (FULL || ea[j] < hd);
     }
-    const int pos = a.pos[row];
-    for (int i = tid; i < hd >> 1; i += blockDim.x) {
+    auto has = [&](int e) { return FULL ? live : e < hd; };
+    const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (live ? row0 * ld + (int64_t)h * hd : 0);
+    Chunk<T, C> ca[R][NIT] = {}, cb[R][NIT] = {};
+#pragma unroll
+    for (int k = 0; k < R; k++)
+#pragma unroll
+        for (int j = 0; j < NIT; j++) {
+            if (k < n && has(ea[j])) ca[k][j] = *(const Chunk<T, C> *)(src + k * ld + ea[j]);
+            if (k < n && has(eb[j])) cb[k][j] = *(const Chunk<T, C> *)(src + k * ld + eb[j]);
+        }
+    // the lanes of a warp want different entries: read as memory, since the constant cache gives one address at a time
+    const uint64_t *step = f.t;
+    asm volatile("" : "+l"(step));
+    for (int i = tid; i < n * half_hd; i += blockDim.x) {
+        const int k = R == 1 ? 0 : FULL ? i >> (31 - __clz(half_hd)) : i / half_hd, p = R == 1 ? i : FULL ? i & (half_hd - 1) : i % half_hd;
         float s = 0.0f, c = 1.0f;
-        if (a.rotate && 2 * i < a.rot) {
-            const double t = (double)pos * f.t[i];
-            sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+        if (2 * p < a.rot) {
+            const uint64_t t = (uint64_t)(int64_t)a.pos[row0 + k] * step[p];
+            sincospif((float)(int32_t)(t >> 32) * 4.656612873077393e-10f, &s, &c);  // 2^-31: half turns in [-1, 1)
             s *= a.mscale, c *= a.mscale;
         }
-        cs[i] = make_float2(c, s);
+        cs[k][p] = make_float2(c, s);
     }
-    if (a.qw)
-        for (int i = tid; i < hd; i += blockDim.x) w_s[0][i] = a.qw[i];
-    if (a.kw)
-        for (int i = tid; i < hd; i += blockDim.x) w_s[1][i] = a.kw[i];
-    if (cache && tid == (int)blockDim.x - 1) {
-        // -1: no slot; -2: padding
-        const int sq = a.seq ? a.seq[row] : (int)row;
-        int64_t slot = -2;
+    if (const int k = (int)blockDim.x - 1 - tid; cache && k < n) {
+        int64_t slot = -2;  // padding; -1: none
+        const int64_t row = row0 + k;
+        const int sq = a.seq ? a.seq[row] : (int)row, pos = a.pos[row];
         if (sq >= 0 && pos >= 0) {
             slot = -1;
             const int e = pos / a.page_size;
@@ -135,92 +153,119 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const __grid_constant__ 
             }
             if (slot < 0) raise_error(a.err, kErrBadIndex);
         }
-        slot_s = slot;
+        slot_s[k] = slot;
     }
-    __syncthreads();
-    const int64_t slot = cache ? slot_s : 0;
-    if (slot == -2) return;  // the whole row's blocks
-    const float *w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
-    if (w) {  // the same for a head's lanes; other heads of the warp may differ, so the shuffles are masked to the group
-        float ss = 0.0f;
+    const float *w = !live ? nullptr : kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
+    float wa[NIT][C], wb[NIT][C];
+    if (w)
 #pragma unroll
         for (int j = 0; j < NIT; j++)
 #pragma unroll
-            for (int i = 0; i < C; i++) ss = fmaf(xa[j][i], xa[j][i], fmaf(xb[j][i], xb[j][i], ss));
-        const unsigned group = (lph == 32 ? 0xffffffffu : ((1u << lph) - 1u)) << ((tid & 31) & ~(lph - 1));
-        for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-        const float r = 1.0f / sqrtf(ss / (float)hd + a.eps);
-        const float *ws = w_s[kind];
+            for (int i = 0; i < C; i++) wa[j][i] = has(ea[j]) ? w[ea[j] + i] : 0.0f, wb[j][i] = has(eb[j]) ? w[eb[j] + i] : 0.0f;
+    __syncthreads();
+    if (FULL && !live) return;
+    const float inv_hd = a.inv_hd, eps = a.eps;
+    const int row_elems = a.kv * hd;
+    CT *const cbase = (kind == 1 ? (CT *)a.kc : (CT *)a.vc) + (live ? h * hd : 0);
+    T *dst = (T *)(kind == 0 ? a.qo : a.ko) + (!live || (cache && kind) ? 0 : row0 * (kind == 0 ? a.ldqo : a.ldko) + (int64_t)h * hd);
+    const int64_t ldo = kind == 0 ? a.ldqo : a.ldko;
+    const unsigned group = (lph == 32 ? 0xffffffffu : ((1u << lph) - 1u)) << ((tid & 31) & ~(lph - 1));
+    constexpr int G = R > 1 ? 2 : 1;  // rows worked on together, without a branch between them: their latencies overlap
 #pragma unroll
-        for (int j = 0; j < NIT; j++) {
-            int ea, eb, pa, pb;
-            bool across, turn;
-            item_offsets<C>(li + j * lph, a.half, a.rot, ea, eb, pa, pb, across, turn);
+    for (int k0 = 0; k0 < R; k0 += G) {
+        float xa[G][NIT][C], xb[G][NIT][C];
 #pragma unroll
-            for (int i = 0; i < C; i++) {
-                if (ea < hd) xa[j][i] *= r * ws[ea + i];
-                if (eb < hd) xb[j][i] *= r * ws[eb + i];
+        for (int k = 0; k < G; k++)
+#pragma unroll
+            for (int j = 0; j < NIT; j++) widen(ca[k0 + k][j], xa[k][j]), widen(cb[k0 + k][j], xb[k][j]);
+        if (w) {  // the same for a head's lanes; other heads of the warp may differ, so the shuffles are masked to the group
+            float ss[G];
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                ss[k] = 0.0f;  // missing chunks are zeros
+#pragma unroll
+                for (int j = 0; j < NIT; j++)
+#pragma unroll
+                    for (int i = 0; i < C; i++) ss[k] = fmaf(xa[k][j][i], xa[k][j][i], fmaf(xb[k][j][i], xb[k][j][i], ss[k]));
+            }
+            for (int o = lph >> 1; o; o >>= 1)
+#pragma unroll
+                for (int k = 0; k < G; k++) ss[k] += __shfl_xor_sync(group, ss[k], o);
+#pragma unroll
+            for (int k = 0; k < G; k++) {
+                const float r = rsqrtf(fmaf(ss[k], inv_hd, eps));  // two units in the last place
+#pragma unroll
+                for (int j = 0; j < NIT; j++)
+#pragma unroll
+                    for (int i = 0; i < C; i++) xa[k][j][i] *= r * wa[j][i], xb[k][j][i] *= r * wb[j][i];
             }
         }
-    }
-    if (!live || (kind != 0 && slot < 0)) return;
-    T *dst = kind == 0 ? (T *)a.qo + row * a.ldqo + (int64_t)h * hd : (T *)a.ko + (cache ? 0 : row * a.ldko + (int64_t)h * hd);
-    CT *cdst = (kind == 1 ? (CT *)a.kc : (CT *)a.vc) + (cache ? (slot * a.kv + h) * hd : 0);
 #pragma unroll
-    for (int j = 0; j < NIT; j++) {
-        int ea, eb, pa, pb;
-        bool across, turn;
-        item_offsets<C>(li + j * lph, a.half, a.rot, ea, eb, pa, pb, across, turn);
-        if (ea >= hd) continue;
-        if (kind != 2 && turn) {
-            if (across) {
+        for (int j = 0; j < NIT; j++)
+            if (turn[j])
 #pragma unroll
-                for (int i = 0; i < C; i++) {
-                    const float2 r = cs[pa + i];
-                    const float u = xa[j][i], v = xb[j][i];
-                    xa[j][i] = u * r.x - v * r.y;
-                    xb[j][i] = u * r.y + v * r.x;
-                }
-            } else {
+                for (int k = 0; k < G; k++) {
+                    float2 r[C];
+                    load_turns<C>(&cs[k0 + k][pa[j]], r);
 #pragma unroll
-                for (int i = 0; i + 1 < C; i += 2) {
-                    const float2 r = cs[pa + i / 2];
-                    const float u = xa[j][i], v = xa[j][i + 1];
-                    xa[j][i] = u * r.x - v * r.y;
-                    xa[j][i + 1] = u * r.y + v * r.x;
-                    if (eb < hd) {
-                        const float2 r2 = cs[pb + i / 2];
-                        const float u2 = xb[j][i], v2 = xb[j][i + 1];
-                        xb[j][i] = u2 * r2.x - v2 * r2.y;
-                        xb[j][i + 1] = u2 * r2.y + v2 * r2.x;
+                    for (int i = 0; i < C; i++) {
+                        if (HALF || C == 1) rotate(xa[k][j][i], xb[k][j][i], r[i]);
+                        else if (i % 2 == 0) rotate(xa[k][j][i], xa[k][j][(i + 1) % C], r[i / 2]), rotate(xb[k][j][i], xb[k][j][(i + 1) % C], r[(C + i) / 2]);
                     }
                 }
+#pragma unroll
+        for (int k = 0; k < G; k++) {
+            const int64_t slot = cache && k0 + k < n ? slot_s[k0 + k] : 0;
+            if (k0 + k >= n || slot == -2) continue;  // padding: for the whole row
+            if (kind == 0 || !cache) {
+                T *o = dst + (k0 + k) * ldo;
+#pragma unroll
+                for (int j = 0; j < NIT; j++) {
+                    if (FULL || ea[j] < hd) store_chunk<T, C>(o + ea[j], xa[k][j]);
+                    if (FULL || eb[j] < hd) store_chunk<T, C>(o + eb[j], xb[k][j]);
+                }
+            } else if (slot >= 0) {
+                CT *cdst = cbase + slot * (int64_t)row_elems;
+#pragma unroll
+                for (int j = 0; j < NIT; j++) {
+                    if (FULL || ea[j] < hd) store_chunk<CT, C>(cdst + ea[j], xa[k][j]);
+                    if (FULL || eb[j] < hd) store_chunk<CT, C>(cdst + eb[j], xb[k][j]);
+                }
             }
-        }
-        if (kind == 0 || !cache) {
-            store_chunk<T, C>(dst + ea, xa[j]);
-            if (eb < hd) store_chunk<T, C>(dst + eb, xb[j]);
-        } else {
-            store_chunk<CT, C>(cdst + ea, xa[j]);
-            if (eb < hd) store_chunk<CT, C>(cdst + eb, xb[j]);
         }
     }
 }
 
+template <typename T, typename CT, int C, int NIT, int R, bool FULL>
+int launch_r(RowsArgs &a, const Turns &f, int64_t warps, cudaStream_t s) {
+    const int64_t parts = (warps + 9) / 10, wpb = (warps + parts - 1) / parts;  // even blocks of at most ten warps
+    if (parts > 65535) return set_error(QMC_EINVAL, "rope rows: %d heads are too many", a.heads + a.kv);
+    const dim3 grid((unsigned)((a.rows + R - 1) / R), (unsigned)parts);
+    if (a.half) rope_rows_kernel<T, CT, C, NIT, R, true, FULL><<<grid, (unsigned)wpb * 32, 0, s>>>(a, f);
+    else rope_rows_kernel<T, CT, C, NIT, R, false, FULL><<<grid, (unsigned)wpb * 32, 0, s>>>(a, f);
+    QMC_LAUNCH_CHECK();
+    return QMC_OK;
+}
+
 template <typename T, typename CT, int C, int NIT>
 int launch_t(RowsArgs &a, const Turns &f, int64_t rows, cudaStream_t s) {
+    const DevCtx *dc = ctx();
+    const int64_t sms = dc ? dc->num_sms : 148;
     const int P = a.half ? (a.rot >> 1) / C : 0;
     const int chunks = a.half ? (a.hd - a.rot) / C : a.hd / C;
     const int items = P + (chunks + 1) / 2;
     a.shift = 0;
     while ((NIT << a.shift) < items) a.shift++;
+    a.rows = rows, a.inv_hd = 1.0f / (float)a.hd;
     const int heads = a.heads + a.kv + (a.kc ? a.kv : 0);
-    const int lanes = heads << a.shift, warps = (lanes + 31) / 32;
-    const int parts = (warps + 7) / 8, wpb = (warps + parts - 1) / parts;  // even blocks of at most 8 warps
-    if (parts > 65535) return set_error(QMC_EINVAL, "rope rows: %d heads are too many", heads);
-    rope_rows_kernel<T, CT, C, NIT><<<dim3((unsigned)rows, parts), wpb * 32, 0, s>>>(a, f);
-    QMC_LAUNCH_CHECK();
-    return QMC_OK;
+    const int64_t warps = ((int64_t)heads * (1 << a.shift) + 31) / 32;
+    // several rows a block once one row each fills the SMs twice over
+    if constexpr (NIT == 1)
+        if (rows * warps > 64 * sms) {
+            const bool full = items == 1 << a.shift && chunks % 2 == 0 && (a.hd & (a.hd - 1)) == 0;
+            return full ? launch_r<T, CT, C, NIT, kRows, true>(a, f, warps, s) : launch_r<T, CT, C, NIT, kRows, false>(a, f, warps, s);
+        }
+    return launch_r<T, CT, C, NIT, 1, false>(a, f, warps, s);
 }
 
 // the widest chunk that divides the head, the rotated half, the strides and every address; hd <= 256, so a lane needs at most
@@ -256,7 +301,6 @@ int launch_ct(RowsArgs &a, const Turns &f, int cdt, int64_t rows, cudaStream_t s
 int launch_rows(RowsArgs &a, const qmc_rope_plan *p, int dtype, int cdt, int64_t rows, cudaStream_t s) {
     static const Turns none{};
     Turns f = none;
-    a.rotate = p != nullptr;
     a.half = p && p->layout == QMC_ROPE_HALF;
     a.rot = p ? p->rot_dim : 0;
     a.mscale = p ? p->mscale : 1.0f;
@@ -326,7 +370,11 @@ int qmc_rope_plan_create(const qmc_rope_config *c, qmc_rope_plan **out) {
             const double r = fmin(fmax((i - lo) / fmax(hi - lo, 0.001), 0.0), 1.0);
             f = f / c->factor * r + f * (1.0 - r);
         }
-        p->turns[i] = f / two_pi;
+        double turns = f / two_pi;  // f < 2^1023: the whole turns go, the rest is exact
+        turns -= floor(turns);
+        // two halves of 32 bits: a double holds 53 bits of the fraction, none is lost
+        const double hi = floor(turns * 4294967296.0);
+        p->turns[i] = ((uint64_t)hi << 32) + (uint64_t)((turns * 4294967296.0 - hi) * 4294967296.0);
     }
     *out = p;
     return QMC_OK;
