@@ -10,8 +10,9 @@
 // HBM bound: each element is read once and written once with ~10 operations between.  A lane group of 1 to 32 lanes
 // holds one head, each lane two chunks of C elements (16 bytes each where the layout allows it) that hold whole
 // pairs between them: in the half layout the chunks at t C and t C + rot / 2, in the interleaved one neighbours.  So a
-// rotation needs no exchange, a norm log2(lanes) shuffles, and every access is a full vector.  A row's (c, s) are formed once
-// per block, in shared memory, while its elements are in flight.
+// rotation needs no exchange, a norm log2(lanes) shuffles, and every access is a full vector.  While the elements are in flight the
+// block forms a table of its rows' pairs in shared memory, (w0 c, w1 s, w0 s, w1 c) with the pair's weights folded in, for
+// queries and for keys: with r the head's 1 / sqrt(mean + eps), a' = (a w0 c - b w1 s) r and b' = (a w0 s + b w1 c) r.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -53,6 +54,7 @@ struct RowsArgs {
     int n_seq, ld_table, page_size, n_pages;
     int heads, kv, hd, rot;
     int shift;      // log2 of a head's lanes
+    int pairs;      // of the table: items times C
     bool half;
     float eps, mscale, inv_hd;
 };
@@ -61,23 +63,17 @@ struct Turns {
     uint64_t t[128];
 };
 
-// N consecutive (c, s), an even number of them from a 16-byte boundary (one: 8)
-template <int N>
-__device__ __forceinline__ void load_turns(const float2 *p, float2 (&r)[N]) {
-    if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float4 v = *(const float4 *)(p + i);
-            r[i] = make_float2(v.x, v.y), r[i + 1] = make_float2(v.z, v.w);
-        }
-    } else {
-        r[0] = p[0];
-    }
+// where item t's pair e lies among the C of its item: the 16-byte entries that eight neighbouring lanes read together fall on
+// distinct banks
+template <int C>
+__device__ __forceinline__ int spread(int t, int e) {
+    return e ^ ((t / (8 / C)) & (C - 1));
 }
-__device__ __forceinline__ void rotate(float &a, float &b, float2 r) {
+// (a, b) of a pair through its row of the table, times the head's factor
+__device__ __forceinline__ void rotate(float &a, float &b, float4 r, float f) {
     const float u = a, v = b;
-    a = u * r.x - v * r.y;
-    b = u * r.y + v * r.x;
+    a = (u * r.x - v * r.y) * f;
+    b = (u * r.z + v * r.w) * f;
 }
 
 // T rows, CT cache elements, C elements per chunk, NIT items per lane, R rows a block: their elements are all on their way before
@@ -85,9 +81,9 @@ __device__ __forceinline__ void rotate(float &a, float &b, float2 r) {
 // and pairs are powers of two.
 template <typename T, typename CT, int C, int NIT, int R, bool HALF, bool FULL>
 __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Turns f) {
-    __shared__ __align__(16) float2 cs[R][128];
+    __shared__ float4 tab[2][R][128];  // [queries, keys][row][pair]
     __shared__ int64_t slot_s[R];
-    const int tid = threadIdx.x, lph = 1 << a.shift, li = tid & (lph - 1), hd = a.hd, half_hd = hd >> 1;
+    const int tid = threadIdx.x, lph = 1 << a.shift, li = tid & (lph - 1), hd = a.hd;
     const int head = (int)blockIdx.y * ((int)blockDim.x >> a.shift) + (tid >> a.shift);
     const bool cache = a.kc != nullptr;
     const int kind = head < a.heads ? 0 : head < a.heads + a.kv ? 1 : 2;  // q, k, v
@@ -96,26 +92,17 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
     const int64_t row0 = (int64_t)blockIdx.x * R, ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
     const int n = (int)(a.rows - row0 < R ? a.rows - row0 : R);
 
-    // this lane's items: chunks at ea and eb (hd: none), in whose pairs the turns of pa, ... (and pb, ...) apply.  HALF: element i of one
-    // chunk pairs with element i of the other, the dimensions past the rotated ones stay; else pairs lie within a chunk, or,
-    // of one element, in the two neighbours
-    int ea[NIT], eb[NIT], pa[NIT];
-    bool turn[NIT];
+    // this lane's items: chunks at ea and eb (hd: none), which hold the pairs t C, ... of item t.  HALF: element i of one chunk
+    // pairs with element i of the other; else pairs lie within a chunk, or, of one element, in the two neighbours
+    const int rot_items = (a.rot >> 1) / C;
+    int ea[NIT], eb[NIT];
 #pragma unroll
     for (int j = 0; j < NIT; j++) {
-        const int t = li + j * lph, P = (a.rot >> 1) / C;
-        if (HALF) {
-            turn[j] = t < P;
-            ea[j] = turn[j] ? t * C : a.rot + 2 * (t - P) * C;
-            eb[j] = turn[j] ? ea[j] + (a.rot >> 1) : ea[j] + C;
-            pa[j] = t * C;
-        } else {
-            ea[j] = 2 * t * C, eb[j] = ea[j] + C, pa[j] = t * C;
-            turn[j] = ea[j] < a.rot;  // pairs past the rotated ones hold (1, 0)
-        }
+        const int t = li + j * lph;
+        ea[j] = !HALF ? 2 * t * C : t < rot_items ? t * C : a.rot + 2 * (t - rot_items) * C;
+        eb[j] = ea[j] + (HALF && t < rot_items ? a.rot >> 1 : C);
         if (!FULL && (!live || ea[j] > hd)) ea[j] = hd;
         if (!FULL && (!live || eb[j] > hd)) eb[j] = hd;
-        turn[j] = turn[j] && kind != 2 && (FULL || ea[j] < hd);
     }
     auto has = [&](int e) { return FULL ? live : e < hd; };
     const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (live ? row0 * ld + (int64_t)h * hd : 0);
@@ -130,15 +117,22 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
     // the lanes of a warp want different entries: read as memory, since the constant cache gives one address at a time
     const uint64_t *step = f.t;
     asm volatile("" : "+l"(step));
-    for (int i = tid; i < n * half_hd; i += blockDim.x) {
-        const int k = R == 1 ? 0 : FULL ? i >> (31 - __clz(half_hd)) : i / half_hd, p = R == 1 ? i : FULL ? i & (half_hd - 1) : i % half_hd;
+    for (int i = tid; i < n * a.pairs; i += blockDim.x) {
+        const int k = R == 1 ? 0 : FULL ? i >> (31 - __clz(a.pairs)) : i / a.pairs, p = R == 1 ? i : FULL ? i & (a.pairs - 1) : i % a.pairs;
+        const int t = p / C, d0 = !HALF ? 2 * p : t < rot_items ? p : a.rot + 2 * (t - rot_items) * C + p % C;
+        const int d1 = !HALF ? 2 * p + 1 : t < rot_items ? p + (a.rot >> 1) : d0 + C;
         float s = 0.0f, c = 1.0f;
-        if (2 * p < a.rot) {
-            const uint64_t t = (uint64_t)(int64_t)a.pos[row0 + k] * step[p];
-            sincospif((float)(int32_t)(t >> 32) * 4.656612873077393e-10f, &s, &c);  // 2^-31: half turns in [-1, 1)
+        if (HALF ? t < rot_items : d0 < a.rot) {
+            const uint64_t turns = (uint64_t)(int64_t)a.pos[row0 + k] * step[p];
+            sincospif((float)(int32_t)(turns >> 32) * 4.656612873077393e-10f, &s, &c);  // 2^-31: half turns in [-1, 1)
             s *= a.mscale, c *= a.mscale;
         }
-        cs[k][p] = make_float2(c, s);
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const float *w = q ? a.kw : a.qw;
+            const float w0 = w && d0 < hd ? w[d0] : 1.0f, w1 = w && d1 < hd ? w[d1] : 1.0f;
+            tab[q][k][t * C + spread<C>(t, p % C)] = make_float4(w0 * c, w1 * s, w0 * s, w1 * c);
+        }
     }
     if (const int k = (int)blockDim.x - 1 - tid; cache && k < n) {
         int64_t slot = -2;  // padding; -1: none
@@ -155,13 +149,7 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
         }
         slot_s[k] = slot;
     }
-    const float *w = !live ? nullptr : kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
-    float wa[NIT][C], wb[NIT][C];
-    if (w)
-#pragma unroll
-        for (int j = 0; j < NIT; j++)
-#pragma unroll
-            for (int i = 0; i < C; i++) wa[j][i] = has(ea[j]) ? w[ea[j] + i] : 0.0f, wb[j][i] = has(eb[j]) ? w[eb[j] + i] : 0.0f;
+    const bool norm = live && (kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr) != nullptr;
     __syncthreads();
     if (FULL && !live) return;
     const float inv_hd = a.inv_hd, eps = a.eps;
@@ -178,7 +166,10 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
         for (int k = 0; k < G; k++)
 #pragma unroll
             for (int j = 0; j < NIT; j++) widen(ca[k0 + k][j], xa[k][j]), widen(cb[k0 + k][j], xb[k][j]);
-        if (w) {  // the same for a head's lanes; other heads of the warp may differ, so the shuffles are masked to the group
+        float r[G];
+#pragma unroll
+        for (int k = 0; k < G; k++) r[k] = 1.0f;
+        if (norm) {  // the same for a head's lanes; other heads of the warp may differ, so the shuffles are masked to the group
             float ss[G];
 #pragma unroll
             for (int k = 0; k < G; k++) {
@@ -192,25 +183,21 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
 #pragma unroll
                 for (int k = 0; k < G; k++) ss[k] += __shfl_xor_sync(group, ss[k], o);
 #pragma unroll
-            for (int k = 0; k < G; k++) {
-                const float r = rsqrtf(fmaf(ss[k], inv_hd, eps));  // two units in the last place
-#pragma unroll
-                for (int j = 0; j < NIT; j++)
-#pragma unroll
-                    for (int i = 0; i < C; i++) xa[k][j][i] *= r * wa[j][i], xb[k][j][i] *= r * wb[j][i];
-            }
+            for (int k = 0; k < G; k++) r[k] = rsqrtf(fmaf(ss[k], inv_hd, eps));  // two units in the last place
         }
+        if (kind != 2)
 #pragma unroll
-        for (int j = 0; j < NIT; j++)
-            if (turn[j])
+            for (int k = 0; k < G; k++)
 #pragma unroll
-                for (int k = 0; k < G; k++) {
-                    float2 r[C];
-                    load_turns<C>(&cs[k0 + k][pa[j]], r);
+                for (int j = 0; j < NIT; j++) {
+                    if (!FULL && ea[j] >= hd) continue;
+                    const int t = li + j * lph, x = spread<C>(t, 0);
+                    const float4 *row = &tab[kind][k0 + k][t * C];
 #pragma unroll
                     for (int i = 0; i < C; i++) {
-                        if (HALF || C == 1) rotate(xa[k][j][i], xb[k][j][i], r[i]);
-                        else if (i % 2 == 0) rotate(xa[k][j][i], xa[k][j][(i + 1) % C], r[i / 2]), rotate(xb[k][j][i], xb[k][j][(i + 1) % C], r[(C + i) / 2]);
+                        if (HALF || C == 1) rotate(xa[k][j][i], xb[k][j][i], row[i ^ x], r[k]);
+                        else if (i < C / 2) rotate(xa[k][j][2 * i % C], xa[k][j][(2 * i + 1) % C], row[i ^ x], r[k]);
+                        else rotate(xb[k][j][2 * i % C], xb[k][j][(2 * i + 1) % C], row[i ^ x], r[k]);
                     }
                 }
 #pragma unroll
@@ -256,6 +243,7 @@ int launch_t(RowsArgs &a, const Turns &f, int64_t rows, cudaStream_t s) {
     const int items = P + (chunks + 1) / 2;
     a.shift = 0;
     while ((NIT << a.shift) < items) a.shift++;
+    a.pairs = items * C;
     a.rows = rows, a.inv_hd = 1.0f / (float)a.hd;
     const int heads = a.heads + a.kv + (a.kc ? a.kv : 0);
     const int64_t warps = ((int64_t)heads * (1 << a.shift) + 31) / 32;
