@@ -80,7 +80,7 @@ __device__ __forceinline__ void rotate(float &a, float &b, float4 r, float f) {
 // the rows' (c, s) and slots are formed, each by a thread of its own.  FULL: every lane has both its chunks, and a head's lanes
 // and pairs are powers of two.
 template <typename T, typename CT, int C, int NIT, int R, bool HALF, bool FULL>
-__global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Turns f) {
+__global__ void __launch_bounds__(288, 3) rope_rows_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Turns f) {
     __shared__ float4 tab[2][R][128];  // [queries, keys][row][pair]
     __shared__ int64_t slot_s[R];
     const int tid = threadIdx.x, lph = 1 << a.shift, li = tid & (lph - 1), hd = a.hd;
@@ -158,66 +158,49 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
     T *dst = (T *)(kind == 0 ? a.qo : a.ko) + (!live || (cache && kind) ? 0 : row0 * (kind == 0 ? a.ldqo : a.ldko) + (int64_t)h * hd);
     const int64_t ldo = kind == 0 ? a.ldqo : a.ldko;
     const unsigned group = (lph == 32 ? 0xffffffffu : ((1u << lph) - 1u)) << ((tid & 31) & ~(lph - 1));
-    constexpr int G = R > 1 ? 2 : 1;  // rows worked on together, without a branch between them: their latencies overlap
 #pragma unroll
-    for (int k0 = 0; k0 < R; k0 += G) {
-        float xa[G][NIT][C], xb[G][NIT][C];
+    for (int k = 0; k < R; k++) {
+        float xa[NIT][C], xb[NIT][C], r = 1.0f;
 #pragma unroll
-        for (int k = 0; k < G; k++)
-#pragma unroll
-            for (int j = 0; j < NIT; j++) widen(ca[k0 + k][j], xa[k][j]), widen(cb[k0 + k][j], xb[k][j]);
-        float r[G];
-#pragma unroll
-        for (int k = 0; k < G; k++) r[k] = 1.0f;
+        for (int j = 0; j < NIT; j++) widen(ca[k][j], xa[j]), widen(cb[k][j], xb[j]);
         if (norm) {  // the same for a head's lanes; other heads of the warp may differ, so the shuffles are masked to the group
-            float ss[G];
+            float ss = 0.0f;  // missing chunks are zeros
 #pragma unroll
-            for (int k = 0; k < G; k++) {
-                ss[k] = 0.0f;  // missing chunks are zeros
+            for (int j = 0; j < NIT; j++)
 #pragma unroll
-                for (int j = 0; j < NIT; j++)
-#pragma unroll
-                    for (int i = 0; i < C; i++) ss[k] = fmaf(xa[k][j][i], xa[k][j][i], fmaf(xb[k][j][i], xb[k][j][i], ss[k]));
-            }
-            for (int o = lph >> 1; o; o >>= 1)
-#pragma unroll
-                for (int k = 0; k < G; k++) ss[k] += __shfl_xor_sync(group, ss[k], o);
-#pragma unroll
-            for (int k = 0; k < G; k++) r[k] = rsqrtf(fmaf(ss[k], inv_hd, eps));  // two units in the last place
+                for (int i = 0; i < C; i++) ss = fmaf(xa[j][i], xa[j][i], fmaf(xb[j][i], xb[j][i], ss));
+            for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+            r = rsqrtf(fmaf(ss, inv_hd, eps));  // two units in the last place
         }
         if (kind != 2)
 #pragma unroll
-            for (int k = 0; k < G; k++)
+            for (int j = 0; j < NIT; j++) {
+                if (!FULL && ea[j] >= hd) continue;
+                const int t = li + j * lph, x = spread<C>(t, 0);
+                const float4 *row = &tab[kind][k][t * C];
 #pragma unroll
-                for (int j = 0; j < NIT; j++) {
-                    if (!FULL && ea[j] >= hd) continue;
-                    const int t = li + j * lph, x = spread<C>(t, 0);
-                    const float4 *row = &tab[kind][k0 + k][t * C];
-#pragma unroll
-                    for (int i = 0; i < C; i++) {
-                        if (HALF || C == 1) rotate(xa[k][j][i], xb[k][j][i], row[i ^ x], r[k]);
-                        else if (i < C / 2) rotate(xa[k][j][2 * i % C], xa[k][j][(2 * i + 1) % C], row[i ^ x], r[k]);
-                        else rotate(xb[k][j][2 * i % C], xb[k][j][(2 * i + 1) % C], row[i ^ x], r[k]);
-                    }
+                for (int i = 0; i < C; i++) {
+                    if (HALF || C == 1) rotate(xa[j][i], xb[j][i], row[i ^ x], r);
+                    else if (i < C / 2) rotate(xa[j][2 * i % C], xa[j][(2 * i + 1) % C], row[i ^ x], r);
+                    else rotate(xb[j][2 * i % C], xb[j][(2 * i + 1) % C], row[i ^ x], r);
                 }
+            }
+        // rows past the last, and padding, have gone through this for nothing: no branch lies between the rows' arithmetic
+        const int64_t slot = cache && k < n ? slot_s[k] : 0;
+        if (k >= n || slot == -2) continue;
+        if (kind == 0 || !cache) {
+            T *o = dst + k * ldo;
 #pragma unroll
-        for (int k = 0; k < G; k++) {
-            const int64_t slot = cache && k0 + k < n ? slot_s[k0 + k] : 0;
-            if (k0 + k >= n || slot == -2) continue;  // padding: for the whole row
-            if (kind == 0 || !cache) {
-                T *o = dst + (k0 + k) * ldo;
+            for (int j = 0; j < NIT; j++) {
+                if (FULL || ea[j] < hd) store_chunk<T, C>(o + ea[j], xa[j]);
+                if (FULL || eb[j] < hd) store_chunk<T, C>(o + eb[j], xb[j]);
+            }
+        } else if (slot >= 0) {
+            CT *o = cbase + slot * (int64_t)row_elems;
 #pragma unroll
-                for (int j = 0; j < NIT; j++) {
-                    if (FULL || ea[j] < hd) store_chunk<T, C>(o + ea[j], xa[k][j]);
-                    if (FULL || eb[j] < hd) store_chunk<T, C>(o + eb[j], xb[k][j]);
-                }
-            } else if (slot >= 0) {
-                CT *cdst = cbase + slot * (int64_t)row_elems;
-#pragma unroll
-                for (int j = 0; j < NIT; j++) {
-                    if (FULL || ea[j] < hd) store_chunk<CT, C>(cdst + ea[j], xa[k][j]);
-                    if (FULL || eb[j] < hd) store_chunk<CT, C>(cdst + eb[j], xb[k][j]);
-                }
+            for (int j = 0; j < NIT; j++) {
+                if (FULL || ea[j] < hd) store_chunk<CT, C>(o + ea[j], xa[j]);
+                if (FULL || eb[j] < hd) store_chunk<CT, C>(o + eb[j], xb[j]);
             }
         }
     }
@@ -225,7 +208,7 @@ __global__ void __launch_bounds__(320, R > 1 ? 2 : 3) rope_rows_kernel(const __g
 
 template <typename T, typename CT, int C, int NIT, int R, bool FULL>
 int launch_r(RowsArgs &a, const Turns &f, int64_t warps, cudaStream_t s) {
-    const int64_t parts = (warps + 9) / 10, wpb = (warps + parts - 1) / parts;  // even blocks of at most ten warps
+    const int64_t parts = (warps + 8) / 9, wpb = (warps + parts - 1) / parts;  // even blocks of at most nine warps, three of which an SM holds
     if (parts > 65535) return set_error(QMC_EINVAL, "rope rows: %d heads are too many", a.heads + a.kv);
     const dim3 grid((unsigned)((a.rows + R - 1) / R), (unsigned)parts);
     if (a.half) rope_rows_kernel<T, CT, C, NIT, R, true, FULL><<<grid, (unsigned)wpb * 32, 0, s>>>(a, f);
