@@ -2,30 +2,35 @@
 // (qmc_beam_reorder).
 //
 // Selection in two launches.  Both the log-sum-exp and the order need every logit once, so the first reads each row
-// once, kChunk logits per block held in registers: the chunk's maximum m and sum of exp(x - m), and its n best logits.
+// once, a chunk per block held in registers: the chunk's maximum m and sum of exp(x - m), and its n best logits.
 // Within a row the order of scores is the order of logits, so n per chunk suffice whatever the row's log-sum-exp
-// turns out to be.  The second, one block per prompt, joins a row's (m, sum) pairs in double, and merges the rows'
-// sorted lists by score, n rounds of a block-wide maximum over the lists' heads.
+// turns out to be.  The second, one block per prompt, joins a row's (m, sum) pairs in double and takes the n best of the rows'
+// sorted lists.
 //
-// The n best of a chunk: the n-th largest of the 256 threads' maxima is a lower bound T that at least n elements reach, found
-// by building T's bits from the top in one warp; the few elements >= T are collected in shared memory and ranked by
-// counting.  Keys (logit, index) are distinct, so with all 64 bits of the key at most n threads' elements
-// reach T (n * kItems, the collection's size); the first 32 bits are tried alone first and almost always enough.
-#include "batch.cuh"
+// The n best, in both: the n-th largest of the 256 threads' maxima is a lower bound T that at least n elements reach, found
+// by building the bits of its 32-bit order-preserving form from the top in one warp; the few elements >= T are collected in shared
+// memory and ranked by counting, with the index, so that ties go to the lower one.  Where too many reach T (equal logits), the
+// chunk continues T's bits over the indices, after which at most n threads' elements remain, and the second kernel takes n rounds
+// of a block-wide maximum over the lists' heads.
+#include "attn_prefix.cuh"
 
 namespace qmc {
 namespace {
 
-constexpr int kBT = 256;               // threads
-constexpr int kItems = 16;             // logits per thread
-constexpr int kChunk = kBT * kItems;   // logits per block
-constexpr int kMaxOut = 64;            // n_out and beams
-constexpr int kCap = kMaxOut * kItems; // collected candidates
+constexpr int kBT = 256;      // threads
+constexpr int kMaxOut = 64;   // n_out and beams
+constexpr int kLeast = 4096;  // logits of the smallest chunk
+// logits per thread: four 16-byte loads
+template <typename T>
+__host__ __device__ constexpr int items() {
+    return 64 / sizeof(T);
+}
+static_assert(items<float>() * kBT == kLeast, "smallest chunk");
 
 struct SelArgs {
     const void *logits;
     int64_t ld;
-    int prompts, beams, vocab, n_out, eos, chunks;
+    int prompts, beams, vocab, n_out, eos, chunks, chunk;
     const float *scores;
     const uint8_t *finished;
     float2 *stat;              // [row][chunk] (m, sum exp(x - m))
@@ -34,95 +39,101 @@ struct SelArgs {
     float *out_scores;
 };
 
-// order-preserving bits of a float; NaN counts as -inf, -0 as +0.  Never 0.
+// order-preserving bits of a float, -0 as +0; no NaN comes here.  Never 0.
 __device__ __forceinline__ uint32_t order_bits(float v) {
-    if (v != v) v = -INFINITY;
-    uint32_t u = v == 0.0f ? 0u : __float_as_uint(v);
+    const uint32_t u = __float_as_uint(v + 0.0f);  // -0 + 0 = +0
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float order_value(uint32_t u) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
-__device__ __forceinline__ unsigned long long order_key(float v, int idx) {
-    return ((unsigned long long)order_bits(v) << 32) | (uint32_t)~idx;
+
+// by one warp: the largest T that at least n of the 256 values reach (their n-th largest, or a value above it that exactly n
+// reach), at least 1
+__device__ __forceinline__ uint32_t nth_largest(const uint32_t *vals, int lane, int n) {
+    uint32_t mine[kBT / 32], hi = 0, lo = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < kBT / 32; j++) {
+        mine[j] = vals[lane + 32 * j];
+        hi = max(hi, mine[j]), lo = min(lo, mine[j]);
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi), lo = __reduce_min_sync(0xffffffffu, lo);
+    int bit = 31 - __clz(hi ^ lo);  // the bits above are common to all; -1: all equal
+    uint32_t t = bit < 0 ? hi : hi & ~((2u << bit) - 1u);
+    for (; bit >= 0; bit--) {
+        const uint32_t c = t | (1u << bit);
+        int k = 0;
+#pragma unroll
+        for (int j = 0; j < kBT / 32; j++) k += mine[j] >= c;
+        k = __reduce_add_sync(0xffffffffu, k);
+        if (k >= n) t = c;
+        if (k == n) break;
+    }
+    return max(t, 1u);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
-    __shared__ unsigned long long kmax[kBT], buf[kCap], T64_s;
+    constexpr int E = items<T>(), C = 16 / sizeof(T), CAP = kMaxOut * E;
+    __shared__ uint32_t vmax[kBT], T_s;
+    __shared__ unsigned long long buf[CAP], T64_s;
     __shared__ float red[kBT / 32];
     __shared__ double redd[kBT / 32];
     __shared__ int cnt_s;
     const int chunk = blockIdx.x, row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
     // the second kernel does not look at the lists of a finished or dead beam
     if ((a.finished && a.finished[row]) || !(a.scores[row] > -INFINITY)) return;
-    const int base = chunk * kChunk, nel = min(kChunk, a.vocab - base), n = min(a.n_out, nel);
+    const int base = chunk * a.chunk, nel = min(a.chunk, a.vocab - base), n = min(a.n_out, nel);
     const T *x = (const T *)a.logits + (int64_t)row * a.ld + base;
 
-    constexpr int C = 16 / sizeof(T), NV = kItems / C;
-    const bool vec = ((uintptr_t)x & 15) == 0;
-    float v[kItems];
+    float v[E];
+    if (((uintptr_t)x & 15) == 0 && nel == a.chunk) {
+        Chunk<T, C> raw[E / C];
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int e0 = (j * kBT + tid) * C;
-        float t[C];
-        if (vec && e0 + C <= nel) {
-            load_chunk<T, C>(x + e0, t);
+        for (int j = 0; j < E / C; j++) raw[j] = *(const Chunk<T, C> *)(x + (j * kBT + tid) * C);
 #pragma unroll
-            for (int i = 0; i < C; i++) v[j * C + i] = t[i];
-        } else {
+        for (int j = 0; j < E / C; j++) {
+            float t[C];
+            widen(raw[j], t);
 #pragma unroll
-            for (int i = 0; i < C; i++) v[j * C + i] = e0 + i < nel ? to_f32(x[e0 + i]) : 0.0f;
+            for (int i = 0; i < C; i++) v[j * C + i] = fmaxf(t[i], -INFINITY);  // NaN counts as -inf
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const int e = ((k / C) * kBT + tid) * C + k % C;
+            v[k] = e < nel ? fmaxf(to_f32(x[e]), -INFINITY) : -INFINITY;
         }
     }
-    auto index = [&](int k) { return ((k / C) * kBT + tid) * C + k % C; };  // place in the chunk
+    auto place = [&](int k) { return ((k / C) * kBT + tid) * C + k % C; };  // in the chunk
 
-    unsigned long long best = 0;
-    float m = -INFINITY;
+    float best = v[0];
 #pragma unroll
-    for (int k = 0; k < kItems; k++) {
-        if (index(k) >= nel) continue;
-        m = fmaxf(m, v[k]);  // fmaxf ignores NaN
-        const unsigned long long key = order_key(v[k], base + index(k));
-        best = key > best ? key : best;
-    }
-    kmax[tid] = best;
-    m = warp_max(m);
+    for (int k = 1; k < E; k++) best = fmaxf(best, v[k]);
+    const uint32_t mine = place(0) < nel ? order_bits(best) : 0u;  // a thread's first element comes before its others
+    vmax[tid] = mine;
+    float m = warp_max(best);
     if (lane == 0) red[warp] = m;
     if (tid == 0) cnt_s = 0;
     __syncthreads();
     m = red[0];
 #pragma unroll
     for (int w = 1; w < kBT / 32; w++) m = fmaxf(m, red[w]);
-    if (warp == 0) {  // T: the n-th largest of the threads' maxima, its upper 32 bits
-        uint32_t mine[kBT / 32], hi = 0, lo = 0xffffffffu;
-#pragma unroll
-        for (int j = 0; j < kBT / 32; j++) {
-            mine[j] = (uint32_t)(kmax[lane + 32 * j] >> 32);
-            hi = max(hi, mine[j]), lo = min(lo, mine[j]);
-        }
-        hi = __reduce_max_sync(0xffffffffu, hi), lo = __reduce_min_sync(0xffffffffu, lo);
-        int bit = 31 - __clz(hi ^ lo);  // the bits above are common to all; -1: all equal
-        uint32_t t = bit < 0 ? hi : hi & ~((2u << bit) - 1u);
-        for (; bit >= 0; bit--) {
-            const uint32_t c = t | (1u << bit);
-            int k = 0;
-#pragma unroll
-            for (int j = 0; j < kBT / 32; j++) k += mine[j] >= c;
-            k = __reduce_add_sync(0xffffffffu, k);
-            if (k >= n) t = c;
-            if (k == n) break;
-        }
-        if (lane == 0) T64_s = (unsigned long long)max(t, 1u) << 32;
+    if (warp == 0) {  // while the others take their exponentials
+        const uint32_t t = nth_largest(vmax, lane, n);
+        if (lane == 0) T_s = t;
     }
-    float s = 0.0f;  // every thread, while the first warp looks for T
-    if (m > -INFINITY) {
+    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (m == INFINITY) {  // the infinities share the probability
 #pragma unroll
-        for (int k = 0; k < kItems; k++)
-            if (index(k) < nel && v[k] == v[k]) s += v[k] == m ? 1.0f : expf(v[k] - m);
+        for (int k = 0; k < E; k++) s4[0] += v[k] == m ? 1.0f : 0.0f;
+    } else if (m > -INFINITY) {
+#pragma unroll
+        for (int k = 0; k < E; k++) s4[k & 3] += exp2f((v[k] - m) * 1.4426950408889634f);
     }
-    const double sd = warp_sum_d((double)s);
+    const double sd = warp_sum_d((double)((s4[0] + s4[1]) + (s4[2] + s4[3])));
     if (lane == 0) redd[warp] = sd;
     __syncthreads();
     if (tid == 0) {
@@ -130,31 +141,39 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
         for (int w = 0; w < kBT / 32; w++) tot += redd[w];
         a.stat[(int64_t)row * a.chunks + chunk] = make_float2(m, (float)tot);
     }
+    auto key_of = [&](int k) { return ((unsigned long long)order_bits(v[k]) << 32) | (uint32_t)~(base + place(k)); };
     auto collect = [&](unsigned long long least) {
-        if (best >= least) {
+        if (mine >= (uint32_t)(least >> 32)) {
 #pragma unroll
-            for (int k = 0; k < kItems; k++) {
-                if (index(k) >= nel) continue;
-                const unsigned long long key = order_key(v[k], base + index(k));
+            for (int k = 0; k < E; k++) {
+                if (place(k) >= nel) continue;
+                const unsigned long long key = key_of(k);
                 if (key >= least) {
                     const int at = atomicAdd(&cnt_s, 1);  // places differ from run to run, ranks do not
-                    if (at < kCap) buf[at] = key;
+                    if (at < CAP) buf[at] = key;
                 }
             }
         }
     };
-    collect(T64_s);
+    collect((unsigned long long)T_s << 32);
     __syncthreads();
     int cnt = cnt_s;
     __syncthreads();  // read by all before a second collection changes it
-    if (cnt > kCap) {  // many equal logits: the rest of T's bits, over the indices
+    if (cnt > CAP) {
+        // many equal logits: the threads' maxima with their indices are distinct; T's lower bits are built over those
+        unsigned long long top = 0;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+            if (place(k) < nel) top = max(top, key_of(k));
+        buf[tid] = top;
+        __syncthreads();
         if (warp == 0) {
-            unsigned long long t = T64_s;
+            unsigned long long t = (unsigned long long)T_s << 32;
             for (int bit = 31; bit >= 0; bit--) {
                 const unsigned long long c = t | (1ull << bit);
                 int k = 0;
 #pragma unroll
-                for (int j = 0; j < kBT / 32; j++) k += kmax[lane + 32 * j] >= c;
+                for (int j = 0; j < kBT / 32; j++) k += buf[lane + 32 * j] >= c;
                 if (__reduce_add_sync(0xffffffffu, k) >= n) t = c;
             }
             if (lane == 0) T64_s = t, cnt_s = 0;
@@ -162,7 +181,7 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
         __syncthreads();
         collect(T64_s);
         __syncthreads();
-        cnt = min(cnt_s, kCap);
+        cnt = min(cnt_s, CAP);
     }
     unsigned long long *out = a.cand + ((int64_t)row * a.chunks + chunk) * a.n_out;
     for (int i = tid; i < cnt; i += kBT) {
@@ -181,22 +200,25 @@ __device__ __forceinline__ int virtual_token(bool ended, int eos, int i) {
 
 struct Head {
     double score;
-    int64_t flat;  // beam * vocab + token; INT64_MAX: none
+    uint64_t at;  // beam << 32 | token: ordered as beam * vocab + token.  ~0: none
 };
 __device__ __forceinline__ bool before(const Head &a, const Head &b) {
-    return a.score > b.score || (a.score == b.score && a.flat < b.flat);
+    return a.score > b.score || (a.score == b.score && a.at < b.at);
 }
+constexpr int kMergeCap = 512;  // candidates that are ranked by counting
 
 __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
     __shared__ double lse_s[kMaxOut], cum_s[kMaxOut];
     __shared__ float top_s[kMaxOut];
     __shared__ uint8_t kind_s[kMaxOut];  // 0 logits, 1 finished, 2 dead
-    __shared__ double wsc[kBT / 32];
-    __shared__ int64_t wfl[kBT / 32];
-    __shared__ int wth[kBT / 32];
-    extern __shared__ int next_s[];  // [beams * chunks] entries taken of each list
+    __shared__ Head buf[kMergeCap];
+    __shared__ uint32_t vmax[kBT], T_s;
+    __shared__ int cnt_s, wth[kBT / 32];
+    extern __shared__ int next_s[];  // [beams * chunks] entries taken of each list (the rounds)
     const int prompt = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int lists = a.beams * a.chunks;
+    const int lists = a.beams * a.chunks, offered = min(a.n_out, a.vocab);
+    pdl_launch_dependents();
+    pdl_wait();
     for (int b = warp; b < a.beams; b += kBT / 32) {
         const int row = prompt * a.beams + b;
         const float cum = a.scores[row];
@@ -209,7 +231,7 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
             m = warp_max(m);
             for (int c = lane; c < a.chunks; c += 32) {
                 const float2 p = st[c];
-                if (p.x > -INFINITY) s += (double)p.y * (p.x == m ? 1.0 : exp((double)p.x - (double)m));
+                if (p.x > -INFINITY) s += (double)(p.y * (p.x == m ? 1.0f : exp2f((p.x - m) * 1.4426950408889634f)));
             }
             s = warp_sum_d(s);
         }
@@ -219,38 +241,80 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
             lse_s[b] = m == INFINITY ? log(s) : (double)m + log(s);
         }
     }
-    for (int i = tid; i < lists; i += kBT) next_s[i] = 0;
+    if (tid == 0) cnt_s = 0;
     __syncthreads();
 
-    auto head_of = [&](int list) {
-        Head h{-INFINITY, INT64_MAX};
-        const int b = list / a.chunks, c = list % a.chunks, i = next_s[list], kind = kind_s[b];
+    auto entry = [&](int list, int i) {  // the i-th of a list
+        Head h{-INFINITY, ~0ull};
+        const int b = list / a.chunks, c = list % a.chunks, kind = kind_s[b];
         if (kind) {
-            if (c == 0 && i < min(a.n_out, a.vocab)) {
-                h.flat = (int64_t)b * a.vocab + virtual_token(kind == 1, a.eos, i);
+            if (c == 0 && i < offered) {
+                h.at = (uint64_t)b << 32 | (uint32_t)virtual_token(kind == 1, a.eos, i);
                 if (kind == 1 && i == 0) h.score = cum_s[b];
             }
             return h;
         }
-        const int nel = min(kChunk, a.vocab - c * kChunk);
-        if (i >= min(a.n_out, nel)) return h;
+        if (i >= min(a.n_out, a.vocab - c * a.chunk)) return h;
+        if (i >= a.chunk) return h;
         const unsigned long long key = a.cand[((int64_t)(prompt * a.beams + b) * a.chunks + c) * a.n_out + i];
         const float x = order_value((uint32_t)(key >> 32));
-        h.flat = (int64_t)b * a.vocab + (int)~(uint32_t)key;
+        h.at = (uint64_t)b << 32 | (uint32_t)~(uint32_t)key;
         // with an infinite maximum lse is the log of the number of infinities
         if (top_s[b] == INFINITY) h.score = x == INFINITY ? cum_s[b] - lse_s[b] : -INFINITY;
         else h.score = cum_s[b] + ((double)x - lse_s[b]);
         if (h.score != h.score) h.score = -INFINITY;
         return h;
     };
-    Head mine{-INFINITY, INT64_MAX};
+    // the score rounded down to a float keeps the order; equal bits are settled by the whole score and the index
+    auto bits = [&](const Head &h) { return h.at == ~0ull ? 0u : order_bits(__double2float_rd(h.score)); };
+    auto put = [&](int r, const Head &h) {
+        const int64_t o = (int64_t)prompt * a.n_out + r;
+        a.parents[o] = (int)(h.at >> 32);
+        a.tokens[o] = (int)(uint32_t)h.at;
+        a.out_scores[o] = (float)h.score;
+    };
+    uint32_t best = 0;
+    for (int l = tid; l < lists; l += kBT) best = max(best, bits(entry(l, 0)));
+    vmax[tid] = best;
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t t = nth_largest(vmax, lane, a.n_out);
+        if (lane == 0) T_s = t;
+    }
+    __syncthreads();
+    const uint32_t least = T_s;
+    if (best >= least)
+        for (int l = tid; l < lists; l += kBT)
+            for (int i = 0; i < offered; i++) {
+                const Head h = entry(l, i);
+                if (bits(h) < least) break;
+                const int at = atomicAdd(&cnt_s, 1);
+                if (at < kMergeCap) buf[at] = h;
+                else break;
+            }
+    __syncthreads();
+    const int cnt = cnt_s;
+    if (cnt <= kMergeCap) {
+        for (int i = tid; i < cnt; i += kBT) {
+            const Head h = buf[i];
+            int rank = 0;
+            for (int j = 0; j < cnt; j++) rank += before(buf[j], h);
+            if (rank < a.n_out) put(rank, h);
+        }
+        return;
+    }
+
+    // many equal scores: n rounds of a maximum over the lists' heads, each thread's in registers
+    for (int i = tid; i < lists; i += kBT) next_s[i] = 0;
+    __syncthreads();
+    Head mine{-INFINITY, ~0ull};
     int my_list = -1;
     auto scan = [&]() {
-        mine = Head{-INFINITY, INT64_MAX};
+        mine = Head{-INFINITY, ~0ull};
         my_list = -1;
         for (int l = tid; l < lists; l += kBT) {
-            const Head h = head_of(l);
-            if (h.flat != INT64_MAX && (my_list < 0 || before(h, mine))) mine = h, my_list = l;
+            const Head h = entry(l, next_s[l]);
+            if (h.at != ~0ull && (my_list < 0 || before(h, mine))) mine = h, my_list = l;
         }
     };
     scan();
@@ -261,24 +325,17 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
         for (int o = 16; o; o >>= 1) {
             Head g;
             g.score = __shfl_xor_sync(0xffffffffu, h.score, o);
-            g.flat = __shfl_xor_sync(0xffffffffu, h.flat, o);
+            g.at = __shfl_xor_sync(0xffffffffu, h.at, o);
             const int gt = __shfl_xor_sync(0xffffffffu, th, o);
             if (before(g, h)) h = g, th = gt;
         }
-        if (lane == 0) wsc[warp] = h.score, wfl[warp] = h.flat, wth[warp] = th;
+        if (lane == 0) buf[warp] = h, wth[warp] = th;
         __syncthreads();
-        h = Head{wsc[0], wfl[0]}, th = wth[0];
+        h = buf[0], th = wth[0];
 #pragma unroll
-        for (int w = 1; w < kBT / 32; w++) {
-            const Head g{wsc[w], wfl[w]};
-            if (before(g, h)) h = g, th = wth[w];
-        }
-        if (tid == 0) {
-            const int64_t o = (int64_t)prompt * a.n_out + r;
-            a.parents[o] = (int)(h.flat / a.vocab);
-            a.tokens[o] = (int)(h.flat % a.vocab);
-            a.out_scores[o] = (float)h.score;
-        }
+        for (int w = 1; w < kBT / 32; w++)
+            if (before(buf[w], h)) h = buf[w], th = wth[w];
+        if (tid == 0) put(r, h);
         if (tid == th && my_list >= 0) {
             next_s[my_list]++;
             scan();
@@ -291,17 +348,18 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
 struct ReorderArgs {
     uint8_t *pool[2];
     int64_t layer_bytes, page_bytes, slot_bytes;
-    int n_pages, page_size, beams, ld_parents, ld_table;
+    int n_pages, page_size, beams, ld_parents, ld_table, pools;  // pools: of all layers, k and v
     const int *parents, *lens, *tin;
     int *tout, *err;
 };
 
-// blockIdx.x: row; blockIdx.y: 2 * layer + (k or v).  Every block works out its beam's parent and pages from the prompt's
-// parents; the first of a row writes the table.
+// blockIdx.x: row; blockIdx.y, + gridDim.y, ...: 2 * layer + (k or v).  Every block works out its beam's parent and pages from the
+// prompt's parents; the first of a row writes the table.
 __global__ void __launch_bounds__(kBT) beam_reorder_kernel(const ReorderArgs a) {
     __shared__ int par[kMaxOut];
     __shared__ uint8_t has[kMaxOut], first[kMaxOut];
     const int row = blockIdx.x, prompt = row / a.beams, j = row % a.beams, tid = threadIdx.x;
+    pdl_wait();
     int n = a.lens[prompt * a.beams];
     if (n < 0) {
         if (tid == 0) raise_error(a.err, kErrBadIndex);
@@ -348,18 +406,21 @@ __global__ void __launch_bounds__(kBT) beam_reorder_kernel(const ReorderArgs a) 
         if (tid == 0) raise_error(a.err, kErrBadIndex);
         return;
     }
-    uint8_t *pool = a.pool[blockIdx.y & 1] + (int64_t)(blockIdx.y >> 1) * a.layer_bytes;
-    const uint8_t *s = pool + src * a.page_bytes;
-    uint8_t *d = pool + dst * a.page_bytes;
     const int64_t bytes = filled * a.slot_bytes;
-    if ((((uintptr_t)s | (uintptr_t)d | (uintptr_t)bytes) & 15) == 0) {
-        for (int64_t i = tid; i < bytes / 16; i += kBT) ((uint4 *)d)[i] = ((const uint4 *)s)[i];
-    } else {
-        for (int64_t i = tid; i < bytes / 2; i += kBT) ((uint16_t *)d)[i] = ((const uint16_t *)s)[i];
+    for (int y = blockIdx.y; y < a.pools; y += gridDim.y) {
+        uint8_t *pool = a.pool[y & 1] + (int64_t)(y >> 1) * a.layer_bytes;
+        const uint8_t *s = pool + src * a.page_bytes;
+        uint8_t *d = pool + dst * a.page_bytes;
+        if ((((uintptr_t)s | (uintptr_t)d | (uintptr_t)bytes) & 15) == 0) {
+#pragma unroll 4
+            for (int64_t i = tid; i < bytes / 16; i += kBT) ((uint4 *)d)[i] = __ldcs((const uint4 *)s + i);
+        } else {
+            for (int64_t i = tid; i < bytes / 2; i += kBT) ((uint16_t *)d)[i] = ((const uint16_t *)s)[i];
+        }
     }
 }
 
-int beam_chunks(int vocab) { return (vocab + kChunk - 1) / kChunk; }
+int beam_chunks(int vocab, int chunk) { return (vocab + chunk - 1) / chunk; }
 size_t beam_stat_bytes(int64_t rows, int chunks) { return ((size_t)rows * chunks * sizeof(float2) + 255) / 256 * 256; }
 
 int check_beams(const char *op, int64_t prompts, int beams, int vocab, int n_out) {
@@ -368,7 +429,7 @@ int check_beams(const char *op, int64_t prompts, int beams, int vocab, int n_out
     if (n_out < 1 || n_out > kMaxOut || n_out > (int64_t)beams * vocab) return set_error(QMC_EINVAL, "%s: n_out %d", op, n_out);
     if (prompts * beams > 65535) return set_error(QMC_EINVAL, "%s: %lld rows exceed 65535", op, (long long)prompts * beams);
     // the merge keeps one counter a list in shared memory
-    if ((int64_t)beams * beam_chunks(vocab) > 10240)
+    if ((int64_t)beams * beam_chunks(vocab, kLeast) > 8192)
         return set_error(QMC_EINVAL, "%s: %d beams over a vocabulary of %d are too many", op, beams, vocab);
     return QMC_OK;
 }
@@ -385,7 +446,7 @@ int qmc_beam_workspace(int32_t n_prompts, int32_t beams, int32_t n_vocab, int32_
     *bytes = 0;
     if (const int rc = check_beams("beam_workspace", n_prompts, beams, n_vocab, n_out)) return rc;
     const int64_t rows = (int64_t)n_prompts * beams;
-    const int chunks = beam_chunks(n_vocab);
+    const int chunks = beam_chunks(n_vocab, kLeast);  // whatever the logits' type
     *bytes = beam_stat_bytes(rows, chunks) + (size_t)rows * chunks * n_out * 8 + 256;
     return QMC_OK;
 }
@@ -409,7 +470,8 @@ int qmc_beam_select(int dtype, const void *logits, int64_t ld, int32_t n_prompts
     if (!c) return QMC_ECUDA;
     SelArgs a{};
     a.logits = logits, a.ld = ld, a.prompts = n_prompts, a.beams = beams, a.vocab = n_vocab, a.n_out = n_out, a.eos = eos_token;
-    a.chunks = beam_chunks(n_vocab);
+    a.chunk = dtype == QMC_F32 ? kLeast : 2 * kLeast;
+    a.chunks = beam_chunks(n_vocab, a.chunk);
     a.scores = scores, a.finished = finished;
     const int64_t rows = (int64_t)n_prompts * beams;
     uint8_t *w = (uint8_t *)(((uintptr_t)workspace + 255) / 256 * 256);
@@ -422,9 +484,7 @@ int qmc_beam_select(int dtype, const void *logits, int64_t ld, int32_t n_prompts
     else if (dtype == QMC_F16) beam_chunk_kernel<__half><<<grid, kBT, 0, s>>>(a);
     else beam_chunk_kernel<__nv_bfloat16><<<grid, kBT, 0, s>>>(a);
     QMC_LAUNCH_CHECK();
-    beam_merge_kernel<<<n_prompts, kBT, (size_t)beams * a.chunks * 4, s>>>(a);
-    QMC_LAUNCH_CHECK();
-    return QMC_OK;
+    return launch_after(beam_merge_kernel, dim3(n_prompts), kBT, beams * a.chunks * 4, s, true, a);
 }
 
 int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t beams, const int32_t *parents,
@@ -435,7 +495,7 @@ int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t be
     if (n_prompts < 0 || beams < 1 || beams > kMaxOut || ld_parents < beams || ld_table < 1)
         return set_error(QMC_EINVAL, "%s: %d prompts of %d beams, parents %d apart, table %d wide", op, n_prompts, beams,
                          ld_parents, ld_table);
-    if (cache->n_layers > 32767) return set_error(QMC_EINVAL, "%s: %d layers exceed the grid", op, cache->n_layers);
+    if (cache->n_layers > 1 << 20) return set_error(QMC_EINVAL, "%s: %d layers", op, cache->n_layers);
     if ((int64_t)n_prompts * beams > INT32_MAX) return set_error(QMC_EINVAL, "%s: too many rows", op);
     if (n_prompts == 0) return QMC_OK;
     if (!parents || !seq_lens || !page_table || !page_table_out) return set_error(QMC_EINVAL, "%s: null argument", op);
@@ -451,9 +511,12 @@ int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t be
     a.n_pages = cache->n_pages, a.page_size = cache->page_size, a.beams = beams;
     a.ld_parents = ld_parents, a.ld_table = ld_table;
     a.parents = parents, a.lens = seq_lens, a.tin = page_table, a.tout = page_table_out, a.err = c->err;
-    beam_reorder_kernel<<<dim3((unsigned)n_prompts * beams, 2u * cache->n_layers), kBT, 0, pick_stream(stream)>>>(a);
-    QMC_LAUNCH_CHECK();
-    return QMC_OK;
+    // a third of the beams copy: enough blocks of them to fill the SMs, each with several pools.  It may start while the
+    // selection before it ends, and reads nothing before it has ended.
+    a.pools = 2 * cache->n_layers;
+    const int64_t rows = (int64_t)n_prompts * beams, want = (16 * c->num_sms + rows - 1) / rows;
+    const dim3 grid((unsigned)rows, (unsigned)(want < a.pools ? want : a.pools));
+    return launch_after(beam_reorder_kernel, grid, kBT, 0, pick_stream(stream), true, a);
 }
 
 }  // extern "C"
