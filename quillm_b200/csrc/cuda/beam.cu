@@ -48,6 +48,11 @@ __device__ __forceinline__ float order_value(uint32_t u) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
+__device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22; below 2^-126 it is 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // by one warp: the largest T that at least n of the 256 values reach (their n-th largest, or a value above it that exactly n
 // reach), at least 1
 __device__ __forceinline__ uint32_t nth_largest(const uint32_t *vals, int lane, int n) {
@@ -98,20 +103,20 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
             float t[C];
             widen(raw[j], t);
 #pragma unroll
-            for (int i = 0; i < C; i++) v[j * C + i] = fmaxf(t[i], -INFINITY);  // NaN counts as -inf
+            for (int i = 0; i < C; i++) v[j * C + i] = t[i];
         }
     } else {
 #pragma unroll
         for (int k = 0; k < E; k++) {
             const int e = ((k / C) * kBT + tid) * C + k % C;
-            v[k] = e < nel ? fmaxf(to_f32(x[e]), -INFINITY) : -INFINITY;
+            v[k] = e < nel ? to_f32(x[e]) : -INFINITY;
         }
     }
     auto place = [&](int k) { return ((k / C) * kBT + tid) * C + k % C; };  // in the chunk
 
-    float best = v[0];
+    float best = -INFINITY;  // NaN counts as -inf: maxima pass it over
 #pragma unroll
-    for (int k = 1; k < E; k++) best = fmaxf(best, v[k]);
+    for (int k = 0; k < E; k++) best = fmaxf(best, v[k]);
     const uint32_t mine = place(0) < nel ? order_bits(best) : 0u;  // a thread's first element comes before its others
     vmax[tid] = mine;
     float m = warp_max(best);
@@ -131,9 +136,15 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
         for (int k = 0; k < E; k++) s4[0] += v[k] == m ? 1.0f : 0.0f;
     } else if (m > -INFINITY) {
 #pragma unroll
-        for (int k = 0; k < E; k++) s4[k & 3] += exp2f((v[k] - m) * 1.4426950408889634f);
+        for (int k = 0; k < E; k++) s4[k & 3] += ex2((v[k] - m) * 1.4426950408889634f);
     }
-    const double sd = warp_sum_d((double)((s4[0] + s4[1]) + (s4[2] + s4[3])));
+    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    if (s != s) {  // some NaN among them
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < E; k++) s += v[k] == v[k] ? ex2((v[k] - m) * 1.4426950408889634f) : 0.0f;
+    }
+    const double sd = warp_sum_d((double)s);
     if (lane == 0) redd[warp] = sd;
     __syncthreads();
     if (tid == 0) {
@@ -141,11 +152,16 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
         for (int w = 0; w < kBT / 32; w++) tot += redd[w];
         a.stat[(int64_t)row * a.chunks + chunk] = make_float2(m, (float)tot);
     }
-    auto key_of = [&](int k) { return ((unsigned long long)order_bits(v[k]) << 32) | (uint32_t)~(base + place(k)); };
+    auto key_of = [&](int k) { return ((unsigned long long)order_bits(fmaxf(v[k], -INFINITY)) << 32) | (uint32_t)~(base + place(k)); };
     auto collect = [&](unsigned long long least) {
         if (mine >= (uint32_t)(least >> 32)) {
+            // T as a float, for one comparison an element; where -inf and NaN reach it, all do
+            const uint32_t bits = (uint32_t)(least >> 32);
+            const bool any = bits <= order_bits(-INFINITY);
+            const float value = any ? -INFINITY : order_value(bits);
 #pragma unroll
             for (int k = 0; k < E; k++) {
+                if (!(v[k] >= value) && !any) continue;
                 if (place(k) >= nel) continue;
                 const unsigned long long key = key_of(k);
                 if (key >= least) {
@@ -231,7 +247,7 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
             m = warp_max(m);
             for (int c = lane; c < a.chunks; c += 32) {
                 const float2 p = st[c];
-                if (p.x > -INFINITY) s += (double)(p.y * (p.x == m ? 1.0f : exp2f((p.x - m) * 1.4426950408889634f)));
+                if (p.x > -INFINITY) s += (double)(p.y * (p.x == m ? 1.0f : ex2((p.x - m) * 1.4426950408889634f)));
             }
             s = warp_sum_d(s);
         }
@@ -348,12 +364,12 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
 struct ReorderArgs {
     uint8_t *pool[2];
     int64_t layer_bytes, page_bytes, slot_bytes;
-    int n_pages, page_size, beams, ld_parents, ld_table, pools;  // pools: of all layers, k and v
+    int n_pages, page_size, beams, ld_parents, ld_table, layers;
     const int *parents, *lens, *tin;
     int *tout, *err;
 };
 
-// blockIdx.x: row; blockIdx.y, + gridDim.y, ...: 2 * layer + (k or v).  Every block works out its beam's parent and pages from the
+// blockIdx.x: row; blockIdx.y, + gridDim.y, ...: layer.  Every block works out its beam's parent and pages from the
 // prompt's parents; the first of a row writes the table.
 __global__ void __launch_bounds__(kBT) beam_reorder_kernel(const ReorderArgs a) {
     __shared__ int par[kMaxOut];
@@ -407,15 +423,27 @@ __global__ void __launch_bounds__(kBT) beam_reorder_kernel(const ReorderArgs a) 
         return;
     }
     const int64_t bytes = filled * a.slot_bytes;
-    for (int y = blockIdx.y; y < a.pools; y += gridDim.y) {
-        uint8_t *pool = a.pool[y & 1] + (int64_t)(y >> 1) * a.layer_bytes;
-        const uint8_t *s = pool + src * a.page_bytes;
-        uint8_t *d = pool + dst * a.page_bytes;
-        if ((((uintptr_t)s | (uintptr_t)d | (uintptr_t)bytes) & 15) == 0) {
-#pragma unroll 4
-            for (int64_t i = tid; i < bytes / 16; i += kBT) ((uint4 *)d)[i] = __ldcs((const uint4 *)s + i);
+    for (int y = blockIdx.y; y < a.layers; y += gridDim.y) {
+        const int64_t from_at = y * a.layer_bytes + src * a.page_bytes, to_at = y * a.layer_bytes + dst * a.page_bytes;
+        uint8_t *const k = a.pool[0], *const v = a.pool[1];
+        if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)from_at | (uintptr_t)to_at | (uintptr_t)bytes) & 15) == 0) {
+            const int64_t n = bytes / 16;
+            const uint4 *ks = (const uint4 *)(k + from_at), *vs = (const uint4 *)(v + from_at);
+            uint4 *kd = (uint4 *)(k + to_at), *vd = (uint4 *)(v + to_at);
+            for (int64_t i = tid; i < n; i += 4 * kBT) {  // eight loads on their way
+                uint4 x[4], z[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (i + u * kBT < n) x[u] = __ldcs(ks + i + u * kBT), z[u] = __ldcs(vs + i + u * kBT);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (i + u * kBT < n) kd[i + u * kBT] = x[u], vd[i + u * kBT] = z[u];
+            }
         } else {
-            for (int64_t i = tid; i < bytes / 2; i += kBT) ((uint16_t *)d)[i] = ((const uint16_t *)s)[i];
+            for (int64_t i = tid; i < bytes / 2; i += kBT) {
+                ((uint16_t *)(k + to_at))[i] = ((const uint16_t *)(k + from_at))[i];
+                ((uint16_t *)(v + to_at))[i] = ((const uint16_t *)(v + from_at))[i];
+            }
         }
     }
 }
@@ -511,11 +539,11 @@ int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t be
     a.n_pages = cache->n_pages, a.page_size = cache->page_size, a.beams = beams;
     a.ld_parents = ld_parents, a.ld_table = ld_table;
     a.parents = parents, a.lens = seq_lens, a.tin = page_table, a.tout = page_table_out, a.err = c->err;
-    // a third of the beams copy: enough blocks of them to fill the SMs, each with several pools.  It may start while the
+    // a third of the beams copy: enough blocks of them to fill the SMs, each with several layers.  It may start while the
     // selection before it ends, and reads nothing before it has ended.
-    a.pools = 2 * cache->n_layers;
+    a.layers = cache->n_layers;
     const int64_t rows = (int64_t)n_prompts * beams, want = (16 * c->num_sms + rows - 1) / rows;
-    const dim3 grid((unsigned)rows, (unsigned)(want < a.pools ? want : a.pools));
+    const dim3 grid((unsigned)rows, (unsigned)(want < a.layers ? want : a.layers));
     return launch_after(beam_reorder_kernel, grid, kBT, 0, pick_stream(stream), true, a);
 }
 
