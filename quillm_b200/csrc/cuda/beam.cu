@@ -7,11 +7,15 @@
 // turns out to be.  The second, one block per prompt, joins a row's (m, sum) pairs in double and takes the n best of the rows'
 // sorted lists.
 //
-// The n best, in both: the n-th largest of the 256 threads' maxima is a lower bound T that at least n elements reach, found
-// by building the bits of its 32-bit order-preserving form from the top in one warp; the few elements >= T are collected in shared
-// memory and ranked by counting, with the index, so that ties go to the lower one.  Where too many reach T (equal logits), the
-// chunk continues T's bits over the indices, after which at most n threads' elements remain, and the second kernel takes n rounds
-// of a block-wide maximum over the lists' heads.
+// The n best of a chunk: with w warps, the smallest of the warps' ceil(n / w)-th largest thread maxima is a lower bound T that at
+// least n elements reach, found in a few warp-wide maxima (in the 32-bit order-preserving form); the few elements >= T are
+// collected in shared memory and ranked by counting, with the index, so that ties go to the lower one.  Where too many reach T
+// (equal logits), the exact n-th largest of the threads' maxima is built from the top bit, and its bits continued over the indices, after
+// which at most n threads' elements remain.  Blocks stay and take chunk after chunk, the next one's logits on their way to registers.
+// Of the lists' heads, whose beams' scores lie apart, the exact n-th largest is taken at once; where too many reach it, n rounds of a
+// block-wide maximum over the heads.
+#include <algorithm>
+
 #include "attn_prefix.cuh"
 
 namespace qmc {
@@ -19,8 +23,9 @@ namespace {
 
 constexpr int kBT = 256;      // threads
 constexpr int kMaxOut = 64;   // n_out and beams
+constexpr int kGroups = 256;  // 16-byte groups of logits of a chunk that may reach the bound before it counts as one with too many
 constexpr int kLeast = 4096;  // logits of the smallest chunk
-// logits per thread: four 16-byte loads
+// logits per thread: 4 16-byte loads
 template <typename T>
 __host__ __device__ constexpr int items() {
     return 64 / sizeof(T);
@@ -77,59 +82,106 @@ __device__ __forceinline__ uint32_t nth_largest(const uint32_t *vals, int lane, 
     return max(t, 1u);
 }
 
+// the k-th largest of the warp's values (0: there are fewer)
+__device__ __forceinline__ uint32_t warp_kth(uint32_t v, int lane, int k) {
+    uint32_t mx = 0;
+    for (int r = 0; r < k; r++) {
+        mx = __reduce_max_sync(0xffffffffu, v);
+        const unsigned holders = __ballot_sync(0xffffffffu, v == mx);
+        if (lane == __ffs(holders) - 1) v = 0;
+    }
+    return mx;
+}
+// how many of the warps' largest make n together, and over how many warps, when the first `threads` threads have a value; no warp: no
+// bound
+__device__ __forceinline__ int kth_of(int threads, int n, int &warps) {
+    warps = min(threads, kBT) / 32;
+    const int k = warps ? (n + warps - 1) / warps : 33;
+    if (k > 32) warps = 0;
+    return k;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
+__global__ void __launch_bounds__(kBT, 3) beam_chunk_kernel(const SelArgs a) {
     constexpr int E = items<T>(), C = 16 / sizeof(T), CAP = kMaxOut * E;
-    __shared__ uint32_t vmax[kBT], T_s;
+    __shared__ uint32_t vmax[kBT], kth[kBT / 32];
     __shared__ unsigned long long buf[CAP], T64_s;
+    __shared__ float gval[kGroups][C];  // 16-byte groups that reach the bound
+    __shared__ int gat[kGroups], groups_s;
     __shared__ float red[kBT / 32];
     __shared__ double redd[kBT / 32];
     __shared__ int cnt_s;
-    const int chunk = blockIdx.x, row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_launch_dependents();
+    const int total = a.prompts * a.beams * a.chunks;
     // the second kernel does not look at the lists of a finished or dead beam
-    if ((a.finished && a.finished[row]) || !(a.scores[row] > -INFINITY)) return;
-    const int base = chunk * a.chunk, nel = min(a.chunk, a.vocab - base), n = min(a.n_out, nel);
-    const T *x = (const T *)a.logits + (int64_t)row * a.ld + base;
-
-    float v[E];
-    if (((uintptr_t)x & 15) == 0 && nel == a.chunk) {
-        Chunk<T, C> raw[E / C];
-#pragma unroll
-        for (int j = 0; j < E / C; j++) raw[j] = *(const Chunk<T, C> *)(x + (j * kBT + tid) * C);
+    auto live_row = [&](int item) {
+        if (item >= total) return false;
+        const int row = item / a.chunks;
+        const bool ended = a.finished && a.finished[row];
+        return a.scores[row] > -INFINITY && !ended;
+    };
+    Chunk<T, C> raw[E / C] = {};
+    auto fetch = [&](int item) {  // -inf past the end
+        const int row = item / a.chunks, base = item % a.chunks * a.chunk, nel = min(a.chunk, a.vocab - base);
+        const T *x = (const T *)a.logits + (int64_t)row * a.ld + base;
+        const bool vec = ((uintptr_t)x & 15) == 0;
 #pragma unroll
         for (int j = 0; j < E / C; j++) {
-            float t[C];
-            widen(raw[j], t);
+            const int e = (j * kBT + tid) * C;
+            if (vec && e + C <= nel) {
+                raw[j] = *(const Chunk<T, C> *)(x + e);
+            } else {
 #pragma unroll
-            for (int i = 0; i < C; i++) v[j * C + i] = t[i];
+                for (int i = 0; i < C; i++) {
+                    if (e + i < nel) raw[j].e[i] = x[e + i];
+                    else from_f32(-INFINITY, &raw[j].e[i]);
+                }
+            }
         }
-    } else {
-#pragma unroll
-        for (int k = 0; k < E; k++) {
-            const int e = ((k / C) * kBT + tid) * C + k % C;
-            v[k] = e < nel ? to_f32(x[e]) : -INFINITY;
-        }
-    }
+    };
+    bool live = live_row(blockIdx.x), live_next = live_row(blockIdx.x + gridDim.x);
+    if (live) fetch(blockIdx.x);
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    const bool now = live;
+    const int chunk = item % a.chunks, row = item / a.chunks;
+    const int base = chunk * a.chunk, nel = min(a.chunk, a.vocab - base), n = min(a.n_out, nel);
     auto place = [&](int k) { return ((k / C) * kBT + tid) * C + k % C; };  // in the chunk
-
-    float best = -INFINITY;  // NaN counts as -inf: maxima pass it over
+    float v[E];
 #pragma unroll
-    for (int k = 0; k < E; k++) best = fmaxf(best, v[k]);
+    for (int j = 0; j < E / C; j++) {
+        float t[C];
+        widen(raw[j], t);
+#pragma unroll
+        for (int i = 0; i < C; i++) v[j * C + i] = t[i];
+    }
+    live = live_next;
+    if (live) fetch(item + gridDim.x);
+    live_next = live_row(item + 2 * gridDim.x);
+    if (!now) continue;
+
+    float top[E / C], best = -INFINITY;  // NaN counts as -inf: maxima pass it over
+#pragma unroll
+    for (int j = 0; j < E / C; j++) {
+        top[j] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < C; i++) top[j] = fmaxf(top[j], v[j * C + i]);
+        best = fmaxf(best, top[j]);
+    }
     const uint32_t mine = place(0) < nel ? order_bits(best) : 0u;  // a thread's first element comes before its others
-    vmax[tid] = mine;
+    int warps;
+    const int k_each = kth_of((nel + C - 1) / C, n, warps);
+    const uint32_t my_kth = warps ? warp_kth(mine, lane, k_each) : 0u;
     float m = warp_max(best);
-    if (lane == 0) red[warp] = m;
-    if (tid == 0) cnt_s = 0;
+    if (lane == 0) red[warp] = m, kth[warp] = my_kth;
+    if (tid == 0) cnt_s = groups_s = 0;
     __syncthreads();
     m = red[0];
 #pragma unroll
     for (int w = 1; w < kBT / 32; w++) m = fmaxf(m, red[w]);
-    if (warp == 0) {  // while the others take their exponentials
-        const uint32_t t = nth_largest(vmax, lane, n);
-        if (lane == 0) T_s = t;
-    }
+    uint32_t bound = 0xffffffffu;  // T
+    for (int w = 0; w < warps; w++) bound = min(bound, kth[w]);
+    bound = warps ? max(bound, 1u) : 1u;
     float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (m == INFINITY) {  // the infinities share the probability
 #pragma unroll
@@ -160,20 +212,50 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
             const bool any = bits <= order_bits(-INFINITY);
             const float value = any ? -INFINITY : order_value(bits);
 #pragma unroll
-            for (int k = 0; k < E; k++) {
-                if (!(v[k] >= value) && !any) continue;
-                if (place(k) >= nel) continue;
-                const unsigned long long key = key_of(k);
-                if (key >= least) {
-                    const int at = atomicAdd(&cnt_s, 1);  // places differ from run to run, ranks do not
-                    if (at < CAP) buf[at] = key;
+            for (int j = 0; j < E / C; j++) {
+                if (!(top[j] >= value)) continue;
+#pragma unroll
+                for (int i = 0; i < C; i++) {
+                    const int k = j * C + i;
+                    if (!(v[k] >= value) && !any) continue;
+                    if (place(k) >= nel) continue;
+                    const unsigned long long key = key_of(k);
+                    if (key >= least) {
+                        const int at = atomicAdd(&cnt_s, 1);  // places differ from run to run, ranks do not
+                        if (at < CAP) buf[at] = key;
+                    }
                 }
             }
         }
     };
-    collect((unsigned long long)T_s << 32);
+    // first the 16-byte groups that reach the bound, then, an element a thread, what of them does.  -inf never does: where fewer than
+    // n others exist, every element is looked at below
+    const float value = bound <= order_bits(-INFINITY) ? -INFINITY : order_value(bound);
+    if (best >= value) {
+#pragma unroll
+        for (int j = 0; j < E / C; j++)
+            if (top[j] >= value && place(j * C) < nel) {
+                const int at = atomicAdd(&groups_s, 1);  // places differ from run to run, ranks do not
+                if (at < kGroups) {
+                    gat[at] = place(j * C);
+#pragma unroll
+                    for (int i = 0; i < C; i++) gval[at][i] = v[j * C + i];
+                }
+            }
+    }
     __syncthreads();
-    int cnt = cnt_s;
+    const int groups = groups_s;
+    if (groups <= kGroups)
+        for (int i = tid; i < groups * C; i += kBT) {
+            const float y = gval[i / C][i % C];
+            const int at = gat[i / C] + i % C;
+            if ((y >= value || value == -INFINITY) && at < nel) {
+                const int to = atomicAdd(&cnt_s, 1);
+                if (to < CAP) buf[to] = ((unsigned long long)order_bits(fmaxf(y, -INFINITY)) << 32) | (uint32_t)~(base + at);
+            }
+        }
+    __syncthreads();
+    int cnt = groups <= kGroups ? cnt_s : CAP + 1;
     __syncthreads();  // read by all before a second collection changes it
     if (cnt > CAP) {
         // many equal logits: the threads' maxima with their indices are distinct; T's lower bits are built over those
@@ -181,10 +263,10 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
 #pragma unroll
         for (int k = 0; k < E; k++)
             if (place(k) < nel) top = max(top, key_of(k));
-        buf[tid] = top;
+        buf[tid] = top, vmax[tid] = mine;
         __syncthreads();
         if (warp == 0) {
-            unsigned long long t = (unsigned long long)T_s << 32;
+            unsigned long long t = (unsigned long long)nth_largest(vmax, lane, n) << 32;
             for (int bit = 31; bit >= 0; bit--) {
                 const unsigned long long c = t | (1ull << bit);
                 int k = 0;
@@ -205,6 +287,8 @@ __global__ void __launch_bounds__(kBT) beam_chunk_kernel(const SelArgs a) {
         int rank = 0;
         for (int j = 0; j < cnt; j++) rank += buf[j] > key;
         if (rank < n) out[rank] = key;
+    }
+    __syncthreads();  // before the next chunk
     }
 }
 
@@ -507,7 +591,7 @@ int qmc_beam_select(int dtype, const void *logits, int64_t ld, int32_t n_prompts
     a.cand = (unsigned long long *)(w + beam_stat_bytes(rows, a.chunks));
     a.parents = parents, a.tokens = tokens, a.out_scores = out_scores;
     cudaStream_t s = pick_stream(stream);
-    const dim3 grid(a.chunks, (unsigned)rows);
+    const int grid = (int)std::min<int64_t>(rows * a.chunks, 3 * c->num_sms);
     if (dtype == QMC_F32) beam_chunk_kernel<float><<<grid, kBT, 0, s>>>(a);
     else if (dtype == QMC_F16) beam_chunk_kernel<__half><<<grid, kBT, 0, s>>>(a);
     else beam_chunk_kernel<__nv_bfloat16><<<grid, kBT, 0, s>>>(a);
