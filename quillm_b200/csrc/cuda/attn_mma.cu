@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(128) attn_mma_kernel(const AttnArgs a) {
     pdl_launch_dependents();
     if (WM > 1 && jb.b < 0) mma_job<T, CT, HDP, WM>(a, jb, sm, sc);
     else mma_job<T, CT, HDP, 1>(a, jb, sm, sc);
-    pdl_wait();  // launched beside the prefix's kernel, this one ends after it: the join waits for this one
+    // launched beside the prefix's kernel, this grid ends after it, which the join relies on: one block waits, the others make room
+    if (blockIdx.x == 0) pdl_wait();
 }
 
 template <typename T, typename CT, int HDP, int WM>

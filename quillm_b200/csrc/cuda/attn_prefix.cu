@@ -233,8 +233,24 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
     const Shape &ps = shape[p.pkind], &os = shape[p.okind];
     p.ptiles = ceil_div(p.rows, ps.ptile);
     p.gtiles = ceil_div(group, os.otile);
-    if (prefix) p.psplit = split_for((int64_t)kv * p.ptiles, ceil_div(prefix, ps.quantum), ps.blocks * sms);
     if (own) p.osplit = split_for((int64_t)n_seq * kv * p.gtiles, ceil_div(own, os.quantum), os.blocks * sms);
+    const int64_t units = (int64_t)kv * p.ptiles;
+    if (prefix && p.pkind == kTcKernel && own) {
+        // The tensor-core blocks take whole SMs; the own jobs run on what they leave, and on all SMs afterwards.  Of the numbers
+        // of ranges the one that ends first, with a block's tile 2.0 us for two row tiles and 1.2 us for one, three more for
+        // its start and end, and an own job 4 us and 1 us for every 64 positions of half the longest, two at once on an SM.
+        const double tile = p.rows > 128 ? 2.0 : 1.2;
+        const double job = 4.0 + 0.5 * ceil_div(own, 64) / p.osplit, work = 0.5 * job * n_seq * kv * p.gtiles * p.osplit;
+        double least = 1e30;
+        for (int n = 1; n <= std::min(kMostSplits, ceil_div(prefix, 128)); n++) {
+            const int64_t blocks = units * n, left = sms - std::min<int64_t>(sms, blocks - (blocks - 1) / sms * sms);
+            const double tc = tile * ((blocks + sms - 1) / sms) * (ceil_div(ceil_div(prefix, 128), n) + kBlockTiles);
+            const double end = tc + std::max(0.0, work - left * tc) / sms;
+            if (end < least) least = end, p.psplit = n;
+        }
+    } else if (prefix) {
+        p.psplit = split_for(units, ceil_div(prefix, ps.quantum), ps.blocks * sms);
+    }
     p.pparts = p.psplit;
     const int64_t parts = p.pparts + p.osplit, all = (int64_t)n_seq * n_heads;
     p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;

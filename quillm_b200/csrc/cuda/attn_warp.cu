@@ -65,6 +65,35 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
     pdl_launch_dependents();
     const int hd = a.hd, nch = hd / 8;
 
+    // the next group's keys are loaded as soon as this one's scores are formed, its values as soon as this one's are used
+    auto locate = [&](int p0) {  // elements from the pool's start of position p0 + lane % 16, -1: none
+        const int64_t slot = p0 + (lane & 15) < jb.p1 ? slot_of(a, jb.b, p0 + (lane & 15)) : -1;
+        return slot >= 0 ? (slot * a.kv + jb.h) * hd : (int64_t)-1;
+    };
+    uint4 k[2][NU], v[4][NC];
+    auto load_k = [&](int64_t at) {
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const int64_t s = __shfl_sync(0xffffffffu, at, g + 8 * n);
+#pragma unroll
+            for (int u = 0; u < NU; u++)
+                k[n][u] = s >= 0 && t + 4 * u < nch ? load_stream((const CT *)a.kc + s + 8 * (t + 4 * u)) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto load_v = [&](int64_t at) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t s = __shfl_sync(0xffffffffu, at, 2 * t + (i & 1) + 4 * (i & 2));
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                v[i][c] = s >= 0 && g + 8 * c < nch ? load_stream((const CT *)a.vc + s + 8 * (g + 8 * c)) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    int64_t at = locate(jb.p0 + 16 * warp);
+    load_k(at);
+    load_v(at);
+    at = locate(jb.p0 + 16 * warp + 64);
+
     uint32_t q[H][2 * NU][4];
     float scale[2];  // of rows g and g + 8
 #pragma unroll
@@ -109,34 +138,6 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
         for (int j = 0; j < 8; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) o[c][j][i] = 0.0f;
-    // the next group's keys are loaded as soon as this one's scores are formed, its values as soon as this one's are used
-    auto locate = [&](int p0) {  // elements from the pool's start of position p0 + lane % 16, -1: none
-        const int64_t slot = p0 + (lane & 15) < jb.p1 ? slot_of(a, jb.b, p0 + (lane & 15)) : -1;
-        return slot >= 0 ? (slot * a.kv + jb.h) * hd : (int64_t)-1;
-    };
-    uint4 k[2][NU], v[4][NC];
-    auto load_k = [&](int64_t at) {
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-            const int64_t s = __shfl_sync(0xffffffffu, at, g + 8 * n);
-#pragma unroll
-            for (int u = 0; u < NU; u++)
-                k[n][u] = s >= 0 && t + 4 * u < nch ? load_stream((const CT *)a.kc + s + 8 * (t + 4 * u)) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    auto load_v = [&](int64_t at) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int64_t s = __shfl_sync(0xffffffffu, at, 2 * t + (i & 1) + 4 * (i & 2));
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-                v[i][c] = s >= 0 && g + 8 * c < nch ? load_stream((const CT *)a.vc + s + 8 * (g + 8 * c)) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    int64_t at = locate(jb.p0 + 16 * warp);
-    load_k(at);
-    load_v(at);
-    at = locate(jb.p0 + 16 * warp + 64);
     for (int p0 = jb.p0 + 16 * warp; p0 < jb.p1; p0 += 64) {
         float s[2][4] = {};
 #pragma unroll
@@ -247,7 +248,8 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
             a.ml[to] = make_float2(M, sum);
         }
     }
-    pdl_wait();  // launched beside the prefix's kernel, this one ends after it: the join waits for this one
+    // launched beside the prefix's kernel, this grid ends after it, which the join relies on: one block waits, the others make room
+    if (blockIdx.x == 0) pdl_wait();
 }
 
 template <typename T, typename CT, int HDP>
