@@ -8,6 +8,7 @@
 // maximum m, sum l and unnormalised o in the workspace, and a second launch joins the parts of every row:
 // o = sum_j e^(m_j - M) o_j / sum_j e^(m_j - M) l_j.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_prefix.cuh"
 
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < TW; j++) {
-            const int r = warp * TW + j;
+            const int r = 4 * j + warp;  // few rows spread over the warps
             if (r >= jb.nr) break;
             const float *q = Qs + r * hd4;
             float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
     const int64_t all = (int64_t)a.n_seq * a.heads;
 #pragma unroll
     for (int j = 0; j < TW; j++) {
-        const int r = warp * TW + j;
+        const int r = 4 * j + warp;  // few rows spread over the warps
         if (r >= jb.nr) break;
         const int64_t at = jb.part * all + out_row(a, jb.h, jb.r0 + r);
         if (lane == 0) a.ml[at] = make_float2(m[j], l[j]);
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int pa
         }
 }
 
+constexpr int kMostSplits = 64;
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // 16-bit rows of whole 16-byte chunks go to the matrix instructions
@@ -202,17 +204,29 @@ bool takes_mma(const qmc_paged_cache *c) {
     return c->dtype != QMC_F32 && c->head_dim % 8 == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0;
 }
 
-// position ranges for each of `units` row tiles over `tiles` position tiles, `slots` blocks running at once: the number with
-// the fewest rounds of tiles, a block costing kBlockTiles more for its start, its end and its parts' way through memory
-constexpr int kBlockTiles = 3, kMostSplits = 64;
-int split_for(int64_t units, int tiles, int slots) {
-    int best = 1;
-    int64_t least = INT64_MAX;
-    for (int n = 1; n <= std::min(kMostSplits, tiles); n++) {
-        const int64_t cost = (units * n + slots - 1) / slots * (ceil_div(tiles, n) + kBlockTiles);
-        if (cost < least) least = cost, best = n;
+// The time of a call whose prefix blocks and own jobs are split into n and m position ranges, in the microseconds that one block takes
+// while its SM runs as many as fit.  The prefix's blocks come first; own jobs take the places that these leave, and all places
+// once they are done.  Sequences are taken to be half as long as the table allows, the last job as long as the longest.
+struct Work {
+    double start, tile;  // of a block: its start, end and parts' way through memory, and each tile of positions
+    int64_t units;       // row tiles
+    int tiles, take;     // tiles of positions, places that a block takes
+};
+double time_of(const Work &pre, const Work &own, int n, int m, int64_t places) {
+    double done = 0.0, here = 0.0;  // when the prefix's last round ends, and its length
+    int64_t left = places;
+    if (n) {
+        const int64_t blocks = pre.units * n * pre.take, rounds = (blocks + places - 1) / places;
+        here = pre.start + pre.tile * ((pre.tiles + n - 1) / n);
+        done = rounds * here, left = rounds * places - blocks;
     }
-    return best;
+    if (!m) return done;
+    const int64_t jobs = own.units * m;
+    const double half = own.tile * 0.5 * ((own.tiles + m - 1) / m), job = own.start + half;
+    if (!n) return (jobs + places - 1) / places * job + half;
+    const int64_t beside = left * (int64_t)ceil(here / job);
+    if (jobs <= beside) return std::max(done, done - here + (jobs + left - 1) / left * job + half);
+    return done + (jobs - beside + places - 1) / places * job + half;
 }
 
 Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int prefix, int ld_table, int sms) {
@@ -227,29 +241,31 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
         p.pkind = dtype == c->dtype && c->page_size % 8 == 0 && (int64_t)c->n_pages * c->page_size <= INT32_MAX ? kTcKernel : kMmaKernel;
     struct Shape {
         int ptile, otile, quantum, blocks;  // rows of a prefix and of an own job, positions of a tile, blocks an SM runs at once
+        double start, tile;                 // see Work
     };
-    const Shape shape[4] = {{kQR, kQR, kPT, 4}, {kWarpRows, kWarpRows, 64, 2}, {attn_mma_tile(p.rows), 16, 64, 2},
-                            {attn_tc_tile(p.rows), 0, 128, 1}};
+    const Shape shape[4] = {{kQR, kQR, kPT, 4, 5.0, 4.0}, {kWarpRows, kWarpRows, 64, 2, 5.0, 2.2},
+                            {attn_mma_tile(p.rows), 16, 64, 2, 6.0, 2.2}, {attn_tc_tile(p.rows), 0, 128, 1, 6.0, 2.0}};
     const Shape &ps = shape[p.pkind], &os = shape[p.okind];
     p.ptiles = ceil_div(p.rows, ps.ptile);
     p.gtiles = ceil_div(group, os.otile);
-    if (own) p.osplit = split_for((int64_t)n_seq * kv * p.gtiles, ceil_div(own, os.quantum), os.blocks * sms);
-    const int64_t units = (int64_t)kv * p.ptiles;
-    if (prefix && p.pkind == kTcKernel && own) {
-        // The tensor-core blocks take whole SMs; the own jobs run on what they leave, and on all SMs afterwards.  Of the numbers
-        // of ranges the one that ends first, with a block's tile 2.0 us for two row tiles and 1.2 us for one, three more for
-        // its start and end, and an own job 4 us and 1 us for every 64 positions of half the longest, two at once on an SM.
-        const double tile = p.rows > 128 ? 2.0 : 1.2;
-        const double job = 4.0 + 0.5 * ceil_div(own, 64) / p.osplit, work = 0.5 * job * n_seq * kv * p.gtiles * p.osplit;
-        double least = 1e30;
-        for (int n = 1; n <= std::min(kMostSplits, ceil_div(prefix, 128)); n++) {
-            const int64_t blocks = units * n, left = sms - std::min<int64_t>(sms, blocks - (blocks - 1) / sms * sms);
-            const double tc = tile * ((blocks + sms - 1) / sms) * (ceil_div(ceil_div(prefix, 128), n) + kBlockTiles);
-            const double end = tc + std::max(0.0, work - left * tc) / sms;
-            if (end < least) least = end, p.psplit = n;
+    const Work pre{ps.start, ps.tile, (int64_t)kv * p.ptiles, ceil_div(prefix, ps.quantum), std::max(1, os.blocks / ps.blocks)};
+    const Work mine{os.start, os.tile, (int64_t)n_seq * kv * p.gtiles, ceil_div(own, os.quantum), 1};
+    // one at a time, from the own jobs by themselves: two rounds end within 15 % of the best pair for 99 of 100 shapes
+    auto best = [&](int tiles, auto time) {
+        int at = 0;
+        double least = 0.0;
+        for (int n = 1; n <= std::min(kMostSplits, tiles); n++) {
+            if (n > 1 && (tiles + n - 1) / n == (tiles + n - 2) / (n - 1)) continue;  // no range gets shorter
+            const double t = time(n);
+            if (!at || t < least) least = t, at = n;
         }
-    } else if (prefix) {
-        p.psplit = split_for(units, ceil_div(prefix, ps.quantum), ps.blocks * sms);
+        return at;
+    };
+    const int64_t places = (int64_t)os.blocks * sms;
+    if (own) p.osplit = best(mine.tiles, [&](int m) { return time_of(pre, mine, 0, m, places); });
+    for (int i = 0; prefix && i < 2; i++) {
+        p.psplit = best(pre.tiles, [&](int n) { return time_of(pre, mine, n, p.osplit, places); });
+        if (own) p.osplit = best(mine.tiles, [&](int m) { return time_of(pre, mine, p.psplit, m, places); });
     }
     p.pparts = p.psplit;
     const int64_t parts = p.pparts + p.osplit, all = (int64_t)n_seq * n_heads;
