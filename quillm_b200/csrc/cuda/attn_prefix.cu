@@ -325,8 +325,8 @@ int check_attn(const char *op, int dtype, const qmc_paged_cache *c, int n_seq, i
     if (n_seq < 0 || n_heads < 1 || n_heads % c->n_kv_heads || prefix < 0 || ld_table < 1)
         return set_error(QMC_EINVAL, "%s: %d sequences, %d heads over %d, prefix %d, table %d wide", op, n_seq, n_heads,
                          c->n_kv_heads, prefix, ld_table);
-    if ((int64_t)ld_table * c->page_size > INT32_MAX || (int64_t)n_seq * n_heads > INT32_MAX)
-        return set_error(QMC_EINVAL, "%s: more than 2^31 - 1 positions or rows", op);
+    if ((int64_t)ld_table * c->page_size > INT32_MAX - 1024 || (int64_t)n_seq * n_heads > INT32_MAX)  // a position past the last is counted too
+        return set_error(QMC_EINVAL, "%s: more than 2^31 - 1025 positions or 2^31 - 1 rows", op);
     if (prefix > (int64_t)ld_table * c->page_size)
         return set_error(QMC_EINVAL, "%s: prefix of %d past a table of %d pages of %d", op, prefix, ld_table, c->page_size);
     return QMC_OK;

@@ -25,8 +25,7 @@ struct Job {
 };
 
 __device__ __forceinline__ int own_len(const AttnArgs &a, int b) {
-    const int n = a.lens[b];
-    return min(max(n - a.prefix, 0), a.ld_table * a.page_size - a.prefix);
+    return min(max(a.lens[b], a.prefix), a.ld_table * a.page_size) - a.prefix;
 }
 
 // jobs: prefix [h][tile][split], then own [b][h][group tile][split]; ranges of positions are multiples of `quantum`

@@ -118,6 +118,12 @@ def test_attn_refusals(bad):
     refused(qb.cuda().qmc_attn_prefix_workspace(1, C.addressof(c), 3, 4, 9, 4, None))
 
 
+def test_attn_refuses_positions_near_the_end_of_int():
+    c, n = cache(page_size=1, n_pages=1 << 20), C.c_size_t(0)
+    refused(qb.cuda().qmc_attn_prefix_workspace(1, C.addressof(c), 1, 4, 0, (1 << 31) - 1, C.byref(n)), "positions")
+    assert n.value == 0
+
+
 def select(**k):
     d = dict(dtype=0, logits=A, ld=100, prompts=2, beams=3, vocab=100, scores=A, finished=A, eos=2, n_out=6, parents=A, tokens=A,
              out=A, ws=A, bytes=1 << 30)
