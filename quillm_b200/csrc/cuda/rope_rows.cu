@@ -37,7 +37,7 @@ int check_cache(const qmc_paged_cache *c, const char *op) {
     if ((uintptr_t)c->k % sz || (uintptr_t)c->v % sz) return set_error(QMC_EINVAL, "%s: misaligned cache", op);
     // slots of a layer are counted in 64 bits, elements of the pool must be too
     const __int128 n = (__int128)c->n_layers * c->n_pages * c->page_size * c->n_kv_heads * c->head_dim * sz;
-    if (n > ((__int128)1 << 62)) return set_error(QMC_EINVAL, "%s: cache too large", op);
+    if (n > ((__int128)1 << 62) || (int64_t)c->n_kv_heads * c->head_dim > 1 << 28) return set_error(QMC_EINVAL, "%s: cache too large", op);
     return QMC_OK;
 }
 
@@ -282,9 +282,12 @@ int launch_rows(RowsArgs &a, const qmc_rope_plan *p, int dtype, int cdt, int64_t
     return launch_ct<__nv_bfloat16>(a, f, cdt, rows, s);
 }
 
+constexpr int kMostHeads = 1 << 20;  // of a row, queries or keys: their elements are counted in 32 bits
+
 // rows of `n` heads `ld` elements apart
 int check_rows(const char *op, const char *name, const void *p, int64_t ld, int64_t n, int hd, int dtype) {
     if (!p) return set_error(QMC_EINVAL, "%s: null %s", op, name);
+    if (n > kMostHeads) return set_error(QMC_EINVAL, "%s: %lld heads are too many", op, (long long)n);
     if (ld < n * hd) return set_error(QMC_EINVAL, "%s: %s rows of %lld elements are %lld apart", op, name, (long long)(n * hd), (long long)ld);
     if (ld > (int64_t)1 << 40) return set_error(QMC_EINVAL, "%s: ld of %s too large", op, name);
     if ((uintptr_t)p % dtype_size(dtype)) return set_error(QMC_EINVAL, "%s: misaligned %s", op, name);

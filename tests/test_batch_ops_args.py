@@ -162,3 +162,13 @@ def test_beam_reorder_refusals(bad):
     assert reorder(cache(), prompts=0) == 0
     for c in BAD_CACHE:
         refused(reorder(cache(**c)), "beam_reorder")
+
+
+def test_sizes_counted_in_32_bits_are_bounded():
+    many = (1 << 20) + 1
+    c = cache(n_layers=1, n_pages=1, page_size=1, n_kv_heads=1 << 24, head_dim=32)
+    refused(reorder(c), "too large")
+    refused(attn(c), "too large")
+    p = qb.RopePlan(2)
+    refused(qb.cuda().qmc_qk_norm_rope(p.h, 0, A, 1 << 30, A, 1 << 30, many, None, 0, None, 0, 0, None, None, 0.0, A, 1, None), "too many")
+    refused(qb.cuda().qmc_qk_norm_rope(p.h, 0, None, 0, None, 0, 0, A, 1 << 30, A, 1 << 30, 2**31 - 1, None, None, 0.0, A, 1, None))

@@ -8,7 +8,8 @@ Tolerances, with u = 2^-24 and e the output type's half step (2^-24, 2^-11, 2^-8
     by the root, the root, the quotient and two products).  Together under 2^-19 m (|a| + |b|), plus e |out|.
   attention: a score is off by d_s <= (hd + 8) u scale sum_d |q k| (2^-21 more where a float query is split in
     two halves); a weight by 2 d_s + 2^-20 and, where weights are rounded to 16 bits for the product, e_P of that type;
-    the sum of weights likewise.  o is off by at most 2 (2 d_s + 2^-20 + e_P) sum_p w_p |v_p|, plus e |o|.
+    the sum of weights likewise (where a third of the exponentials come from a polynomial, 2^-13.7 for bf16 and 2^-18.5 for fp16
+    join them, far below e_P, which the sum does not have).  o is off by at most 2 (2 d_s + 2^-20 + e_P) sum_p w_p |v_p|, plus e |o|.
   beam scores: exp is off by 2 u (1 + |x - m|) <= 2^-19 for the terms that count, the chunk's float sum by 21 u: 2^-18 in
     the log-sum-exp, plus u |score|."""
 import math
@@ -723,3 +724,132 @@ def test_beam_search_over_pages(cuda_dev, dtype, cdt):
         close(f64(sc)[0], chosen, drift)
         hist = [hist[j] for j in pn]
         ref_scores, scores, tokens, table = chosen, sc[0].contiguous(), tok[0].long(), out
+
+
+# ------------------------------------------------------------------ captured, at once, at the ends of the ranges
+TC = [  # seqs, heads, kv, hd, prefix, own lengths, page: many rows, every padded head width, pages from one copy to many
+    (20, 2, 2, 8, 1000, [3] * 20, 8), (5, 16, 2, 24, 2049, [0, 1, 7, 8, 9], 24), (40, 8, 1, 40, 129, [i for i in range(40)], 40),
+    (9, 16, 1, 56, 128, [1] * 9, 128), (17, 8, 8, 72, 127, [2] * 17, 256), (130, 2, 1, 88, 777, [i % 3 for i in range(130)], 16),
+    (12, 16, 1, 104, 3001, [5] * 12, 512), (33, 8, 1, 120, 640, [1] * 33, 64), (257, 1, 1, 128, 500, [0] * 257, 32),
+    (18, 1, 1, 64, 5, [1] * 18, 8)]
+
+
+@pytest.mark.parametrize("dtype,cdt", [("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("case", range(len(TC)))
+def test_attn_many_rows(cuda_dev, case, dtype, cdt):
+    n_seq, heads, kv, hd, prefix, own, page = TC[case]
+    g = gen(500 + case)
+    kp, vp, c, pp, table, lens = attn_setup(g, n_seq, heads, kv, hd, prefix, own, page, dtype, cdt)
+    _, q = strided(g, n_seq, heads * hd, dtype, [0, 5][case % 2], [0, 3][case % 2])
+    out = torch.zeros(n_seq, heads * hd, dtype=DT[dtype], device="cuda")
+    scale = 1.0 / math.sqrt(hd)
+    do_attn(c, 0, dtype, q, out, heads, scale, pp, prefix, table, lens)
+    clean()
+    check_attn(out, q, kp, vp, lens, prefix, pp, table, page, kv, hd, scale, dtype, cdt)
+
+
+@pytest.mark.parametrize("dtype,cdt", TYPES)
+def test_attn_pages_listed_more_than_once(cuda_dev, dtype, cdt):
+    """two sequences with the same pages of their own, a prefix that repeats a page; on the library's own stream"""
+    n_seq, heads, kv, hd, prefix, page = 3, 24, 1, 64, 96, 16
+    g = gen(19)
+    kp, vp, c, pp, table, lens = attn_setup(g, n_seq, heads, kv, hd, prefix, [30, 30, 17], page, dtype, cdt, stale=0.0)
+    table[1] = table[0]
+    pp[3:] = pp[0]
+    q = rand(g, (n_seq, heads * hd), dtype)
+    q[1] = q[0]
+    out = torch.zeros_like(q)
+    ws = torch.empty(qb.attn_prefix_workspace(CODE[dtype], c, n_seq, heads, prefix, table.shape[1]), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    qb.check(lib().qmc_attn_prefix(c.ref, 0, CODE[dtype], q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads, n_seq, 0.125,
+                                   pp.data_ptr(), prefix, table.data_ptr(), table.shape[1], lens.data_ptr(), ws.data_ptr(), ws.numel(),
+                                   None))
+    qb.check(lib().qmc_sync())
+    assert torch.equal(out[0], out[1])
+    check_attn(out, q, kp, vp, lens, prefix, pp, table, page, kv, hd, 0.125, dtype, cdt)
+
+
+def test_decoding_step_captured(cuda_dev):
+    """append, attention, selection and reordering in one graph, replayed on another stream with other inputs, against the same
+    calls one by one: the same bits"""
+    prompts, beams, heads, kv, hd, page, width, prefix, vocab = 2, 3, 8, 2, 64, 8, 6, 13, 9001
+    rows, g = prompts * beams, gen(23)
+    n_pages = rows * width + 2
+    p = plan(hd, hd, 1, 0)
+    perm = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32)
+    pp, own = perm[:2].clone(), perm[2:2 + rows * (width - 1)].view(rows, width - 1)
+    state = []
+    for _ in range(2):  # [0] replayed, [1] one by one
+        kp, vp, c = pools(gen(24), 2, n_pages, page, kv, hd, "f16")
+        table = torch.cat([pp[:1].expand(rows, 1), own], 1).contiguous()
+        state.append(dict(kp=kp, vp=vp, c=c, table=table, out=torch.zeros_like(table), lens=torch.full((rows,), 30, dtype=torch.int32, device="cuda"),
+                          pos=torch.full((rows,), 29, dtype=torch.int32, device="cuda"), x=torch.zeros(rows, (heads + 2 * kv) * hd, device="cuda").half(),
+                          y=torch.zeros(rows, heads * hd, device="cuda").half(), logits=torch.zeros(rows, vocab, device="cuda"),
+                          scores=torch.zeros(rows, device="cuda"), par=torch.zeros(prompts, 5, dtype=torch.int32, device="cuda"),
+                          tok=torch.zeros(prompts, 5, dtype=torch.int32, device="cuda"), best=torch.zeros(prompts, 5, device="cuda"),
+                          w1=torch.full((qb.attn_prefix_workspace(qb.QMC_F16, c, rows, heads, prefix, width),), 255, dtype=torch.uint8, device="cuda"),
+                          w2=torch.full((qb.beam_workspace(prompts, beams, vocab, 5),), 255, dtype=torch.uint8, device="cuda")))
+
+    def step(s):
+        k, v = s["x"][:, heads * hd:(heads + kv) * hd], s["x"][:, (heads + kv) * hd:]
+        do_append(p, s["c"], 1, "f16", s["x"][:, :heads * hd], s["x"][:, :heads * hd], heads, k, v, None, None, None, s["pos"], s["table"], rows)
+        do_attn(s["c"], 1, "f16", s["x"][:, :heads * hd], s["y"], heads, 0.125, pp, prefix, s["table"], s["lens"], s["w1"])
+        qb.check(lib().qmc_beam_select(qb.QMC_F32, s["logits"].data_ptr(), vocab, prompts, beams, vocab, s["scores"].data_ptr(), None, 0, 5,
+                                       s["par"].data_ptr(), s["tok"].data_ptr(), s["best"].data_ptr(), s["w2"].data_ptr(), s["w2"].numel(),
+                                       qb.torch_stream()))
+        qb.check(lib().qmc_beam_reorder(s["c"].ref, prompts, beams, s["par"].data_ptr(), 5, s["lens"].data_ptr(), s["table"].data_ptr(),
+                                        s["out"].data_ptr(), width, qb.torch_stream()))
+
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step(state[0])
+    for n in (30, 33, 40):
+        x, z = rand(g, (rows, (heads + 2 * kv) * hd), "f16"), rand(g, (rows, vocab), "f32", 3.0)
+        for s in state:
+            s["x"].copy_(x), s["logits"].copy_(z), s["lens"].fill_(n), s["pos"].fill_(n - 1)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        step(state[1])
+        clean()
+        for name in ("kp", "vp", "x", "y", "par", "tok", "best", "out"):
+            a, b = (s[name].view(torch.int16) if s[name].dtype == torch.float16 else s[name] for s in state)
+            assert torch.equal(a, b), name
+        for s in state:
+            s["table"].copy_(s["out"])
+            s["scores"].copy_(s["best"][:, :beams].reshape(-1))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_beam_select_at_once(cuda_dev, dtype):
+    """two selections at once, on streams and workspaces of their own"""
+    g = gen(31)
+    jobs = []
+    for prompts, beams, vocab, n_out in ((3, 8, 40000, 16), (2, 5, 70001, 10)):
+        x = rand(g, (prompts * beams, vocab), dtype, 3.0)
+        jobs.append((x, vocab, prompts, beams, -torch.rand(prompts * beams, generator=g, device="cuda"), None, 0, n_out))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in jobs], [[] for _ in jobs]
+    for _ in range(5):
+        for i, (s, j) in enumerate(zip(streams, jobs)):
+            with torch.cuda.stream(s):
+                got[i].append(do_select(dtype, *j))
+    clean()
+    for all_of, (x, vocab, prompts, beams, scores, _, eos, n_out) in zip(got, jobs):
+        want = ref_select(f64(x), f64(scores), None, eos, n_out, prompts, beams)
+        for one in all_of:
+            check_select(one, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_beam_select_largest(cuda_dev, dtype):
+    """as many beams and logits as a call takes: 64 rows of 2^19, and all of one chunk's logits equal"""
+    g = gen(37)
+    x = rand(g, (64, 1 << 19), dtype, 2.0)
+    x[5, :20000] = 9.0
+    scores = -torch.rand(64, generator=g, device="cuda")
+    scores[5] += 3.0
+    got = do_select(dtype, x, 1 << 19, 1, 64, scores, None, 0, 64)
+    clean()
+    check_select(got, ref_select(f64(x), f64(scores), None, 0, 64, 1, 64))
