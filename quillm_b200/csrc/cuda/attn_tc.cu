@@ -230,6 +230,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int hd = a.hd, nch = hd / 8;
     const Job jb = job_of(a, blockIdx.x, PAIR ? 2 * kM : kM, 0, kN);
     const int ntile = (jb.p1 - jb.p0 + kN - 1) / kN;
+    // the copy warp's lane i finds the pages of box i of a tile; the first tile's are on their way before anything else
+    const int groups = kN / box;
+    auto page_at = [&](int p) { return p < jb.p1 ? a.prefix_pages[p / a.page_size] : -1; };
+    const int first = warp == kCopyWarp ? page_at(jb.p0 + lane % groups * box) : -1;
     // chunk c of row r of a tile, 128-byte swizzle
     auto place = [](int r, int c) { return (c >> 3) * PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
 
@@ -257,19 +261,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // all 512 columns are this block's, so they start at 0: S (and P) of stream w at 128 w, O at 256 + HDP w
 
     if (warp == kCopyWarp) {  // ---------------------------------------------------------------- TMA
-        // lane i: box i % groups of the tile's rows, panel i / groups of 64 dimensions
-        const int groups = kN / box, g = lane % groups, panel = lane / groups;
-        const bool mine = panel < HDP / 64;
-        int issued = 0;
+        // one lane issues the copies: lanes that each issue their own take 90 cycles apiece
+        const int g = lane % groups;
+        const bool lead = elect_one();
+        int issued = 0, page = first;
         auto issue = [&](int row, int left, int u, const CUtensorMap *map) {  // tile u of the sequence K0 V0 K1 V1 ...
             const int at = u % NS, here = min(groups, (left + box - 1) / box);
             if (u >= NS && __any_sync(0xffffffffu, !mbar_wait(&sh.empty[at], (u / NS - 1) & 1))) {
                 if (lane == 0) raise_error(a.err, kErrMbarTimeout);
                 return false;
             }
-            if (lane == 0) mbar_arrive_tx(&sh.full[at], here * (HDP / 64) * box * 128);
-            __syncwarp();
-            if (mine && g < here) tma_2d(smk + at * TB + panel * PANEL + g * box * 128, map, jb.h * hd + 64 * panel, row, &sh.full[at]);
+            if (lead) mbar_arrive_tx(&sh.full[at], here * (HDP / 64) * box * 128);
+#pragma unroll 4
+            for (int i = 0; i < here; i++) {
+                const int y = __shfl_sync(0xffffffffu, row, i);
+                if (lead)
+#pragma unroll
+                    for (int k = 0; k < HDP / 64; k++)
+                        tma_2d(smk + at * TB + k * PANEL + i * box * 128, map, jb.h * hd + 64 * k, y, &sh.full[at]);
+            }
             issued = u + 1;
             return true;
         };
@@ -277,9 +287,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const int p = jb.p0 + j * kN + g * box, left = jb.p1 - jb.p0 - j * kN;
             int row = -kN;  // a page outside the pool: rows that do not exist read as zeros
             if (p < jb.p1) {
-                const int64_t slot = slot_of(a, -1, p);
-                if (slot >= 0) row = (int)slot;
+                if (page >= 0 && page < a.n_pages) row = page * a.page_size + p % a.page_size;
+                else raise_error(a.err, kErrBadIndex);
             }
+            page = page_at(p + kN);
             if (!issue(row, left, 2 * j, &kmap) || !issue(row, left, 2 * j + 1, &vmap)) break;
             if (left < kN) {  // the last V tile: zeros behind the range, once its copies have landed
                 const int u = 2 * j + 1, at = u % NS;
@@ -304,57 +315,73 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         __syncwarp();
     } else if (warp == kMmaWarp) {  // ---------------------------------------------------------------- MMA issuer
         // the whole warp runs this, one lane issues: addresses and descriptors stay uniform, where a lone lane would move each
-        // of them to the uniform registers that the instruction takes
+        // of them to the uniform registers that the instruction takes.  It shares its issue slots with four busy warps: a wait that
+        // is over costs a few instructions, and the ring's places are counted along, not divided for.
         const bool lead = elect_one();
         auto wait = [&](uint64_t *bar, uint32_t parity) {
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
             const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
             if (!ok && lane == 0) raise_error(a.err, kErrMbarTimeout);
             return ok;
         };
-        auto tile = [&](int u) {  // has landed
-            if ((u & 1) && jb.p1 - jb.p0 < (u / 2 + 1) * kN && !wait(&sh.vlast, 0)) return false;
-            return wait(&sh.full[u % NS], (u / NS) & 1);
+        struct Place {  // of the next K or V tile in the ring
+            uint32_t at, parity;
+        } k{0, 0}, v{1, 0};
+        auto advance = [&](Place &p) {
+            p.at += 2;
+            if (p.at >= NS) p.at -= NS, p.parity ^= 1;
         };
-        auto scores = [&](int w, int j) {  // S_w = Q_w K_j^T
-            const uint32_t q = (smq + (PAIR ? w : 0) * TB) / 16 | kLowK, k = (smk + (2 * j) % NS * TB) / 16 | kLowK;
+        const bool cut = (jb.p1 - jb.p0) % kN != 0;  // the last V tile waits for its zeros too
+        auto v_landed = [&](int j) { return wait(&sh.full[v.at], v.parity) && (!cut || j < ntile - 1 || wait(&sh.vlast, 0)); };
+        auto scores = [&](int w) {  // S_w = Q_w K^T
+            const uint32_t qd = (smq + (PAIR ? w : 0) * TB) / 16 | kLowK, kd = (smk + k.at * TB) / 16 | kLowK;
             if (lead) {
 #pragma unroll
                 for (int i = 0; i < HDP / 16; i++) {
                     const uint32_t off = ((i >> 2) * PANEL + (i & 3) * 32) / 16;
-                    mma_ss(128 * w, desc(q + off), desc(k + off), idesc(kN, false, BF), i > 0);
+                    mma_ss(128 * w, desc(qd + off), desc(kd + off), idesc(kN, false, BF), i > 0);
                 }
                 mma_commit(&sh.sfull[w]);
-                if (!PAIR || w == 1) mma_commit(&sh.empty[(2 * j) % NS]);
+                if (!PAIR || w == 1) mma_commit(&sh.empty[k.at]);
             }
+            if (!PAIR || w == 1) advance(k);
         };
-        auto weigh = [&](int w, int j, bool first) {  // O_w += P_w V_j
-            const uint32_t v = (smk + (2 * j + 1) % NS * TB) / 16 | kLowMN;
+        auto weigh = [&](int w, bool first) {  // O_w += P_w V
+            const uint32_t vd = (smk + v.at * TB) / 16 | kLowMN;
             if (lead) {
 #pragma unroll
-                for (int k = 0; k < kN / 16; k++)
-                    mma_ts(256 + HDP * w, 128 * w + 8 * k, desc(v + k * (16 * 128 / 16)), idesc(HDP, true, BF), !first || k > 0);
-                if (!PAIR || w == 1) mma_commit(&sh.empty[(2 * j + 1) % NS]);
+                for (int i = 0; i < kN / 16; i++)
+                    mma_ts(256 + HDP * w, 128 * w + 8 * i, desc(vd + i * (16 * 128 / 16)), idesc(HDP, true, BF), !first || i > 0);
+                if (!PAIR || w == 1) mma_commit(&sh.empty[v.at]);
             }
+            if (!PAIR || w == 1) advance(v);
         };
         constexpr int step = PAIR ? 1 : 2;  // tiles from one of a stream's to its next
         bool ok = wait(&sh.qready, 0);
         for (int w = 0; w < 2 && ok; w++) {
-            const int j = PAIR ? 0 : w;
-            if (j < ntile && (ok = tile(2 * j))) scores(w, j);
+            if ((PAIR ? 0 : w) >= ntile) continue;
+            ok = wait(&sh.full[k.at], k.parity);
+            if (ok) scores(w);
         }
+        ok = ok && (ntile == 0 || v_landed(0));
         for (int i = 0; i * step < ntile && ok; i++)
-            for (int w = 0; w < 2 && ok; w++) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
                 const int j = PAIR ? i : 2 * i + w;
-                if (j >= ntile) continue;
-                // the tiles of both products first (PAIR: of both streams), while the tensor cores work on the other stream, so that
-                // nothing but the issue follows the weights
-                if (!PAIR || w == 0) ok = tile(2 * j + 1) && (j + step >= ntile || tile(2 * (j + step)));
-                ok = ok && wait(&sh.pfull[w], i & 1u);
+                if (!ok || j >= ntile) break;
+                ok = wait(&sh.pfull[w], i & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                weigh(w, j, i == 0);
-                if (j + step < ntile) scores(w, j + step);
-                else if (lead) mma_commit(&sh.ofin[w]);
+                weigh(w, i == 0);
+                // the tiles of what follows, waited for while the tensor cores have these products to do: the V tile of the next
+                // step (PAIR: with the second stream), then the K tile of the scores
+                if ((!PAIR || w == 1) && j + 1 < ntile && !(ok = v_landed(j + 1))) break;
+                if (j + step < ntile) {
+                    if ((!PAIR || w == 0) && !(ok = wait(&sh.full[k.at], k.parity))) break;
+                    scores(w);
+                } else if (lead) {
+                    mma_commit(&sh.ofin[w]);
+                }
             }
         // nothing may be in flight when the TMEM is freed
         if (lead) mma_commit(&sh.drain);
@@ -363,17 +390,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     } else {  // ---------------------------------------------------------------- weights
         // the query tiles first; rows past the last and chunks past the head are zeros
         const bool vec = a.ldq % 8 == 0 && (uintptr_t)a.q % 16 == 0;
-        for (int i = tid; i < (PAIR ? 2 : 1) * kM * CH; i += 32 * kCopyWarp) {
-            const int r = i / CH, c = i % CH, rr = jb.r0 + r;
-            alignas(16) CT e[8];
-            *(uint4 *)e = make_uint4(0, 0, 0, 0);
-            if (r < jb.nr && c < nch) {
-                const CT *src = (const CT *)a.q + (rr / a.group) * a.ldq + (int64_t)(jb.h * a.group + rr % a.group) * hd + 8 * c;
-                if (vec) *(uint4 *)e = *(const uint4 *)src;
-                else
-                    for (int k = 0; k < 8; k++) e[k] = src[k];
+        constexpr int NQ = (PAIR ? 2 : 1) * kM * CH / (32 * kCopyWarp);  // chunks of a thread, all on their way at once
+        uint4 x[NQ];
+        const CT *const q0 = (const CT *)a.q + (int64_t)jb.h * a.group * hd + 8 * (tid % CH);
+#pragma unroll
+        for (int u = 0; u < NQ; u++) {
+            const int r = tid / CH + u * (32 * kCopyWarp / CH), b = (jb.r0 + r) / a.group, g = (jb.r0 + r) - b * a.group;
+            const CT *src = q0 + b * a.ldq + (int64_t)g * hd;
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (r < jb.nr && tid % CH < nch) {
+                if (vec) {
+                    x[u] = *(const uint4 *)src;
+                } else {
+                    const uint16_t *e = (const uint16_t *)src;
+                    x[u] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                }
             }
-            *(uint4 *)(base + (r / kM) * TB + place(r % kM, c)) = *(const uint4 *)e;
+        }
+#pragma unroll
+        for (int u = 0; u < NQ; u++) {
+            const int r = tid / CH + u * (32 * kCopyWarp / CH);
+            *(uint4 *)(base + (r / kM) * TB + place(r % kM, tid % CH)) = x[u];
         }
         fence_proxy_async();
         mbar_arrive(&sh.qready);
@@ -482,29 +519,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
         }
         asm volatile("bar.sync 9, 512;" ::: "memory");
-        const int64_t all = (int64_t)a.n_seq * a.heads;
+        // lane i: the place and the factors of the warp's row i
         constexpr int RW = (PAIR ? 2 : 1) * kM / 16;  // rows a warp stores
-        for (int k = 0; k < RW; k++) {
-            const int r = RW * warp + k, rr = r % kM, s = PAIR ? r / kM : 0;
-            if (r >= jb.nr) break;
-            const int64_t at = jb.part * all + out_row(a, jb.h, jb.r0 + r);
-            const float *h = ml + 3 * s * kM + rr;
-            float M = h[0], L = h[kM] + h[2 * kM], c0 = 1.0f, c1 = 0.0f;
+        const int64_t all = (int64_t)a.n_seq * a.heads;
+        const int r0 = RW * warp, here = min(RW, jb.nr - r0), s = PAIR ? r0 / kM : 0;
+        int64_t at = 0;
+        float c0 = 1.0f, c1 = 0.0f;
+        if (lane < here) {
+            at = jb.part * all + out_row(a, jb.h, jb.r0 + r0 + lane);
+            const float *h = ml + 3 * s * kM + (r0 + lane) % kM;
+            float M = h[0], L = h[kM] + h[2 * kM];
             if (!PAIR) {  // the two streams' parts of the row as one
                 const float m0 = M, m1 = h[3 * kM];
                 M = fmaxf(m0, m1);
                 if (M > -INFINITY) c0 = ex2(m0 - M), c1 = ex2(m1 - M);
                 L = L * c0 + (h[4 * kM] + h[5 * kM]) * c1;
             }
-            if (lane == 0) a.ml[at] = make_float2(M, L);
-            if (4 * lane < hd) {
-                const int o = rr * (HDP * 4) + ((lane ^ (rr & 7)) << 4);
+            a.ml[at] = make_float2(M, L);
+        }
+#pragma unroll 4
+        for (int k = 0; k < RW; k++) {
+            const int64_t to = __shfl_sync(0xffffffffu, at, k);
+            const float f0 = __shfl_sync(0xffffffffu, c0, k), f1 = __shfl_sync(0xffffffffu, c1, k);
+            if (k < here && 4 * lane < hd) {
+                const int rr = (r0 + k) % kM, o = rr * (HDP * 4) + ((lane ^ (rr & 7)) << 4);
                 float4 v = *(const float4 *)(rows + s * (kM * HDP * 4) + o);
                 if (!PAIR) {
                     const float4 u = *(const float4 *)(rows + kM * HDP * 4 + o);
-                    v = make_float4(v.x * c0 + u.x * c1, v.y * c0 + u.y * c1, v.z * c0 + u.z * c1, v.w * c0 + u.w * c1);
+                    v = make_float4(v.x * f0 + u.x * f1, v.y * f0 + u.y * f1, v.z * f0 + u.z * f1, v.w * f0 + u.w * f1);
                 }
-                *(float4 *)(a.po + at * hd + 4 * lane) = v;
+                *(float4 *)(a.po + to * hd + 4 * lane) = v;
             }
         }
         tc_fence_before();
