@@ -89,10 +89,19 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
                 v[i][c] = s >= 0 && g + 8 * c < nch ? load_stream((const CT *)a.vc + s + 8 * (g + 8 * c)) : make_uint4(0, 0, 0, 0);
         }
     };
-    int64_t at = locate(jb.p0 + 16 * warp);
+    // the group after that is on its way to the second-level cache: lanes 0-15 ask for the keys, the others for the values
+    const uint8_t *const half = (const uint8_t *)(lane < 16 ? a.kc : a.vc);
+    auto fetch = [&](int64_t at) {
+        if (at < 0) return;
+#pragma unroll
+        for (int i = 0; i < HDP / 64; i++)
+            if (64 * i < hd) asm volatile("prefetch.global.L2 [%0];" ::"l"(half + 2 * (at + 64 * i)));
+    };
+    int64_t at = locate(jb.p0 + 16 * warp), next = locate(jb.p0 + 16 * warp + 64);
     load_k(at);
     load_v(at);
-    at = locate(jb.p0 + 16 * warp + 64);
+    fetch(next);
+    at = next, next = locate(jb.p0 + 16 * warp + 128);
 
     uint32_t q[H][2 * NU][4];
     float scale[2];  // of rows g and g + 8
@@ -139,6 +148,7 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; i++) o[c][j][i] = 0.0f;
     for (int p0 = jb.p0 + 16 * warp; p0 < jb.p1; p0 += 64) {
+        fetch(next);
         float s[2][4] = {};
 #pragma unroll
         for (int u = 0; u < NU; u++)
@@ -197,7 +207,7 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
             }
         }
         load_v(at);
-        at = locate(p0 + 128);
+        at = next, next = locate(p0 + 192);
     }
 
     // join the four warps: maxima and sums first, then the rescaled accumulators; the columns of row r are rotated by 8 r
