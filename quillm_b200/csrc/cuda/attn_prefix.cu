@@ -15,7 +15,7 @@
 namespace qmc {
 namespace {
 
-enum { kRowsKernel, kWarpKernel, kMmaKernel, kTcKernel };
+enum { kRowsKernel, kWarpKernel, kMmaKernel, kTcKernel, kVecKernel };
 
 struct Plan {
     int rows;                 // query rows of a KV head over the whole batch: n_seq * group
@@ -23,6 +23,7 @@ struct Plan {
     int gtiles, osplit;       // own positions: row tiles of a group and position ranges
     int pkind, okind;         // the kernels of the prefix and of own positions
     int pparts;
+    int vtile;                // rows of a job of kVecKernel
     int64_t ml_bytes, bytes;  // workspace: [parts][n_seq * n_heads] float2 (m, l), then [parts][...][hd] floats
 };
 
@@ -235,7 +236,8 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
     const int64_t own = std::max<int64_t>(0, (int64_t)ld_table * c->page_size - prefix);
     p.rows = n_seq * group;
     const bool mma = takes_mma(c), narrow = mma && c->head_dim <= 128;
-    p.okind = narrow ? kWarpKernel : mma ? kMmaKernel : kRowsKernel;
+    const bool vec = c->dtype == QMC_F32 && c->head_dim % 4 == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0;
+    p.okind = narrow ? kWarpKernel : mma ? kMmaKernel : vec ? kVecKernel : kRowsKernel;
     p.pkind = p.okind;
     if (narrow && p.rows > kWarpRows)
         p.pkind = dtype == c->dtype && c->page_size % 8 == 0 && (int64_t)c->n_pages * c->page_size <= INT32_MAX ? kTcKernel : kMmaKernel;
@@ -243,8 +245,10 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
         int ptile, otile, quantum, blocks;  // rows of a prefix and of an own job, positions of a tile, blocks an SM runs at once
         double start, tile;                 // see Work
     };
-    const Shape shape[4] = {{kQR, kQR, kPT, 4, 5.0, 4.0}, {kWarpRows, kWarpRows, 64, 2, 5.0, 2.2},
-                            {attn_mma_tile(p.rows), 16, 64, 2, 6.0, 2.2}, {attn_tc_tile(p.rows), 0, 128, 1, 6.0, 2.0}};
+    const int vtile = attn_vec_tile(prefix ? std::max(p.rows, group) : group);
+    const Shape shape[5] = {{kQR, kQR, kPT, 4, 5.0, 4.0}, {kWarpRows, kWarpRows, 64, 2, 5.0, 2.2},
+                            {attn_mma_tile(p.rows), 16, 64, 2, 6.0, 2.2}, {attn_tc_tile(p.rows), 0, 128, 1, 6.0, 2.0},
+                            {vtile, vtile, 32, vtile == 1 ? 3 : 2, 5.0, 1.8}};
     const Shape &ps = shape[p.pkind], &os = shape[p.okind];
     p.ptiles = ceil_div(p.rows, ps.ptile);
     p.gtiles = ceil_div(group, os.otile);
@@ -267,6 +271,7 @@ Plan plan_for(const qmc_paged_cache *c, int dtype, int n_seq, int n_heads, int p
         p.psplit = best(pre.tiles, [&](int n) { return time_of(pre, mine, n, p.osplit, places); });
         if (own) p.osplit = best(mine.tiles, [&](int m) { return time_of(pre, mine, p.psplit, m, places); });
     }
+    p.vtile = vtile;
     p.pparts = p.psplit;
     const int64_t parts = p.pparts + p.osplit, all = (int64_t)n_seq * n_heads;
     p.ml_bytes = (parts * all * 8 + 255) / 256 * 256;
@@ -294,6 +299,7 @@ int launch_attn(const AttnArgs &a, const Plan &p, int dtype, int cdt, cudaStream
         if (kind == kTcKernel) return launch_attn_tc(x, cdt, s);
         if (kind == kMmaKernel) return launch_attn_mma(x, dtype, cdt, after, s);
         if (kind == kWarpKernel) return launch_attn_warp(x, dtype, cdt, after, s);
+        if (kind == kVecKernel) return launch_attn_vec(x, p.vtile, s);
         const int64_t n = (int64_t)x.kv * x.ptiles * x.psplit + (int64_t)x.n_seq * x.kv * x.gtiles * x.osplit;
         const size_t al = 4 * sizeof(CT);
         const bool vec = x.hd % 4 == 0 && (uintptr_t)x.kc % al == 0 && (uintptr_t)x.vc % al == 0;

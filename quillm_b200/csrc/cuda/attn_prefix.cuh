@@ -102,6 +102,10 @@ int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, bool after, cudaStrea
 constexpr int kWarpRows = 16;
 int launch_attn_warp(const AttnArgs &a, int dtype, int cdt, bool after, cudaStream_t s);
 
+// caches of floats, heads of whole 16-byte chunks (attn_vec.cu): tiles of 1, 4 or 8 rows
+int attn_vec_tile(int rows);
+int launch_attn_vec(const AttnArgs &a, int tile, cudaStream_t s);
+
 // the tensor-core kernel (attn_tc.cu): the prefix jobs of such a cache with rows of its own type, head_dim <= 128, pages of a
 // multiple of 8 positions and under 2^31 slots, for many rows
 int attn_tc_box(int page_size);  // positions of one copy
