@@ -140,64 +140,87 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
     }
 }
 
-// joins the parts of a row, one warp each: lane j takes part j's factor 2^(m_j - M), then every lane V of the row's dimensions (twice
-// above 128, as many times as needed one by one) over the parts, whose loads do not wait for one another
-template <typename T, int V>
+constexpr int kMostSplits = 64;
+
+// Joins the parts of a row, W warps each: a warp takes the factors 2^(m_j - M) of all parts, a lane each, and sums every W-th
+// part over the row's dimensions, V (once, twice above 128, as often as needed one by one) a lane, with loads that do not
+// wait for one another.  Bound by latency: the lengths, the statistics, the parts and the warps' sums follow on one another.
+template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int parts) {
-    const int lane = threadIdx.x & 31;
-    const int64_t all = (int64_t)a.n_seq * a.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    constexpr int NV = 256 / 32 / V, NB = 2 * kMostSplits / 32;
+    __shared__ float sum_s[W][256];
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
+    const int64_t all = (int64_t)a.n_seq * a.heads, row = (int64_t)blockIdx.x * (4 / W) + (threadIdx.x >> 5) / W;
+    const int b = (int)(row / a.heads), h = (int)(row % a.heads);
     pdl_wait();
-    if (row >= all) return;
-    const int b = (int)(row / a.heads), h = (int)(row % a.heads), n = a.lens[b];
+    if (row >= all) return;  // W == 1
+    const int n = a.lens[b];
     if (lane == 0 && ((n != 0 && n < a.prefix) || n > (int64_t)a.ld_table * a.page_size)) raise_error(a.err, kErrBadIndex);
-    constexpr int NV = 256 / 32 / V;
-    float o[NV][V], l = 0.0f, M = -INFINITY;
+    float2 st[NB];
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        st[i] = n > 0 && lane + 32 * i < parts ? a.ml[(lane + 32 * i) * all + row] : make_float2(-INFINITY, 0.0f);
+        M = fmaxf(M, st[i].x);
+    }
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float w[NB], l = 0.0f, o[NV][V];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {  // a part without weights is not read
+        w[i] = st[i].y != 0.0f ? exp2f(st[i].x - ref) : 0.0f;
+        l = st[i].y != 0.0f ? fmaf(w[i], st[i].y, l) : l;
+    }
+    l = warp_sum(l);
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) o[i][k] = 0.0f;
-    if (n > 0) {
-        for (int j = lane; j < parts; j += 32) M = fmaxf(M, a.ml[j * all + row].x);
-        M = warp_max(M);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        for (int j0 = 0; j0 < parts; j0 += 32) {
-            float w = 0.0f;  // of part j0 + lane; one without weights is not read
-            if (j0 + lane < parts) {
-                const float2 ml = a.ml[(j0 + lane) * all + row];
-                if (ml.y != 0.0f) w = exp2f(ml.x - ref), l = fmaf(w, ml.y, l);
-            }
-            const int here = min(32, parts - j0);
-#pragma unroll 8
-            for (int j = 0; j < here; j++) {
-                const float wj = __shfl_sync(0xffffffffu, w, j);
-                const bool live = wj != 0.0f;  // NaN included
-                const float *src = a.po + ((j0 + j) * all + row) * a.hd;
 #pragma unroll
-                for (int i = 0; i < NV; i++) {
-                    const int d = V * (lane + 32 * i);
-                    float v[V];
+    for (int i = 0; i < NB; i++) {
+        const int here = min(32, parts - 32 * i);
+#pragma unroll 4
+        for (int j = warp; j < here; j += W) {
+            const float wj = __shfl_sync(0xffffffffu, w[i], j);
+            const bool live = wj != 0.0f;  // NaN included
+            const float *src = a.po + ((32 * i + j) * all + row) * a.hd;
 #pragma unroll
-                    for (int k = 0; k < V; k++) v[k] = 0.0f;
-                    if (live && d < a.hd) load_chunk<float, V>(src + d, v);
+            for (int e = 0; e < NV; e++) {
+                const int d = V * (lane + 32 * e);
+                float v[V];
 #pragma unroll
-                    for (int k = 0; k < V; k++) o[i][k] = fmaf(wj, v[k], o[i][k]);
-                }
+                for (int k = 0; k < V; k++) v[k] = 0.0f;
+                if (live && d < a.hd) load_chunk<float, V>(src + d, v);
+#pragma unroll
+                for (int k = 0; k < V; k++) o[e][k] = fmaf(wj, v[k], o[e][k]);
             }
         }
-        l = warp_sum(l);
     }
     const float rl = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);  // an empty row gives zeros
     T *out = (T *)a.out + b * a.ldo + (int64_t)h * a.hd;
+    if constexpr (W == 1) {
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+        for (int i = 0; i < NV; i++)
 #pragma unroll
-        for (int k = 0; k < V; k++) {
-            const int d = V * (lane + 32 * i) + k;
-            if (d < a.hd) from_f32(o[i][k] * rl, &out[d]);
+            for (int k = 0; k < V; k++) {
+                const int d = V * (lane + 32 * i) + k;
+                if (d < a.hd) from_f32(o[i][k] * rl, &out[d]);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int k = 0; k < V; k++) sum_s[warp][V * (lane + 32 * i) + k] = o[i][k];
+        __syncthreads();
+        for (int d = threadIdx.x; d < a.hd; d += 128) {
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; i++) x += sum_s[i][d];
+            from_f32(x * rl, &out[d]);
         }
+    }
 }
 
-constexpr int kMostSplits = 64;
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // 16-bit rows of whole 16-byte chunks go to the matrix instructions
@@ -292,7 +315,7 @@ int launch_rows(const AttnArgs &a, int64_t jobs, bool vec, cudaStream_t s) {
 }
 
 template <typename T, typename CT>
-int launch_attn(const AttnArgs &a, const Plan &p, int dtype, int cdt, cudaStream_t s) {
+int launch_attn(const AttnArgs &a, const Plan &p, int dtype, int cdt, int sms, cudaStream_t s) {
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
     auto launch = [&](int kind, const AttnArgs &x, bool after) {
@@ -317,9 +340,12 @@ int launch_attn(const AttnArgs &a, const Plan &p, int dtype, int cdt, cudaStream
     if (rc) return rc;
     // the join may start while the last parts are written; it waits for them before it reads
     const int64_t all = (int64_t)a.n_seq * a.heads;
-    const dim3 grid((unsigned)((all + 3) / 4));
-    if (a.hd % 4 == 0) return launch_after(attn_join_kernel<T, 4>, grid, 128, 0, s, jobs > 0, a, a.pparts + a.osplit);
-    return launch_after(attn_join_kernel<T, 1>, grid, 128, 0, s, jobs > 0, a, a.pparts + a.osplit);
+    auto join = [&](auto fn, int rows) { return launch_after(fn, dim3((unsigned)((all + rows - 1) / rows)), 128, 0, s, jobs > 0, a, a.pparts + a.osplit); };
+    // four warps a row while the SMs hold all rows' blocks at once (1024 rows: 3.6 us less than with one warp each; 1536: 2 us more,
+    // 4096: 3 us more)
+    const bool wide = all <= 8 * (int64_t)sms;
+    if (a.hd % 4 == 0) return wide ? join(attn_join_kernel<T, 4, 4>, 1) : join(attn_join_kernel<T, 4, 1>, 4);
+    return wide ? join(attn_join_kernel<T, 1, 4>, 1) : join(attn_join_kernel<T, 1, 1>, 4);
 }
 
 int check_attn(const char *op, int dtype, const qmc_paged_cache *c, int n_seq, int n_heads, int prefix, int ld_table) {
@@ -390,10 +416,10 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
     a.scale = scale * 1.4426950408889634f;
     cudaStream_t s = pick_stream(stream);
     const int cdt = cache->dtype;
-    if (dtype == QMC_F32 && cdt == QMC_F32) return launch_attn<float, float>(a, p, dtype, cdt, s);
-    if (dtype == QMC_F32) return launch_attn<float, __half>(a, p, dtype, cdt, s);
-    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, p, dtype, cdt, s);
-    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, p, dtype, cdt, s);
+    if (dtype == QMC_F32 && cdt == QMC_F32) return launch_attn<float, float>(a, p, dtype, cdt, c->num_sms, s);
+    if (dtype == QMC_F32) return launch_attn<float, __half>(a, p, dtype, cdt, c->num_sms, s);
+    if (dtype == QMC_F16) return launch_attn<__half, __half>(a, p, dtype, cdt, c->num_sms, s);
+    return launch_attn<__nv_bfloat16, __nv_bfloat16>(a, p, dtype, cdt, c->num_sms, s);
 }
 
 }  // extern "C"
