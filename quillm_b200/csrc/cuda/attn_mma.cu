@@ -7,6 +7,10 @@
 // and accumulators are joined through shared memory at the end.  Rows of K, V and Q lie in shared memory with 16-byte
 // chunk c of row r at c ^ (r & 7): the eight rows of one matrix load hit distinct banks.
 //
+// Bound by the matrix instructions' issue and the loads from shared memory between them (512 rows over 32768 positions: 334 us, 206
+// TFLOP/s; float rows, of twice the products each way, 447 us), with few rows by the copies (32 rows 46 us, 2.9 TB/s).  Its cases are
+// those that the faster two cannot take: pages that are no multiple of 8, float rows in number, heads above 128.
+//
 // Weights are rounded to the cache's type for the second product (at most half a step each, as the outputs are).  Float
 // queries over an fp16 cache keep float accuracy: a row is scaled by a power of two and split in two halves q = qh + ql,
 // the weights likewise, and each product is taken twice.

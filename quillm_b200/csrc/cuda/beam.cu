@@ -12,6 +12,9 @@
 // collected in shared memory and ranked by counting, with the index, so that ties go to the lower one.  Where too many reach T
 // (equal logits), the exact n-th largest of the threads' maxima is built from the top bit, and its bits continued over the indices, after
 // which at most n threads' elements remain.  Blocks stay and take chunk after chunk, the next one's logits on their way to registers.
+// Measured: 24 x 8 rows of 128000 bf16 logits 31.5 us (1.56 TB/s of the 7.5 us that HBM would need: the barriers and the warp-wide
+// steps of a chunk bind it, three blocks an SM; spans of chunks with a running bound took 34-43 us), 4 rows of 32000 floats 4.2 us,
+// the merge 10 and 5 us, the reordering 18 us for 99 MB (5.4 TB/s) and 6 us.
 // Of the lists' heads, whose beams' scores lie apart, the exact n-th largest is taken at once; where too many reach it, n rounds of a
 // block-wide maximum over the heads.
 #include <algorithm>
