@@ -12,9 +12,9 @@
 // collected in shared memory and ranked by counting, with the index, so that ties go to the lower one.  Where too many reach T
 // (equal logits), the exact n-th largest of the threads' maxima is built from the top bit, and its bits continued over the indices, after
 // which at most n threads' elements remain.  Blocks stay and take chunk after chunk, the next one's logits on their way to registers.
-// Measured: 24 x 8 rows of 128000 bf16 logits 31.5 us (1.56 TB/s of the 7.5 us that HBM would need: the barriers and the warp-wide
-// steps of a chunk bind it, three blocks an SM; spans of chunks with a running bound took 34-43 us), 4 rows of 32000 floats 4.2 us,
-// the merge 10 and 5 us, the reordering 18 us for 99 MB (5.4 TB/s) and 6 us.
+// Measured: 24 x 8 rows of 128000 bf16 logits 34 us (1.4 TB/s: the barriers and the warp-wide steps of a chunk bind it, three blocks
+// an SM; spans of chunks with a running bound took longer), with two of eight beams ended 26.5 us (31.5 us before the live rows
+// were listed), 4 rows of 32000 floats 4.2 us; the merge 10 and 5 us; the reordering 18 us for 67 MB (3.7 TB/s) and 6 us.
 // Of the lists' heads, whose beams' scores lie apart, the exact n-th largest is taken at once; where too many reach it, n rounds of a
 // block-wide maximum over the heads.
 #include <algorithm>
@@ -27,6 +27,7 @@ namespace {
 constexpr int kBT = 256;      // threads
 constexpr int kMaxOut = 64;   // n_out and beams
 constexpr int kGroups = 256;  // 16-byte groups of logits of a chunk that may reach the bound before it counts as one with too many
+constexpr int kListed = 1024;  // rows of a call whose live ones are listed
 constexpr int kLeast = 4096;  // logits of the smallest chunk
 // logits per thread: 4 16-byte loads
 template <typename T>
@@ -114,19 +115,40 @@ __global__ void __launch_bounds__(kBT, 3) beam_chunk_kernel(const SelArgs a) {
     __shared__ float red[kBT / 32];
     __shared__ double redd[kBT / 32];
     __shared__ int cnt_s;
+    __shared__ uint16_t list_s[kListed];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_launch_dependents();
-    const int total = a.prompts * a.beams * a.chunks;
+    const int rows = a.prompts * a.beams;
+    int total = rows * a.chunks;
     // the second kernel does not look at the lists of a finished or dead beam
-    auto live_row = [&](int item) {
-        if (item >= total) return false;
-        const int row = item / a.chunks;
+    auto live = [&](int row) {
         const bool ended = a.finished && a.finished[row];
         return a.scores[row] > -INFINITY && !ended;
     };
+    // blocks with several chunks share out those of the live rows alone; where each has one, a dead row's has nothing to do
+    const bool listed = total > (int)gridDim.x && rows <= kListed;
+    if (listed) {
+        int n = 0;
+        for (int r0 = 0; r0 < rows; r0 += kBT) {
+            const bool mine = r0 + tid < rows && live(r0 + tid);
+            const unsigned votes = __ballot_sync(0xffffffffu, mine);
+            if (lane == 0) kth[warp] = __popc(votes);
+            __syncthreads();
+            int at = n + __popc(votes & ((1u << lane) - 1));
+            for (int w = 0; w < kBT / 32; w++) {
+                if (w < warp) at += kth[w];
+                n += kth[w];
+            }
+            if (mine) list_s[at] = (uint16_t)(r0 + tid);
+            __syncthreads();
+        }
+        total = n * a.chunks;
+    }
+    auto row_of = [&](int item) { return listed ? (int)list_s[item / a.chunks] : item / a.chunks; };
+    auto live_item = [&](int item) { return item < total && (listed || live(item / a.chunks)); };
     Chunk<T, C> raw[E / C] = {};
     auto fetch = [&](int item) {  // -inf past the end
-        const int row = item / a.chunks, base = item % a.chunks * a.chunk, nel = min(a.chunk, a.vocab - base);
+        const int row = row_of(item), base = item % a.chunks * a.chunk, nel = min(a.chunk, a.vocab - base);
         const T *x = (const T *)a.logits + (int64_t)row * a.ld + base;
         const bool vec = ((uintptr_t)x & 15) == 0;
 #pragma unroll
@@ -143,11 +165,11 @@ __global__ void __launch_bounds__(kBT, 3) beam_chunk_kernel(const SelArgs a) {
             }
         }
     };
-    bool live = live_row(blockIdx.x), live_next = live_row(blockIdx.x + gridDim.x);
-    if (live) fetch(blockIdx.x);
+    bool here = live_item(blockIdx.x), next = live_item(blockIdx.x + gridDim.x);
+    if (here) fetch(blockIdx.x);
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const bool now = live;
-    const int chunk = item % a.chunks, row = item / a.chunks;
+    const bool now = here;
+    const int chunk = item % a.chunks, row = row_of(item);
     const int base = chunk * a.chunk, nel = min(a.chunk, a.vocab - base), n = min(a.n_out, nel);
     auto place = [&](int k) { return ((k / C) * kBT + tid) * C + k % C; };  // in the chunk
     float v[E];
@@ -158,9 +180,9 @@ __global__ void __launch_bounds__(kBT, 3) beam_chunk_kernel(const SelArgs a) {
 #pragma unroll
         for (int i = 0; i < C; i++) v[j * C + i] = t[i];
     }
-    live = live_next;
-    if (live) fetch(item + gridDim.x);
-    live_next = live_row(item + 2 * gridDim.x);
+    here = next;
+    if (here) fetch(item + gridDim.x);
+    next = live_item(item + 2 * gridDim.x);
     if (!now) continue;
 
     float top[E / C], best = -INFINITY;  // NaN counts as -inf: maxima pass it over
