@@ -14,7 +14,7 @@
 // which at most n threads' elements remain.  Blocks stay and take chunk after chunk, the next one's logits on their way to registers.
 // Measured: 24 x 8 rows of 128000 bf16 logits 34 us (1.4 TB/s: the barriers and the warp-wide steps of a chunk bind it, three blocks
 // an SM; spans of chunks with a running bound took longer), with two of eight beams ended 26.5 us (31.5 us before the live rows
-// were listed), 4 rows of 32000 floats 4.2 us; the merge 10 and 5 us; the reordering 18 us for 67 MB (3.7 TB/s) and 6 us.
+// were listed), 4 rows of 32000 floats 4.2 us; the merge 10 and 5 us; the reordering 15 us for 67 MB (4.5 TB/s) and 6 us.
 // Of the lists' heads, whose beams' scores lie apart, the exact n-th largest is taken at once; where too many reach it, n rounds of a
 // block-wide maximum over the heads.
 #include <algorithm>
@@ -478,14 +478,20 @@ struct ReorderArgs {
     int *tout, *err;
 };
 
-// blockIdx.x: row; blockIdx.y, + gridDim.y, ...: layer.  Every block works out its beam's parent and pages from the
-// prompt's parents; the first of a row writes the table.
+constexpr int kPiece = 4 * 16 * kBT;  // bytes of keys, and of values, that a block copies at a time: eight loads a thread on their way
+
+// blockIdx.x: prompt; its blocks work out all beams' pages from the prompt's parents, and share its table rows and the pieces of its
+// copies evenly.  Bound by latency: length, parents, table entries and the copies follow on one another, so every block stays
+// for several pieces and all run at once (192 beams of 16 layers, two of eight beams ended, with the
+// selection before it: 53.1 us with a block for each beam and few layers, 52.2 so).
 __global__ void __launch_bounds__(kBT) beam_reorder_kernel(const ReorderArgs a) {
-    __shared__ int par[kMaxOut];
-    __shared__ uint8_t has[kMaxOut], first[kMaxOut];
-    const int row = blockIdx.x, prompt = row / a.beams, j = row % a.beams, tid = threadIdx.x;
+    __shared__ int par[kMaxOut], owner[kMaxOut];  // owner: the beam whose page being filled becomes this one's
+    __shared__ int2 copy[kMaxOut];                // pages from and to, of the further children in order
+    __shared__ uint8_t has[kMaxOut], first[kMaxOut], child[kMaxOut];
+    __shared__ int copies_s;
+    const int prompt = blockIdx.x, tid = threadIdx.x;
     pdl_wait();
-    int n = a.lens[prompt * a.beams];
+    int n = a.lens[(int64_t)prompt * a.beams];
     if (n < 0) {
         if (tid == 0) raise_error(a.err, kErrBadIndex);
         n = 0;
@@ -508,48 +514,60 @@ __global__ void __launch_bounds__(kBT) beam_reorder_kernel(const ReorderArgs a) 
         has[par[tid]] = 1;
     }
     __syncthreads();
-    int owner = par[j];  // the beam whose page being filled becomes this one's
-    if (!first[j]) {
-        int e = 0;
-        for (int i = 0; i < j; i++) e += !first[i];
-        // as many beams have no child as there are further children
-        for (int i = 0; i < a.beams; i++)
-            if (!has[i] && e-- == 0) {
-                owner = i;
-                break;
-            }
+    if (tid < a.beams) {
+        int e = 0, o = par[tid];
+        for (int i = 0; i < tid; i++) e += !first[i];
+        if (tid == a.beams - 1) copies_s = e + !first[tid];
+        if (!first[tid]) {
+            child[e] = (uint8_t)tid;
+            // as many beams have no child as there are further children
+            for (int i = 0; i < a.beams; i++)
+                if (!has[i] && e-- == 0) {
+                    o = i;
+                    break;
+                }
+        }
+        owner[tid] = o;
     }
-    const int *own = a.tin + (int64_t)row * a.ld_table, *from = a.tin + (int64_t)(prompt * a.beams + par[j]) * a.ld_table,
-              *give = a.tin + (int64_t)(prompt * a.beams + owner) * a.ld_table;
-    if (blockIdx.y == 0) {
-        int *out = a.tout + (int64_t)row * a.ld_table;
+    __syncthreads();
+    const int *const rows = a.tin + (int64_t)prompt * a.beams * a.ld_table;
+    if (tid < copies_s && filled) {
+        const int j = child[tid];
+        int2 c = make_int2(-1, -1);
+        if (tail < a.ld_table) c = make_int2(rows[(int64_t)par[j] * a.ld_table + tail], rows[(int64_t)owner[j] * a.ld_table + tail]);
+        if (c.x < 0 || c.x >= a.n_pages || c.y < 0 || c.y >= a.n_pages) {
+            raise_error(a.err, kErrBadIndex);
+            c.x = -1;
+        }
+        copy[tid] = c;
+    }
+    for (int j = blockIdx.y; j < a.beams; j += gridDim.y) {
+        const int *own = rows + (int64_t)j * a.ld_table, *from = rows + (int64_t)par[j] * a.ld_table, *give = rows + (int64_t)owner[j] * a.ld_table;
+        int *out = a.tout + ((int64_t)prompt * a.beams + j) * a.ld_table;
         for (int i = tid; i < a.ld_table; i += kBT) out[i] = i < tail ? from[i] : i == tail ? give[i] : own[i];
     }
-    if (first[j] || filled == 0) return;
-    const int src = tail < a.ld_table ? from[tail] : -1, dst = tail < a.ld_table ? give[tail] : -1;
-    if (src < 0 || src >= a.n_pages || dst < 0 || dst >= a.n_pages) {
-        if (tid == 0) raise_error(a.err, kErrBadIndex);
-        return;
-    }
+    __syncthreads();
+    if (filled == 0) return;
     const int64_t bytes = filled * a.slot_bytes;
-    for (int y = blockIdx.y; y < a.layers; y += gridDim.y) {
-        const int64_t from_at = y * a.layer_bytes + src * a.page_bytes, to_at = y * a.layer_bytes + dst * a.page_bytes;
+    const unsigned copies = copies_s, pieces = (unsigned)((bytes + kPiece - 1) / kPiece), units = copies * pieces * a.layers;  // below 2^31
+    for (unsigned u = blockIdx.y; u < units; u += gridDim.y) {
+        const int2 c = copy[u % copies];
+        if (c.x < 0) continue;
+        const int64_t layer = u / copies / pieces * a.layer_bytes, at = (int64_t)(u / copies % pieces) * kPiece, left = min((int64_t)kPiece, bytes - at);
+        const int64_t from_at = layer + c.x * a.page_bytes + at, to_at = layer + c.y * a.page_bytes + at;
         uint8_t *const k = a.pool[0], *const v = a.pool[1];
-        if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)from_at | (uintptr_t)to_at | (uintptr_t)bytes) & 15) == 0) {
-            const int64_t n = bytes / 16;
+        if ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)from_at | (uintptr_t)to_at | (uintptr_t)left) & 15) == 0) {
             const uint4 *ks = (const uint4 *)(k + from_at), *vs = (const uint4 *)(v + from_at);
             uint4 *kd = (uint4 *)(k + to_at), *vd = (uint4 *)(v + to_at);
-            for (int64_t i = tid; i < n; i += 4 * kBT) {  // eight loads on their way
-                uint4 x[4], z[4];
+            uint4 x[4], z[4];
 #pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (i + u * kBT < n) x[u] = __ldcs(ks + i + u * kBT), z[u] = __ldcs(vs + i + u * kBT);
+            for (int i = 0; i < 4; i++)
+                if (16 * (tid + i * kBT) < left) x[i] = __ldcs(ks + tid + i * kBT), z[i] = __ldcs(vs + tid + i * kBT);
 #pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (i + u * kBT < n) kd[i + u * kBT] = x[u], vd[i + u * kBT] = z[u];
-            }
+            for (int i = 0; i < 4; i++)
+                if (16 * (tid + i * kBT) < left) kd[tid + i * kBT] = x[i], vd[tid + i * kBT] = z[i];
         } else {
-            for (int64_t i = tid; i < bytes / 2; i += kBT) {
+            for (int64_t i = tid; i < left / 2; i += kBT) {
                 ((uint16_t *)(k + to_at))[i] = ((const uint16_t *)(k + from_at))[i];
                 ((uint16_t *)(v + to_at))[i] = ((const uint16_t *)(v + from_at))[i];
             }
@@ -634,6 +652,9 @@ int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t be
                          ld_parents, ld_table);
     if (cache->n_layers > 1 << 20) return set_error(QMC_EINVAL, "%s: %d layers", op, cache->n_layers);
     if ((int64_t)n_prompts * beams > INT32_MAX) return set_error(QMC_EINVAL, "%s: too many rows", op);
+    const int64_t page_bytes = (int64_t)cache->n_kv_heads * cache->head_dim * dtype_size(cache->dtype) * cache->page_size;
+    const int64_t most = (int64_t)beams * cache->n_layers * ((page_bytes + kPiece - 1) / kPiece);  // pieces of a prompt
+    if (most > INT32_MAX) return set_error(QMC_EINVAL, "%s: %d beams of %d layers of such pages are too many", op, beams, cache->n_layers);
     if (n_prompts == 0) return QMC_OK;
     if (!parents || !seq_lens || !page_table || !page_table_out) return set_error(QMC_EINVAL, "%s: null argument", op);
     if (page_table == page_table_out) return set_error(QMC_EINVAL, "%s: the table cannot be reordered in place", op);
@@ -643,16 +664,16 @@ int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t be
     const int64_t sz = dtype_size(cache->dtype);
     a.pool[0] = (uint8_t *)cache->k, a.pool[1] = (uint8_t *)cache->v;
     a.slot_bytes = (int64_t)cache->n_kv_heads * cache->head_dim * sz;
-    a.page_bytes = a.slot_bytes * cache->page_size;
+    a.page_bytes = page_bytes;
     a.layer_bytes = a.page_bytes * cache->n_pages;
     a.n_pages = cache->n_pages, a.page_size = cache->page_size, a.beams = beams;
     a.ld_parents = ld_parents, a.ld_table = ld_table;
     a.parents = parents, a.lens = seq_lens, a.tin = page_table, a.tout = page_table_out, a.err = c->err;
-    // a third of the beams copy: enough blocks of them to fill the SMs, each with several layers.  It may start while the
-    // selection before it ends, and reads nothing before it has ended.
+    // as many blocks as run at once, as far as there are pieces.  They may start while the selection before them ends, and read
+    // nothing before it has ended.
     a.layers = cache->n_layers;
-    const int64_t rows = (int64_t)n_prompts * beams, want = (16 * c->num_sms + rows - 1) / rows;
-    const dim3 grid((unsigned)rows, (unsigned)(want < a.layers ? want : a.layers));
+    const int64_t want = (3 * c->num_sms + n_prompts - 1) / n_prompts;
+    const dim3 grid((unsigned)n_prompts, (unsigned)std::min(want, most));
     return launch_after(beam_reorder_kernel, grid, kBT, 0, pick_stream(stream), true, a);
 }
 

@@ -172,3 +172,8 @@ def test_sizes_counted_in_32_bits_are_bounded():
     p = qb.RopePlan(2)
     refused(qb.cuda().qmc_qk_norm_rope(p.h, 0, A, 1 << 30, A, 1 << 30, many, None, 0, None, 0, 0, None, None, 0.0, A, 1, None), "too many")
     refused(qb.cuda().qmc_qk_norm_rope(p.h, 0, None, 0, None, 0, 0, A, 1 << 30, A, 1 << 30, 2**31 - 1, None, None, 0.0, A, 1, None))
+
+
+def test_beam_reorder_refuses_pages_of_too_many_pieces():
+    c = cache(n_layers=1 << 20, n_pages=1, page_size=1 << 20, n_kv_heads=1, head_dim=256)
+    refused(reorder(c, beams=64, ldp=64), "too many")
