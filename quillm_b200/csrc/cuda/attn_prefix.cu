@@ -243,8 +243,8 @@ bool takes_mma(const qmc_paged_cache *c) {
 // The time of a call whose prefix blocks and own jobs are split into n and m position ranges, in the microseconds that one block takes
 // while its SM runs as many as fit.  The prefix's blocks come first; own jobs take the places that these leave, and all places
 // once they are done.  Sequences are taken to be half as long as the table allows, the last job as long as the longest.  The constants
-// come from sweeps of both numbers over a dozen shapes; the numbers it picks are within 5 % of the best of each sweep in all but one
-// (document of 8192 for 16 sequences: 8 ranges and 1, 29.6 us; 4: 35, 16: 46; 64 x 32768: 7 ranges 90, 6: 100, 9: 101).
+// come from sweeps of both numbers over a dozen shapes; the numbers it picks are within 10 % of the best of each sweep (16 sequences
+// behind 8192 positions: 8 ranges and 1, 29.6 us; 6: 30.9, 12: 38, 16: 46; 64 behind 32768: 7 ranges 90, 6: 100, 9: 101).
 struct Work {
     double start, tile;  // of a block: its start, end and parts' way through memory, and each tile of positions
     int64_t units;       // row tiles
