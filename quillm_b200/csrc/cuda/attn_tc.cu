@@ -153,14 +153,23 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^t of a pair without the special-function unit, t in [-126, 127]: n = t rounded to an integer (as the low bits of t +
-// 1.5 * 2^23), 2^(t - n) by the minimax polynomial of the relative error on [-1/2, 1/2] (degree 3: 2^-13.7, under a bf16 step's
-// 1/50; degree 4: 2^-18.5, for fp16), n added to its exponent
+// x * y + c held in [0, 1]
+__device__ __forceinline__ float fma_sat(float x, float y, float c) {
+    float r;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(c));
+    return r;
+}
+// 2^t of a pair without the special-function unit.  t comes as x = (t + 112) / 128, held in [0, 1] by the instruction that forms it: below
+// 2^-112 a weight counts for nothing, and 2^16 is above what a tile's sum may reach, so that the reference moves (beyond 127 the
+// exponent would run into the sign).  x is off by 2^-25, the result by 2^-18.5 of itself.  n = t rounded to an integer (as the low
+// bits of t + 1.5 * 2^23), 2^(t - n) by the minimax polynomial of the relative error on [-1/2, 1/2] (degree 3: 2^-13.7, under a bf16
+// step's 1/50; degree 4: 2^-18.5, for fp16), n added to its exponent
+constexpr float kSpan = 128.0f, kBelow = 112.0f;
 template <bool BF>
-__device__ __forceinline__ void ex2_pair(uint64_t t, float &p0, float &p1) {
+__device__ __forceinline__ void ex2_pair(uint64_t x, float &p0, float &p1) {
     const float kRnd = 12582912.0f;
-    const uint64_t up = add2(t, pair_of(kRnd, kRnd)), n = add2(up, pair_of(-kRnd, -kRnd));
-    const uint64_t f = fma2(n, pair_of(-1.0f, -1.0f), t);
+    const uint64_t span = pair_of(kSpan, kSpan), rnd = pair_of(kRnd - kBelow, kRnd - kBelow);
+    const uint64_t up = fma2(x, span, rnd), f = fma2(x, span, fma2(up, pair_of(-1.0f, -1.0f), rnd));
     uint64_t v;
     if (BF) {
         v = fma2(f, pair_of(0.05517166852951f, 0.05517166852951f), pair_of(0.24261112511158f, 0.24261112511158f));
@@ -185,20 +194,22 @@ template <typename CT, bool MASK>
 __device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *pk, float scale, float m, int left) {
     constexpr bool BF = __is_same(CT, __nv_bfloat16);
     const uint64_t sc = pair_of(scale, scale), mm = pair_of(-m, -m);
+    const float part = scale * (1.0f / kSpan), from = (kBelow - m) * (1.0f / kSpan);
     const uint32_t live = MASK ? live_bits(left, 0) : 0xffffffffu;
     uint64_t sum[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 32; k += 2) {
-        const uint64_t t = fma2(pair_of(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sc, mm);
-        float t0, t1, p0, p1;
-        of_pair(t, t0, t1);
-        if (MASK) {
-            t0 = live >> k & 1u ? t0 : -INFINITY;
-            t1 = live >> (k + 1) & 1u ? t1 : -INFINITY;
-        }
+        const float s0 = __uint_as_float(x[k]), s1 = __uint_as_float(x[k + 1]);
+        float p0, p1;
         if (!MASK && (k >> 1) % 8 % 3 == 1) {
-            ex2_pair<BF>(pair_of(fmaxf(t0, -126.0f), fmaxf(t1, -126.0f)), p0, p1);
+            ex2_pair<BF>(pair_of(fma_sat(s0, part, from), fma_sat(s1, part, from)), p0, p1);
         } else {
+            float t0, t1;
+            of_pair(fma2(pair_of(s0, s1), sc, mm), t0, t1);
+            if (MASK) {
+                t0 = live >> k & 1u ? t0 : -INFINITY;
+                t1 = live >> (k + 1) & 1u ? t1 : -INFINITY;
+            }
             p0 = ex2(t0), p1 = ex2(t1);
         }
         sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(p0, p1));

@@ -1,0 +1,107 @@
+"""The batched-decoding operators where values are extreme and blocks have many tiles, against plain forms in 64 bits:
+scores that rise far above a row's first tile, softmax weights far below the largest, infinities beside dimensions that
+stay, rows of logits with infinities.
+
+Tolerances as in test_gpu_batch_ops.py (u = 2^-24, e and e_P half steps of the output's and the weights' type); what a test
+adds to them stands beside it."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import quillm_b200 as qb
+from test_gpu_batch_ops import CODE, DT, E, TINY, U, clean, do_attn, gen, lib, plan, pools, rand
+
+pytestmark = pytest.mark.gpu
+LOG2E = 1.4426950408889634
+
+
+def shared(g, kv, hd, prefix, page, cdt, std=1.0):
+    """a cache that holds one prefix of whole pages, the prefix's pages, and its keys and values as views by position"""
+    n = prefix // page
+    assert n * page == prefix
+    kp, vp, c = pools(g, 1, n, page, kv, hd, cdt)
+    kp.mul_(std)
+    pp = torch.randperm(n, generator=g, device="cuda").to(torch.int32)
+    slot = (pp.long()[:, None] * page + torch.arange(page, device="cuda")).view(-1)
+    return kp.view(-1, kv, hd), vp.view(-1, kv, hd), c, pp, slot
+
+
+def ranges(c, dtype, n_seq, heads, hd, prefix, page):
+    """position ranges that the prefix is split into: without own positions the workspace is [ranges][rows] (m, l) and o, and 256
+    bytes over"""
+    n = qb.attn_prefix_workspace(CODE[dtype], c, n_seq, heads, prefix, prefix // page)
+    return (n - 256) // (n_seq * heads * (8 + 4 * hd))
+
+
+def over_prefix(c, dtype, q, heads, hd, scale, pp, prefix, page):
+    """the attention of rows that have the prefix alone, twice: the same bits"""
+    n_seq, width = q.shape[0], prefix // page
+    table = torch.full((n_seq, width), -9, dtype=torch.int32, device="cuda")
+    lens = torch.full((n_seq,), prefix, dtype=torch.int32, device="cuda")
+    outs = []
+    for _ in range(2):
+        outs.append(torch.full((n_seq, heads * hd), 77.0, dtype=DT[dtype], device="cuda"))
+        do_attn(c, 0, dtype, q, outs[-1], heads, scale, pp, prefix, table, lens)
+    clean()
+    bits = [o.view(torch.int32 if dtype == "f32" else torch.int16) for o in outs]
+    assert torch.equal(*bits)
+    return outs[0]
+
+
+def check_prefix(got, q, keys, values, slot, kv, hd, scale, dtype, cdt, floor=0.0):
+    """floor: added, of the largest value, for weights far below the largest of their tile"""
+    n_seq = q.shape[0]
+    x = q.double().view(n_seq, kv, -1, hd).transpose(0, 1).flatten(1, 2)  # [kv, rows, hd]
+    y = got.double().view(n_seq, kv, -1, hd).transpose(0, 1).flatten(1, 2)
+    for h in range(kv):
+        k, v = keys[slot, h].double(), values[slot, h].double()
+        w = torch.softmax(scale * (x[h] @ k.T), 1)
+        want, mag = w @ v, w @ v.abs()
+        big = scale * (x[h].abs() @ k.abs().T).amax(1, keepdim=True)
+        ds = (hd + 8) * U * big + (2.0**-21 * big if dtype != cdt else 0)
+        ep = E[cdt] if dtype == cdt and dtype != "f32" else 2.0**-20
+        tol = 2 * (2 * ds + 2.0**-20 + ep) * mag + E[dtype] * want.abs() + TINY[dtype] + floor * v.abs().max()
+        bad = ~((y[h] - want).abs() <= tol)
+        assert not bad.any(), (h, bad.nonzero()[:4].tolist(), y[h][bad][:4].tolist(), want[bad][:4].tolist(), tol[bad][:4].tolist())
+
+
+# kernels of the prefix: type of rows and cache, sequences, query heads of a KV head, head_dim, page, positions of a tile; 148 KV heads fill
+# the SMs, so that a block has several tiles
+MANY = {"tc": ("f16", "f16", 20, 1, 64, 16, 128), "tc bf16": ("bf16", "bf16", 20, 1, 64, 16, 128),
+        "tc pair": ("f16", "f16", 17, 8, 64, 32, 128), "tc pair bf16": ("bf16", "bf16", 17, 8, 64, 32, 128),
+        "tc wide": ("f16", "f16", 5, 8, 128, 64, 128), "tc wide bf16": ("bf16", "bf16", 33, 4, 120, 8, 128),
+        "warp": ("f16", "f16", 3, 4, 64, 16, 64), "warp bf16": ("bf16", "bf16", 2, 8, 128, 16, 64), "warp f32": ("f32", "f16", 4, 2, 128, 16, 64),
+        "mma 32": ("f16", "f16", 20, 1, 64, 4, 64), "mma 64": ("bf16", "bf16", 20, 2, 128, 4, 64), "mma f32": ("f32", "f16", 20, 1, 64, 16, 64),
+        "mma 256": ("f16", "f16", 3, 2, 256, 16, 64), "mma 256 f32": ("f32", "f16", 9, 4, 200, 16, 64),
+        "vec": ("f32", "f32", 3, 2, 64, 16, 32), "rows": ("f16", "f16", 3, 2, 36, 16, 32)}
+
+
+def many(name, prefix=1536, std=0.05):
+    dtype, cdt, n_seq, group, hd, page, tile = MANY[name]
+    kv, g = 148, gen(len(name) + 1000 * n_seq)
+    keys, values, c, pp, slot = shared(g, kv, hd, prefix, page, cdt, std)
+    q = rand(g, (n_seq, kv * group * hd), dtype)
+    n = ranges(c, dtype, n_seq, kv * group, hd, prefix, page)
+    assert -(-prefix // tile) // n >= 4, n  # a block has four tiles and more
+    return dtype, cdt, n_seq, kv, group, hd, page, keys, values, c, pp, slot, q
+
+
+@pytest.mark.parametrize("name", list(MANY))
+def test_attn_scores_far_above_the_first_tile(cuda_dev, name):
+    """for one row of a KV head a key scores 9 to 300 powers of two above what came before it, in every later tile of a block
+    and at every offset modulo 16; the other rows, whose scores stay, do not move the reference for it"""
+    prefix = 1536
+    dtype, cdt, n_seq, kv, group, hd, page, keys, values, c, pp, slot, q = many(name, prefix)
+    scale = 1.0 / math.sqrt(hd)
+    x = q.view(n_seq, kv, group, hd)
+    x[..., 0] = 0
+    for h in range(kv):
+        p = 128 * (1 + h % 11) + 16 * (h // 16 % 8) + h % 16
+        up = [9, 60, 130, 200, 300][h % 5]
+        x[h % n_seq, h, h % group, 0] = 8
+        keys[slot[p], h] = 0
+        keys[slot[p], h, 0] = up / LOG2E / (8 * scale)
+    out = over_prefix(c, dtype, q, kv * group, hd, scale, pp, prefix, page)
+    check_prefix(out, q, keys, values, slot, kv, hd, scale, dtype, cdt)
