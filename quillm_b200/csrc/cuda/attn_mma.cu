@@ -11,9 +11,10 @@
 // TFLOP/s; float rows, of twice the products each way, 447 us), with few rows by the copies (32 rows 46 us, 2.9 TB/s).  Its cases are
 // those that the faster two cannot take: pages that are no multiple of 8, float rows in number, heads above 128.
 //
-// Weights are rounded to the cache's type for the second product (at most half a step each, as the outputs are).  Float
-// queries over an fp16 cache keep float accuracy: a row is scaled by a power of two and split in two halves q = qh + ql,
-// the weights likewise, and each product is taken twice.
+// Weights are rounded to the cache's type for the second product: bf16 by half a step each at most, as the outputs are, fp16 likewise down to
+// 2^-12 of the largest of its tile (Window).  Float queries over an fp16 cache: a row is scaled by a power of two and split in two halves
+// q = qh + ql, the weights likewise, and each product is taken twice.  A score is off by 2^-21 of sum |q k|, a weight by 2^-22 of itself
+// or 2^-23 of the largest of its tile.
 #include "attn_prefix.cuh"
 
 namespace qmc {
@@ -169,7 +170,8 @@ __device__ __forceinline__ void mma_job(const AttnArgs &a, const Job &jb, uint8_
         }
     }
 
-    float o[HDP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    using W = Window<CT>;
+    float o[HDP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, high[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int d = 0; d < HDP / 8; d++)
 #pragma unroll
@@ -221,7 +223,7 @@ __device__ __forceinline__ void mma_job(const AttnArgs &a, const Job &jb, uint8_
             }
         }
         const int left = jb.p1 - jb.p0 - t * kTP - PW * wn;  // positions of this warp's part that exist
-        float mx[2] = {m[0], m[1]};
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -234,9 +236,10 @@ __device__ __forceinline__ void mma_job(const AttnArgs &a, const Job &jb, uint8_
         for (int i = 0; i < 2; i++) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-            ref[i] = mx[i] == -INFINITY ? 0.0f : mx[i];
+            const float to = W::moved(m[i], mx[i], high[i]);
+            ref[i] = to == -INFINITY ? 0.0f : to;
             const float corr = ex2(m[i] - ref[i]);
-            m[i] = mx[i];
+            m[i] = to;
             l[i] *= corr;
 #pragma unroll
             for (int d = 0; d < HDP / 8; d++) o[d][2 * i] *= corr, o[d][2 * i + 1] *= corr;

@@ -4,9 +4,9 @@
 // Per 128 query rows and 128 positions: S = Q K^T (M = 128 rows, N = 128 positions) into 128 TMEM columns; eight warps, two
 // threads per row with 64 positions each, turn S into weights P = 2^(scale S - m) and write them over S as 16-bit pairs;
 // O += P V with P read from TMEM as the A operand and V from shared memory as it lies in the cache ([position][dim], an
-// MN-major operand).  A row's reference m moves only when a thread's weights add up to more than kMost (so each stays below
-// that, exact in the split of l and O): then the row's two warps rescale its O in TMEM and take the tile again, which after
-// a row's first tile is rare, so O normally stays where it is until the end.
+// MN-major operand).  A row's reference m moves only when a thread's weights show that the scores have left the window around it
+// (Window): sums above what its type or l can hold, or, in fp16, too small to keep a weight's bits.  Then the row's two warps rescale
+// its O in TMEM and take the tile again, which after a row's first tile is rare, so O normally stays where it is until the end.
 //
 // A block runs two streams of such tiles, so that the tensor cores work on one while the other's warps take its exponentials.
 // PAIR: the streams are two row tiles over the same positions (each K and V tile is read once for 256 rows).  Otherwise, with
@@ -34,7 +34,14 @@ namespace {
 
 constexpr int kM = 128, kN = 128;  // rows and positions of a tile
 constexpr int kCopyWarp = 16, kMmaWarp = 17, kThreads = 18 * 32;  // warps 0-15: weights
-constexpr float kMost = 256.0f;    // that a thread's weights of a tile may add up to
+// what a thread's weights may add up to, in bf16 the 64 of a tile, in fp16 each eight, of which none then passes the type's largest (level
+// scores at the reference's 2^10: 2^13); and in fp16 the least that a tile's must
+template <typename CT>
+__host__ __device__ constexpr float most_of() {
+    return Window<CT>::kHalf ? 65504.0f : 256.0f;
+}
+constexpr float kLeast = 0.25f;
+constexpr float kLiftSum = 12.5f;  // fp16: a tile whose eight weights pass 65504 has one at 2^12.99 or above
 
 template <int HDP>
 __host__ __device__ constexpr int tile_bytes() {  // of Q, K or V
@@ -187,11 +194,11 @@ __device__ __forceinline__ void ex2_pair(uint64_t x, float &p0, float &p1) {
     p0 = __int_as_float(__float_as_int(v0) + (__float_as_int(u0) << 23));
     p1 = __int_as_float(__float_as_int(v1) + (__float_as_int(u1) << 23));
 }
-// a thread's 32 scores of a row: 2^(scale s - m) as 16-bit pairs in pk, and their sum before rounding.  The special-function unit gives
-// 16 results a cycle and SM: three of every eight pairs, spread among the others, go to the FMA pipe instead.
-// MASK: only the first `left` positions exist
+// a thread's 32 scores of a row: 2^(scale s - m) as 16-bit pairs in pk, and their sum before rounding; most: the largest sum of eight of
+// them.  The special-function unit gives 16 results a cycle and SM: three of every eight pairs, spread among the others, go to the FMA
+// pipe instead.  MASK: only the first `left` positions exist
 template <typename CT, bool MASK>
-__device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *pk, float scale, float m, int left) {
+__device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *pk, float scale, float m, int left, float &most) {
     constexpr bool BF = __is_same(CT, __nv_bfloat16);
     const uint64_t sc = pair_of(scale, scale), mm = pair_of(-m, -m);
     const float part = scale * (1.0f / kSpan), from = (kBelow - m) * (1.0f / kSpan);
@@ -216,6 +223,12 @@ __device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *
         pk[k / 2] = pack2(CT(), p0, p1);
     }
     float s0, s1;
+    if constexpr (Window<CT>::kHalf) {
+        float s2, s3;
+        of_pair(sum[0], s0, s1), of_pair(sum[1], s2, s3);
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(s0), "f"(s1));
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(s2), "f"(s3));
+    }
     of_pair(add2(sum[0], sum[1]), s0, s1);
     return s0 + s1;
 }
@@ -446,7 +459,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             rows_any(id, false);
             return sh.top[w][row];
         };
-        float m = 0.0f, l = 0.0f;
+        using W = Window<CT>;
+        float m = 0.0f, l = 0.0f, high = -INFINITY;
         bool ok = true;
         for (int i = 0; i < mine; i++) {
             const int j = PAIR ? i : 2 * i + w, left = jb.p1 - jb.p0 - j * kN - 64 * half;  // of this thread's positions
@@ -456,21 +470,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
             tc_fence_after();
             uint32_t pk[32];
-            float sum = 0.0f;
+            float sum = 0.0f, most = 0.0f;
             for (int again = i == 0 ? -1 : 0;; again++) {  // -1: no reference yet
                 if (ok && again >= 0) {
-                    sum = 0.0f;
+                    sum = most = 0.0f;
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         uint32_t x[32];
                         tmem_ld32(ts + 64 * half + 32 * c, x);
-                        sum += left >= 64 ? row_weights<CT, false>(x, pk + 16 * c, a.scale, m, left)
-                                          : row_weights<CT, true>(x, pk + 16 * c, a.scale, m, left - 32 * c);
+                        sum += left >= 64 ? row_weights<CT, false>(x, pk + 16 * c, a.scale, m, left, most)
+                                          : row_weights<CT, true>(x, pk + 16 * c, a.scale, m, left - 32 * c, most);
                     }
                 }
-                // both have read the scores; does a row pass its reference?  After a lift none does
-                if (!rows_any(id, again < 0 || (again == 0 && i > 0 && !(sum <= kMost)))) break;
-                // the reference becomes the row's largest score, if that is above it
+                // both have read the scores; does a row leave its window (NaN sums count as that)?  After a move none does
+                bool out;
+                if constexpr (W::kHalf) out = !(most <= most_of<CT>()) || !(sum == sum) || (sum < kLeast && left > 0);
+                else out = !(sum <= most_of<CT>());
+                if (!rows_any(id, again < 0 || (again == 0 && i > 0 && out))) break;
                 float top = -INFINITY;
                 if (ok)
 #pragma unroll 1
@@ -483,20 +499,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 top = largest(top) * a.scale;
                 if (again < 0) {
-                    m = top == -INFINITY ? 0.0f : top;
+                    m = high = top == -INFINITY ? 0.0f : top - W::kTop;
                     continue;
                 }
                 // O (half of its columns each) holds the tiles before this one, whose product is complete (this tile's scores
                 // were committed after it)
-                const float to_m = fmaxf(m, top), down = ex2(m - to_m);
-                m = to_m, l *= down;
+                const float to_m = W::moved(m, top, high, kLiftSum), by = ex2(m - to_m);
+                m = to_m, l *= by;
                 if (ok)
 #pragma unroll 1
                     for (int c = 0; c < HDP / 64; c++) {
                         uint32_t x[32];
                         tmem_ld32(to + 32 * c, x);
 #pragma unroll
-                        for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * down);
+                        for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * by);
                         tmem_st32(to + 32 * c, x);
                     }
             }

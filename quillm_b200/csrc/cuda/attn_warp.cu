@@ -11,17 +11,16 @@
 //   products of 16 dimensions use one chunk, Q's chunks are held the same way;
 //   V (second operand of P V, rows = positions 2t, 2t + 1, 2t + 8, 2t + 9): it holds chunk g (and g + 8) of those positions' values, and
 //   element j of each is column g of product j, so that a product's 8 columns are dimensions j, 8 + j, ..., 56 + j.
-// A row's accumulators are rescaled only when a score passes the row's reference by more than 2^kLift; the four warps' parts are joined
+// A row's accumulators are rescaled only when its scores leave the window around its reference (Window); the four warps' parts are joined
 // through shared memory at the end.
 //
-// Float queries over an fp16 cache keep float accuracy: a row is scaled by a power of two and split in two halves q = qh + ql, the
-// weights likewise, and each product is taken twice.
+// Float queries over an fp16 cache: a row is scaled by a power of two and split in two halves q = qh + ql, the weights likewise, and
+// each product is taken twice.  A score is off by 2^-21 of sum |q k|, a weight by 2^-22 of itself or 2^-25 in the window's scale, 2^-23
+// of the largest of its 16 positions at most.
 #include "attn_prefix.cuh"
 
 namespace qmc {
 namespace {
-
-constexpr float kLift = 8.0f;
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22; below 2^-126 it is 0
     float y;
@@ -143,7 +142,8 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
             }
     }
 
-    float o[NC][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    using W = Window<CT>;
+    float o[NC][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, high[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -172,17 +172,23 @@ __global__ void __launch_bounds__(128, 2) attn_warp_kernel(const AttnArgs a) {
                 s[n][i] = 8 * n + 2 * t + (i & 1) < left ? s[n][i] * scale[i >> 1] : -INFINITY;
                 mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
             }
-        if (__any_sync(0xffffffffu, mx[0] > m[0] + kLift || mx[1] > m[1] + kLift)) {  // the first time, and rarely again
+        bool move = __any_sync(0xffffffffu, mx[0] > m[0] + W::kLift || mx[1] > m[1] + W::kLift);
+        if constexpr (W::kHalf) {  // is a row's every score below the window?  Four lanes hold a row
+            const unsigned in0 = __ballot_sync(0xffffffffu, mx[0] >= m[0] + W::kDrop), in1 = __ballot_sync(0xffffffffu, mx[1] >= m[1] + W::kDrop);
+            const unsigned x = in0 | in0 >> 1, y = in1 | in1 >> 1;
+            move = move || (((x | x >> 2) & (y | y >> 2)) & 0x11111111u) != 0x11111111u;
+        }
+        if (move) {  // the first time, and rarely again
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-                const float to = fmaxf(m[i], mx[i]), down = to == -INFINITY ? 1.0f : ex2(m[i] - to);
-                m[i] = to, l[i] *= down;
+                const float to = W::moved(m[i], mx[i], high[i]), by = to == -INFINITY ? 1.0f : ex2(m[i] - to);
+                m[i] = to, l[i] *= by;
 #pragma unroll
                 for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) o[c][j][2 * i] *= down, o[c][j][2 * i + 1] *= down;
+                    for (int j = 0; j < 8; j++) o[c][j][2 * i] *= by, o[c][j][2 * i + 1] *= by;
             }
         }
         uint32_t p[H][4];

@@ -105,3 +105,55 @@ def test_attn_scores_far_above_the_first_tile(cuda_dev, name):
         keys[slot[p], h, 0] = up / LOG2E / (8 * scale)
     out = over_prefix(c, dtype, q, kv * group, hd, scale, pp, prefix, page)
     check_prefix(out, q, keys, values, slot, kv, hd, scale, dtype, cdt)
+
+
+GAPS = [8, 11, 14, 16, 18, 20]  # natural exponents of a sink above the rest
+
+
+def sinks(g, q, keys, values, slot, where, kv, hd, scale):
+    """a KV head's key at position where(head), of value zero, scores GAPS[head % 6] above all others, which are nearly level and have
+    values that do not cancel: what is left of the output is the others' share, e^-gap of a value each"""
+    keys[..., 0] = 0
+    values.copy_(64 + 16 * torch.randn(values.shape, generator=g, device="cuda"))
+    q.view(q.shape[0], kv, -1, hd)[..., 0] = 8
+    for h in range(kv):
+        keys[slot[where(h)], h] = 0
+        keys[slot[where(h)], h, 0] = GAPS[h % 6] / (8 * scale)
+        values[slot[where(h)], h] = 0
+
+
+# added, of the largest value: a weight is off by 2^-25 where that is more than half its own step, a row's largest of a tile stands at 2^10
+# or above when the sink is in it, and up to 128 positions share the sink's tile: 2^7 2^-25 2^-10
+SINK_FLOOR = 2.0**-28
+
+
+@pytest.mark.parametrize("name", [n for n, case in MANY.items() if case[1] == "f16"])
+def test_attn_small_weights_beside_a_sink(cuda_dev, name):
+    prefix = 1536
+    dtype, cdt, n_seq, kv, group, hd, page, keys, values, c, pp, slot, q = many(name, prefix)
+    scale = 1.0 / math.sqrt(hd)
+    sinks(gen(5), q, keys, values, slot, lambda h: [0, 700, 1535, 130][h // 6 % 4], kv, hd, scale)
+    out = over_prefix(c, dtype, q, kv * group, hd, scale, pp, prefix, page)
+    check_prefix(out, q, keys, values, slot, kv, hd, scale, dtype, cdt, SINK_FLOOR)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attn_small_weights_beside_a_sink_of_its_own(cuda_dev, hd, dtype):
+    """the same in a sequence's own positions"""
+    kv, group, page, own, n_seq = 60, 4, 16, 2048, 5
+    g, scale, heads = gen(hd), 1.0 / math.sqrt(hd), 240
+    keys, values, c, pages, slot = shared(g, kv, hd, n_seq * own, page, "f16", 0.05)
+    q = rand(g, (n_seq, heads * hd), dtype)
+    for b in range(n_seq):
+        at = slot[b * own:(b + 1) * own]
+        k, v = keys[at], values[at]
+        sinks(g, q[b:b + 1], k, v, torch.arange(own), lambda h: [0, 900, 2000][h // 6 % 3], kv, hd, scale)
+        keys[at], values[at] = k, v
+    table = pages.view(n_seq, own // page).contiguous()
+    lens = torch.tensor([own, own - 40, own, own - 47, own], dtype=torch.int32, device="cuda")
+    out = torch.zeros_like(q)
+    do_attn(c, 0, dtype, q, out, heads, scale, torch.empty(0), 0, table, lens)
+    clean()
+    for b, n in enumerate(lens.tolist()):
+        check_prefix(out[b:b + 1], q[b:b + 1], keys, values, slot[b * own:b * own + n], kv, hd, scale, dtype, "f16", SINK_FLOOR)
