@@ -72,11 +72,12 @@ template <int C>
 __device__ __forceinline__ int spread(int t, int e) {
     return e ^ ((t / (8 / C)) & (C - 1));
 }
-// (a, b) of a pair through its row of the table, times the head's factor
-__device__ __forceinline__ void rotate(float &a, float &b, float4 r, float f) {
+// (a, b) of a pair through its row of the table, times the head's factor.  A pair that stays keeps its elements apart: a product with
+// the other's zero would be NaN for an infinite one
+__device__ __forceinline__ void rotate(float &a, float &b, float4 r, float f, bool turns) {
     const float u = a, v = b;
-    a = (u * r.x - v * r.y) * f;
-    b = (u * r.z + v * r.w) * f;
+    a = (turns ? u * r.x - v * r.y : u * r.x) * f;
+    b = (turns ? u * r.z + v * r.w : v * r.w) * f;
 }
 
 // T rows, CT cache elements, C elements per chunk, NIT items per lane, R rows a block: their elements are all on their way before
@@ -181,11 +182,14 @@ __global__ void __launch_bounds__(288, 3) rope_rows_kernel(const __grid_constant
                 if (!FULL && ea[j] >= hd) continue;
                 const int t = li + j * lph, x = spread<C>(t, 0);
                 const float4 *row = &tab[kind][k][t * C];
+                // rotated pairs of this item, none of which the item has left where that is all
+                const int turning = HALF ? (t < rot_items ? C : 0) : (a.rot >> 1) - t * C;
 #pragma unroll
                 for (int i = 0; i < C; i++) {
-                    if (HALF || C == 1) rotate(xa[j][i], xb[j][i], row[i ^ x], r);
-                    else if (i < C / 2) rotate(xa[j][2 * i % C], xa[j][(2 * i + 1) % C], row[i ^ x], r);
-                    else rotate(xb[j][2 * i % C], xb[j][(2 * i + 1) % C], row[i ^ x], r);
+                    const bool turns = i < turning;
+                    if (HALF || C == 1) rotate(xa[j][i], xb[j][i], row[i ^ x], r, turns);
+                    else if (i < C / 2) rotate(xa[j][2 * i % C], xa[j][(2 * i + 1) % C], row[i ^ x], r, turns);
+                    else rotate(xb[j][2 * i % C], xb[j][(2 * i + 1) % C], row[i ^ x], r, turns);
                 }
             }
         // rows past the last, and padding, have gone through this for nothing: no branch lies between the rows' arithmetic

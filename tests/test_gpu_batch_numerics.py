@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import quillm_b200 as qb
-from test_gpu_batch_ops import CODE, DT, E, TINY, U, clean, do_attn, gen, lib, plan, pools, rand
+from test_gpu_batch_ops import CODE, DT, E, TINY, U, clean, do_append, do_attn, gen, lib, plan, pools, rand
 
 pytestmark = pytest.mark.gpu
 LOG2E = 1.4426950408889634
@@ -157,3 +157,43 @@ def test_attn_small_weights_beside_a_sink_of_its_own(cuda_dev, hd, dtype):
     clean()
     for b, n in enumerate(lens.tolist()):
         check_prefix(out[b:b + 1], q[b:b + 1], keys, values, slot[b * own:b * own + n], kv, hd, scale, dtype, "f16", SINK_FLOOR)
+
+
+# ------------------------------------------------------------------ rotation
+def same(got, want):
+    """equal values, infinities and NaN in the same places"""
+    assert torch.equal(got.float().nan_to_num(1e30, 2e30, -2e30), want.float().nan_to_num(1e30, 2e30, -2e30))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [3, 1000])
+@pytest.mark.parametrize("hd,rot,layout", [(128, 64, 1), (128, 64, 0), (64, 20, 0), (48, 20, 1), (36, 12, 1), (256, 2, 1), (10, 6, 0)])
+def test_infinities_beside_dimensions_that_stay(cuda_dev, hd, rot, layout, rows, dtype):
+    """dimensions past the rotated ones, and all of them without a plan, come through as they are, whatever stands beside them"""
+    heads, kv, page, g = 16, 8, 16, gen(hd + rot)
+    x = rand(g, (rows, (heads + 2 * kv) * hd), dtype)
+    v3 = x.view(rows, heads + 2 * kv, hd)
+    stay = torch.arange(rot, hd, device="cuda")
+    for i, value in enumerate((math.inf, -math.inf, math.nan)):
+        at = stay[torch.randint(0, hd - rot, (rows, heads + 2 * kv), generator=g, device="cuda")]
+        pick = torch.randint(0, 3, (rows, heads + 2 * kv), generator=g, device="cuda") == i
+        v3.scatter_(2, at[..., None], torch.where(pick[..., None], torch.tensor(value, device="cuda"), v3.gather(2, at[..., None]).float()).to(DT[dtype]))
+    q, k, v = x[:, :heads * hd], x[:, heads * hd:(heads + kv) * hd], x[:, (heads + kv) * hd:]
+    pos = torch.randint(0, 5000, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    qo, ko = torch.zeros(rows, heads * hd, dtype=DT[dtype], device="cuda"), torch.zeros(rows, kv * hd, dtype=DT[dtype], device="cuda")
+    p = plan(hd, rot, layout, 0)
+    qb.check(lib().qmc_qk_norm_rope(p.h, CODE[dtype], q.data_ptr(), x.stride(0), qo.data_ptr(), heads * hd, heads, k.data_ptr(), x.stride(0),
+                                    ko.data_ptr(), kv * hd, kv, None, None, 0.0, pos.data_ptr(), rows, qb.torch_stream()))
+    clean()
+    same(qo.view(rows, heads, hd)[..., rot:], q.reshape(rows, heads, hd)[..., rot:])
+    same(ko.view(rows, kv, hd)[..., rot:], k.reshape(rows, kv, hd)[..., rot:])
+    assert torch.isfinite(qo.view(rows, heads, hd)[..., :rot]).all() and torch.isfinite(ko.view(rows, kv, hd)[..., :rot]).all()
+    n_pages = -(-rows // page)
+    kp, vp, c = pools(g, 1, n_pages, page, kv, hd, dtype, fill=55.0)
+    at = torch.arange(rows, dtype=torch.int32, device="cuda")
+    table = torch.arange(n_pages, dtype=torch.int32, device="cuda").view(1, -1)
+    do_append(None, c, 0, dtype, q, qo, heads, k, v, None, None, torch.zeros_like(at), at, table, rows)
+    clean()
+    same(qo, q)
+    same(kp.view(-1, kv * hd)[:rows], k)
+    same(vp.view(-1, kv * hd)[:rows], v)
