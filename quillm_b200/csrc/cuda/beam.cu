@@ -381,12 +381,28 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
         }
         if (i >= min(a.n_out, a.vocab - c * a.chunk)) return h;
         if (i >= a.chunk) return h;
-        const unsigned long long key = a.cand[((int64_t)(prompt * a.beams + b) * a.chunks + c) * a.n_out + i];
+        const unsigned long long *const keys = a.cand + ((int64_t)(prompt * a.beams + b) * a.chunks + c) * a.n_out;
+        const unsigned long long key = keys[i];
         const float x = order_value((uint32_t)(key >> 32));
         h.at = (uint64_t)b << 32 | (uint32_t)~(uint32_t)key;
-        // with an infinite maximum lse is the log of the number of infinities
-        if (top_s[b] == INFINITY) h.score = x == INFINITY ? cum_s[b] - lse_s[b] : -INFINITY;
-        else h.score = cum_s[b] + ((double)x - lse_s[b]);
+        if (top_s[b] == INFINITY) {
+            // lse is the log of the number of infinities, which come first.  All other tokens score -inf, so their order is the
+            // tokens', not the logits': chunk 0's list goes on with the lowest ones that are not infinite.  The first i of
+            // these end below n_out, as do the infinities that they pass over, all of which are in the list
+            if (x == INFINITY) {
+                h.score = cum_s[b] - lse_s[b];
+            } else if (c == 0) {
+                int infs = 0;
+                while (infs < i && order_value((uint32_t)(keys[infs] >> 32)) == INFINITY) infs++;
+                uint32_t token = (uint32_t)(i - infs);
+                for (int j = 0; j < infs; j++) token += ~(uint32_t)keys[j] <= token;
+                h.at = (uint64_t)b << 32 | token;
+            } else {
+                h.at = ~0ull;
+            }
+        } else {
+            h.score = cum_s[b] + ((double)x - lse_s[b]);
+        }
         if (h.score != h.score) h.score = -INFINITY;
         return h;
     };

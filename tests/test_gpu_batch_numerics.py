@@ -11,7 +11,8 @@ import pytest
 import torch
 
 import quillm_b200 as qb
-from test_gpu_batch_ops import CODE, DT, E, TINY, U, clean, do_append, do_attn, gen, lib, plan, pools, rand
+from test_gpu_batch_ops import (CODE, DT, E, TINY, U, check_select, clean, do_append, do_attn, do_select, f64, gen, lib, plan, pools,
+                                rand, ref_select)
 
 pytestmark = pytest.mark.gpu
 LOG2E = 1.4426950408889634
@@ -197,3 +198,36 @@ def test_infinities_beside_dimensions_that_stay(cuda_dev, hd, rot, layout, rows,
     same(qo, q)
     same(kp.view(-1, kv * hd)[:rows], k)
     same(vp.view(-1, kv * hd)[:rows], v)
+
+
+# ------------------------------------------------------------------ beams
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [5, 100, 4097, 30000])
+def test_beam_select_fills_up_behind_infinities(cuda_dev, vocab, dtype):
+    """in a row that holds +inf every other token scores -inf: where too few are left, the lowest of them follow"""
+    prompts, beams, g = 7, 3, gen(vocab)
+    x = rand(g, (prompts * beams, vocab), dtype, 3.0)
+    scores = -torch.rand(prompts * beams, generator=g, device="cuda")
+    last = vocab - 1
+    x[0:3, min(50, last)] = math.inf                       # one in each beam
+    x[3, 0] = x[3, 1] = x[3, last] = math.inf              # the lowest are infinite themselves
+    x[4], x[5] = -math.inf, math.nan
+    x[6, :] = math.inf                                     # as many as there are tokens
+    x[7:9] = -math.inf
+    x[9, ::2] = math.inf
+    x[10, 1::3], x[10, 2::3] = math.nan, -math.inf
+    x[10, last] = math.inf
+    x[11] = x[10]
+    scores[12] = -math.inf                                 # a dead beam below one that holds infinities
+    x[13, 3] = x[14, 2] = math.inf
+    finished = torch.zeros(prompts * beams, dtype=torch.uint8, device="cuda")
+    finished[15] = 1                                       # and a finished one
+    x[16, 1] = math.inf
+    scores[17] = math.nan
+    x[18, last] = math.inf                                 # beside rows of finite logits there are enough
+    for n_out in (1, 3, 6, 15, 64):
+        if n_out > beams * vocab:
+            continue
+        got = do_select(dtype, x, vocab, prompts, beams, scores, finished, 2, n_out)
+        clean()
+        check_select(got, ref_select(f64(x), f64(scores), finished.cpu().numpy(), 2, n_out, prompts, beams))
