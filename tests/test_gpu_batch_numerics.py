@@ -231,3 +231,41 @@ def test_beam_select_fills_up_behind_infinities(cuda_dev, vocab, dtype):
         got = do_select(dtype, x, vocab, prompts, beams, scores, finished, 2, n_out)
         clean()
         check_select(got, ref_select(f64(x), f64(scores), finished.cpu().numpy(), 2, n_out, prompts, beams))
+
+
+# ------------------------------------------------------------------ many tiles a block
+@pytest.mark.parametrize("name", list(MANY))
+def test_attn_many_tiles_a_block(cuda_dev, name):
+    """rings of tiles used again and again, both streams of a block, maxima that creep up and fall, a last tile that is cut"""
+    dtype, cdt, n_seq, group, hd, page, tile = MANY[name]
+    for std, prefix in ((1.0, 1536), (3.0, 1536), (1.0, 1984 + page)):
+        kv, g = 148, gen(int(10 * std) + prefix)
+        prefix = prefix // page * page
+        keys, values, c, pp, slot = shared(g, kv, hd, prefix, page, cdt, std)
+        # scores that rise, fall and rise again along the prefix
+        keys[slot] *= (1.0 + 0.8 * torch.sin(torch.arange(prefix, device="cuda") / 200)).to(DT[cdt])[:, None, None]
+        q = rand(g, (n_seq, kv * group * hd), dtype)
+        assert -(-prefix // tile) // ranges(c, dtype, n_seq, kv * group, hd, prefix, page) >= 4
+        scale = 1.0 / math.sqrt(hd)
+        out = over_prefix(c, dtype, q, kv * group, hd, scale, pp, prefix, page)
+        check_prefix(out, q, keys, values, slot, kv, hd, scale, dtype, cdt, SINK_FLOOR if cdt == "f16" else 0.0)
+
+
+@pytest.mark.parametrize("dtype,cdt", [("f16", "f16"), ("bf16", "bf16")])
+def test_attn_repeats_its_bits(cuda_dev, dtype, cdt):
+    """prefix and own positions beside each other, in several tiles each: the same bits from call to call"""
+    n_seq, heads, kv, hd, page, prefix, own = 16, 64, 8, 128, 16, 8192, 512
+    g = gen(3)
+    width = (prefix + own) // page
+    n_pages = prefix // page + n_seq * (own // page)
+    kp, vp, c = pools(g, 1, n_pages, page, kv, hd, cdt)
+    pages = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32)
+    pp = pages[:prefix // page].clone()
+    table = torch.cat([pp.expand(n_seq, -1), pages[prefix // page:].view(n_seq, -1)], 1).contiguous()
+    lens = (prefix + torch.randint(1, own + 1, (n_seq,), generator=g, device="cuda")).to(torch.int32)
+    q = rand(g, (n_seq, heads * hd), dtype)
+    outs = [torch.zeros_like(q) for _ in range(20)]
+    for o in outs:
+        do_attn(c, 0, dtype, q, o, heads, 0.09, pp, prefix, table, lens)
+    clean()
+    assert all(torch.equal(o.view(torch.int16), outs[0].view(torch.int16)) for o in outs)
