@@ -390,6 +390,7 @@ int qmc_attn_prefix_workspace(int dtype, const qmc_paged_cache *cache, int32_t n
     if (!bytes) return set_error(QMC_EINVAL, "attn_prefix_workspace: null argument");
     *bytes = 0;
     if (const int rc = check_attn("attn_prefix_workspace", dtype, cache, n_seq, n_heads, prefix_len, ld_table)) return rc;
+    if (n_seq == 0) return QMC_OK;  // nothing to plan
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;
     *bytes = (size_t)plan_for(cache, dtype, n_seq, n_heads, prefix_len, ld_table, c->num_sms).bytes;

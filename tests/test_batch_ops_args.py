@@ -177,3 +177,10 @@ def test_sizes_counted_in_32_bits_are_bounded():
 def test_beam_reorder_refuses_pages_of_too_many_pieces():
     c = cache(n_layers=1 << 20, n_pages=1, page_size=1 << 20, n_kv_heads=1, head_dim=256)
     refused(reorder(c, beams=64, ldp=64), "too many")
+
+
+def test_attn_workspace_of_no_sequences():
+    c, n = cache(), C.c_size_t(7)
+    for prefix in (0, 9, 16):
+        assert qb.cuda().qmc_attn_prefix_workspace(1, C.addressof(c), 0, 4, prefix, 4, C.byref(n)) == 0
+        assert n.value == 0
