@@ -250,7 +250,7 @@ enum {
 typedef struct {
     int32_t head_dim, rot_dim; /* even; 2 <= rot_dim <= head_dim <= 256 */
     int32_t layout, scaling;
-    double theta, factor; /* > 0 (YARN: theta != 1); factor is read by the three scaled forms */
+    double theta, factor; /* > 0 (YARN: theta != 1), and every f_i finite; factor is read by the three scaled forms */
     double low, high;     /* BANDS: 0 < low < high; YARN: turns 0 < low <= high */
     int32_t orig_ctx;     /* BANDS, YARN: > 0 */
 } qmc_rope_config;

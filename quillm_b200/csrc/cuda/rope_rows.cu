@@ -352,7 +352,11 @@ int qmc_rope_plan_create(const qmc_rope_config *c, qmc_rope_plan **out) {
             const double r = fmin(fmax((i - lo) / fmax(hi - lo, 0.001), 0.0), 1.0);
             f = f / c->factor * r + f * (1.0 - r);
         }
-        double turns = f / two_pi;  // f < 2^1023: the whole turns go, the rest is exact
+        if (!std::isfinite(f)) {
+            delete p;
+            return set_error(QMC_EINVAL, "rope_plan_create: frequency %d of theta %g, factor %g is not finite", i, c->theta, c->factor);
+        }
+        double turns = f / two_pi;  // the whole turns go, the rest is exact
         turns -= floor(turns);
         // two halves of 32 bits: a double holds 53 bits of the fraction, none is lost
         const double hi = floor(turns * 4294967296.0);

@@ -184,3 +184,13 @@ def test_attn_workspace_of_no_sequences():
     for prefix in (0, 9, 16):
         assert qb.cuda().qmc_attn_prefix_workspace(1, C.addressof(c), 0, 4, prefix, 4, C.byref(n)) == 0
         assert n.value == 0
+
+
+@pytest.mark.parametrize("bad", [dict(theta=5e-324), dict(scaling=1, factor=1e-320), dict(scaling=2, factor=1e-320), dict(scaling=3, factor=1e-320)])
+def test_rope_plan_refuses_frequencies_past_the_largest_number(bad):
+    d = dict(head_dim=128, rot_dim=128, layout=0, scaling=0, theta=1e4, factor=2.0, low=1.0, high=4.0, orig_ctx=4096)
+    d.update(bad)
+    cfg = qb.QmcRopeConfig(*(d[f[0]] for f in qb.QmcRopeConfig._fields_))
+    h = C.c_void_p(1)
+    refused(qb.cuda().qmc_rope_plan_create(C.byref(cfg), C.byref(h)), "frequency")
+    assert not h.value
