@@ -245,7 +245,7 @@ enum {
                             s = (t - low) / (high - low) */
     QMC_ROPE_YARN = 3,   /* f_i / factor r + f_i (1 - r) with r rising from 0 to 1 between the pair indices
                             floor(d(high)) and ceil(d(low)), d(t) = rot_dim ln(orig_ctx / (2 pi t)) / (2 ln theta),
-                            clamped to [0, rot_dim - 1]; cos and sin times 0.1 ln(factor) + 1 */
+                            clamped to [0, rot_dim - 1]; cos and sin times 0.1 ln(factor) + 1, for factors up to 1 as they are */
 };
 typedef struct {
     int32_t head_dim, rot_dim; /* even; 2 <= rot_dim <= head_dim <= 256 */

@@ -338,7 +338,7 @@ int qmc_rope_plan_create(const qmc_rope_config *c, qmc_rope_plan **out) {
         auto d = [&](double turns) { return rot * log(c->orig_ctx / (two_pi * turns)) / (2.0 * log(c->theta)); };
         lo = fmin(fmax(floor(d(c->high)), 0.0), rot - 1.0);
         hi = fmin(fmax(ceil(d(c->low)), 0.0), rot - 1.0);
-        p->mscale = (float)(0.1 * log(c->factor) + 1.0);
+        if (c->factor > 1.0) p->mscale = (float)(0.1 * log(c->factor) + 1.0);
     }
     for (int i = 0; i < rot / 2; i++) {
         double f = pow(c->theta, -2.0 * i / rot);

@@ -200,6 +200,21 @@ def test_infinities_beside_dimensions_that_stay(cuda_dev, hd, rot, layout, rows,
     same(vp.view(-1, kv * hd)[:rows], v)
 
 
+@pytest.mark.parametrize("factor", [1e-6, 0.5, 1.0, 1.5, 40.0])
+def test_yarn_scales_only_longer_contexts(cuda_dev, factor):
+    """the factor on cos and sin is 1 for factors up to 1: a turn then keeps the length of every pair"""
+    rows, heads, hd, g = 50, 4, 64, gen(2)
+    q = rand(g, (rows, heads * hd), "f32")
+    out, pos = torch.zeros_like(q), torch.arange(rows, dtype=torch.int32, device="cuda") * 97
+    p = qb.RopePlan(hd, hd, qb.QMC_ROPE_HALF, 10000.0, qb.QMC_ROPE_YARN, factor, 1.0, 32.0, 4096)
+    qb.check(lib().qmc_qk_norm_rope(p.h, 0, q.data_ptr(), heads * hd, out.data_ptr(), heads * hd, heads, None, 0, None, 0, 0, None, None, 0.0,
+                                    pos.data_ptr(), rows, qb.torch_stream()))
+    clean()
+    by = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    a, b = (t.view(rows, heads, 2, hd // 2).double().square().sum(2).sqrt() for t in (q, out))
+    assert ((b - by * a).abs() <= 2.0**-18 * by * a).all()  # two elements, each off by 2^-19 m (|a| + |b|), up to sqrt(2) of the length
+
+
 # ------------------------------------------------------------------ beams
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("vocab", [5, 100, 4097, 30000])
