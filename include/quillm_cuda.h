@@ -223,7 +223,8 @@ int qmc_model_forward_sample(qmc_model *m, int32_t token, int32_t pos, qmc_sampl
  * and rotated, appended to pages, each sequence's token attends to the shared prefix and to its own pages, and
  * beams are selected and their pages reordered.
  *
- * Common to all of them: pointers are device memory of the current device unless said otherwise; rows are
+ * Common to all of them: pointers are device memory of the current device unless said otherwise, aligned to their
+ * elements (a workspace: anyhow); rows are
  * `ld` elements apart (ld >= the row's elements) and a row's heads follow one another; `dtype` is the rows'
  * QMC_F32, QMC_F16 or QMC_BF16; sums, softmax statistics and norms are float (log-sum-exp of a vocabulary:
  * double) and every output is rounded once.  No call allocates or synchronises and each may be captured in a

@@ -413,6 +413,7 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
         return set_error(QMC_EINVAL, "%s: null argument", op);
     if ((uintptr_t)q % dtype_size(dtype) || (uintptr_t)out % dtype_size(dtype))
         return set_error(QMC_EINVAL, "%s: misaligned q or out", op);
+    if (misaligned({prefix_len ? prefix_pages : nullptr, page_table, seq_lens})) return set_error(QMC_EINVAL, "%s: misaligned pages or lengths", op);
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;
     const Plan p = plan_for(cache, dtype, n_seq, n_heads, prefix_len, ld_table, c->num_sms);

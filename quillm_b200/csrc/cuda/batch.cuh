@@ -4,6 +4,8 @@
 
 #include <cuda_bf16.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace qmc {
@@ -79,6 +81,12 @@ __device__ __forceinline__ void store_chunk(T *p, const float (&v)[C]) {
 
 inline bool is_row_dtype(int d) { return d == QMC_F32 || d == QMC_F16 || d == QMC_BF16; }
 inline int dtype_size(int d) { return d == QMC_F32 ? 4 : 2; }
+// arrays of 4-byte elements
+inline bool misaligned(std::initializer_list<const void *> arrays) {
+    for (const void *p : arrays)
+        if ((uintptr_t)p % 4) return true;
+    return false;
+}
 // the caller's cache: QMC_OK, or QMC_EINVAL with `op` in the message
 int check_cache(const qmc_paged_cache *c, const char *op);
 // elements of one layer of a pool

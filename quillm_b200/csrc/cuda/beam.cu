@@ -634,6 +634,7 @@ int qmc_beam_select(int dtype, const void *logits, int64_t ld, int32_t n_prompts
     if (!logits || !scores || !parents || !tokens || !out_scores || !workspace)
         return set_error(QMC_EINVAL, "%s: null argument", op);
     if ((uintptr_t)logits % dtype_size(dtype)) return set_error(QMC_EINVAL, "%s: misaligned logits", op);
+    if (misaligned({scores, parents, tokens, out_scores})) return set_error(QMC_EINVAL, "%s: misaligned scores, parents or tokens", op);
     size_t need = 0;
     qmc_beam_workspace(n_prompts, beams, n_vocab, n_out, &need);
     if (workspace_bytes < need) return set_error(QMC_EINVAL, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
@@ -673,6 +674,8 @@ int qmc_beam_reorder(const qmc_paged_cache *cache, int32_t n_prompts, int32_t be
     if (most > INT32_MAX) return set_error(QMC_EINVAL, "%s: %d beams of %d layers of such pages are too many", op, beams, cache->n_layers);
     if (n_prompts == 0) return QMC_OK;
     if (!parents || !seq_lens || !page_table || !page_table_out) return set_error(QMC_EINVAL, "%s: null argument", op);
+    if (misaligned({parents, seq_lens, page_table, page_table_out}))
+        return set_error(QMC_EINVAL, "%s: misaligned parents, lengths or page table", op);
     if (page_table == page_table_out) return set_error(QMC_EINVAL, "%s: the table cannot be reordered in place", op);
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;

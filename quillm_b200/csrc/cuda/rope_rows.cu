@@ -389,6 +389,7 @@ int qmc_qk_norm_rope(const qmc_rope_plan *plan, int dtype, const void *q, int64_
     if (n_kv_heads && ((rc = check_rows(op, "k", k, ldk, n_kv_heads, hd, dtype)) || (rc = check_rows(op, "k_out", k_out, ldko, n_kv_heads, hd, dtype))))
         return rc;
     if (!positions) return set_error(QMC_EINVAL, "%s: null positions", op);
+    if (misaligned({positions, q_weight, k_weight})) return set_error(QMC_EINVAL, "%s: misaligned positions or weights", op);
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;
     RowsArgs a{};
@@ -422,6 +423,8 @@ int qmc_kv_append_paged(const qmc_rope_plan *plan, const qmc_paged_cache *cache,
         return rc;
     if ((rc = check_rows(op, "k", k, ldk, kv, hd, dtype)) || (rc = check_rows(op, "v", v, ldv, kv, hd, dtype))) return rc;
     if (!positions || !page_table) return set_error(QMC_EINVAL, "%s: null positions or page table", op);
+    if (misaligned({seq, positions, page_table, q_weight, k_weight}))
+        return set_error(QMC_EINVAL, "%s: misaligned sequences, positions, page table or weights", op);
     if (!seq && rows > n_seq) return set_error(QMC_EINVAL, "%s: %lld rows for %d sequences", op, (long long)rows, n_seq);
     DevCtx *c = ctx();
     if (!c) return QMC_ECUDA;

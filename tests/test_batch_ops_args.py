@@ -194,3 +194,28 @@ def test_rope_plan_refuses_frequencies_past_the_largest_number(bad):
     h = C.c_void_p(1)
     refused(qb.cuda().qmc_rope_plan_create(C.byref(cfg), C.byref(h)), "frequency")
     assert not h.value
+
+
+@pytest.mark.parametrize("name", ["pos", "qw", "kw"])
+def test_qk_norm_rope_refuses_misaligned(name):
+    refused(qk(qb.RopePlan(128).h, **{name: A + 2}), "misaligned")
+
+
+@pytest.mark.parametrize("name", ["pos", "seq", "table", "qw", "kw"])
+def test_append_refuses_misaligned(name):
+    refused(append(None, cache(), **{name: A + 2}), "misaligned")
+
+
+@pytest.mark.parametrize("name", ["pages", "table", "lens"])
+def test_attn_refuses_misaligned(name):
+    refused(attn(cache(), **{name: A + 1}), "misaligned")
+
+
+@pytest.mark.parametrize("name", ["scores", "parents", "tokens", "out"])
+def test_beam_select_refuses_misaligned(name):
+    refused(select(**{name: A + 2}), "misaligned")
+
+
+@pytest.mark.parametrize("name", ["parents", "lens", "table", "out"])
+def test_beam_reorder_refuses_misaligned(name):
+    refused(reorder(cache(), **{name: A + 65}), "misaligned")
