@@ -296,7 +296,7 @@ int qmc_kv_append_paged(const qmc_rope_plan *plan, const qmc_paged_cache *cache,
  * entries for whole prefix pages are not read; prefix_len may end inside a page).  seq_lens[b] counts
  * the prefix too: it is 0 (an empty row: zeros) or at least prefix_len; any other value, a length past
  * ld_table * page_size, or a page outside the pool sets the error word, and then the rows concerned are undefined (but
- * written).  scale is finite and not negative; n_heads is a multiple of the cache's n_kv_heads (head h reads kv
+ * written).  scale is not negative, and scale log2(e) and the scaled scores are finite floats; n_heads is a multiple of the cache's n_kv_heads (head h reads kv
  * head h / (n_heads / n_kv_heads)), head_dim <= 256, ld_table * page_size < 2^31 - 1024.  Types (rows, cache): (F32, F32), (F32, F16), (F16, F16), (BF16, BF16).  Keys and values
  * at positions that are read must be finite; what lies in slots past a sequence's end does not matter. */
 int qmc_attn_prefix_workspace(int dtype, const qmc_paged_cache *cache, int32_t n_seq, int32_t n_heads,

@@ -407,7 +407,8 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
     const int64_t n = (int64_t)n_heads * cache->head_dim;
     if (ldq < n || ldo < n || ldq > (int64_t)1 << 40 || ldo > (int64_t)1 << 40)
         return set_error(QMC_EINVAL, "%s: rows of %lld elements are %lld and %lld apart", op, (long long)n, (long long)ldq, (long long)ldo);
-    if (!(scale >= 0.0f) || scale - scale != 0.0f) return set_error(QMC_EINVAL, "%s: scale %g", op, scale);
+    const float scale2 = scale * 1.4426950408889634f;  // scores as exponents of two
+    if (!(scale >= 0.0f) || scale2 - scale2 != 0.0f) return set_error(QMC_EINVAL, "%s: scale %g", op, scale);
     if (n_seq == 0) return QMC_OK;
     if (!q || !out || !page_table || !seq_lens || !workspace || (prefix_len && !prefix_pages))
         return set_error(QMC_EINVAL, "%s: null argument", op);
@@ -429,7 +430,7 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
     a.n_seq = n_seq, a.heads = n_heads, a.kv = cache->n_kv_heads, a.group = n_heads / cache->n_kv_heads;
     a.hd = cache->head_dim, a.page_size = cache->page_size, a.n_pages = cache->n_pages, a.ld_table = ld_table;
     a.prefix = prefix_len, a.rows = p.rows, a.ptiles = p.ptiles, a.psplit = p.psplit, a.gtiles = p.gtiles, a.osplit = p.osplit, a.pparts = p.pparts;
-    a.scale = scale * 1.4426950408889634f;
+    a.scale = scale2;
     cudaStream_t s = pick_stream(stream);
     const int cdt = cache->dtype;
     if (dtype == QMC_F32 && cdt == QMC_F32) return launch_attn<float, float>(a, p, dtype, cdt, c->num_sms, s);

@@ -219,3 +219,7 @@ def test_beam_select_refuses_misaligned(name):
 @pytest.mark.parametrize("name", ["parents", "lens", "table", "out"])
 def test_beam_reorder_refuses_misaligned(name):
     refused(reorder(cache(), **{name: A + 65}), "misaligned")
+
+
+def test_attn_refuses_a_scale_past_the_largest_exponent():
+    refused(attn(cache(), scale=3e38), "scale")  # as an exponent of two, times log2(e), it is infinite
