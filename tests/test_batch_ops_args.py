@@ -198,7 +198,8 @@ def test_rope_plan_refuses_frequencies_past_the_largest_number(bad):
 
 @pytest.mark.parametrize("name", ["pos", "qw", "kw"])
 def test_qk_norm_rope_refuses_misaligned(name):
-    refused(qk(qb.RopePlan(128).h, **{name: A + 2}), "misaligned")
+    p = qb.RopePlan(128)
+    refused(qk(p.h, **{name: A + 2}), "misaligned")
 
 
 @pytest.mark.parametrize("name", ["pos", "seq", "table", "qw", "kw"])
