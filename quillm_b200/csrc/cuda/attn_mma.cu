@@ -358,7 +358,7 @@ int launch_t(const AttnArgs &a, bool after, cudaStream_t s) {
     auto fn = attn_mma_kernel<T, CT, HDP, WM>;
     constexpr int smem = smem_bytes<HDP, 16 * WM, sizeof(T) == 4>();
     static_assert(4 * 16 * HDP * 4 <= stages<HDP>() * stage_bytes<HDP>(), "the join fits the ring");
-    static bool done[64];
+    static std::atomic<bool> done[64];
     if (const int rc = raise_smem(fn, smem, done)) return rc;
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit + (int64_t)a.n_seq * a.kv * a.gtiles * a.osplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");

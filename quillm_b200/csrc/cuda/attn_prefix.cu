@@ -321,7 +321,7 @@ int launch_rows(const AttnArgs &a, int64_t jobs, bool vec, cudaStream_t s) {
     const int hd4 = (a.hd + 3) & ~3;
     auto fn = attn_rows_kernel<T, CT, NG>;
     const int smem = (2 * kPT + kQR) * hd4 * 4;
-    static bool done[64];
+    static std::atomic<bool> done[64];
     if (const int rc = raise_smem(fn, (2 * kPT + kQR) * 256 * 4, done)) return rc;
     fn<<<(unsigned)jobs, 128, smem, s>>>(a, vec);
     QMC_LAUNCH_CHECK();

@@ -1,6 +1,8 @@
 // Work of the shared-prefix attention (attn_prefix.cu), for its kernels: the jobs of a launch and where their parts go.
 #pragma once
 
+#include <atomic>
+
 #include "batch.cuh"
 
 namespace qmc {
@@ -93,9 +95,9 @@ struct Window {
     }
 };
 
-// the kernel's dynamic shared memory limit, raised once per device
+// the kernel's dynamic shared memory limit, raised once per device (twice where two threads make the first call)
 template <typename F>
-int raise_smem(F fn, int bytes, bool (&done)[64]) {
+int raise_smem(F fn, int bytes, std::atomic<bool> (&done)[64]) {
     int dev = 0;
     QMC_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return set_error(QMC_EINVAL, "attn_prefix: device %d out of range", dev);

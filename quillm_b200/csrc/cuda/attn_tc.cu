@@ -598,7 +598,7 @@ int launch_t(const AttnArgs &a, const CUtensorMap &kmap, const CUtensorMap &vmap
     auto fn = attn_tc_kernel<CT, HDP, PAIR>;
     constexpr int smem = smem_bytes<HDP, PAIR>();
     static_assert(smem + sizeof(Shared) <= 232448, "shared memory of a block");
-    static bool done[64];
+    static std::atomic<bool> done[64];
     if (const int rc = raise_smem(fn, smem, done)) return rc;
     const int64_t jobs = (int64_t)a.kv * a.ptiles * a.psplit;
     if (jobs > INT32_MAX) return set_error(QMC_EINVAL, "attn_prefix: too many blocks");
