@@ -231,19 +231,21 @@ __device__ __forceinline__ void mma_job(const AttnArgs &a, const Job &jb, uint8_
                 s[n][i] = 8 * n + 2 * (lane & 3) + (i & 1) < left ? s[n][i] * qs[i >> 1] : -INFINITY;
                 mx[i >> 1] = fmaxf(mx[i >> 1], s[n][i]);
             }
-        float ref[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-            const float to = W::moved(m[i], mx[i], high[i]);
-            ref[i] = to == -INFINITY ? 0.0f : to;
-            const float corr = ex2(m[i] - ref[i]);
-            m[i] = to;
-            l[i] *= corr;
-#pragma unroll
-            for (int d = 0; d < HDP / 8; d++) o[d][2 * i] *= corr, o[d][2 * i + 1] *= corr;
         }
+        if (__any_sync(0xffffffffu, W::left_by(m[0], mx[0]) || W::left_by(m[1], mx[1]))) {  // the first time, and rarely again
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float to = W::moved(m[i], mx[i], high[i]), by = to == -INFINITY ? 1.0f : ex2(m[i] - to);
+                m[i] = to, l[i] *= by;
+#pragma unroll
+                for (int d = 0; d < HDP / 8; d++) o[d][2 * i] *= by, o[d][2 * i + 1] *= by;
+            }
+        }
+        const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll

@@ -82,6 +82,9 @@ template <typename CT>
 struct Window {
     static constexpr bool kHalf = __is_same(CT, __half);
     static constexpr float kTop = kHalf ? 10.0f : 0.0f, kLift = kHalf ? 15.5f : 8.0f, kDrop = -2.0f, kFar = 48.0f;
+    __device__ static __forceinline__ bool left_by(float m, float top) {
+        return top > m + kLift || (kHalf && top > -INFINITY && top < m + kDrop);
+    }
     // the reference after a tile whose largest score is `top` (-inf: it has none); hi: the highest so far, kept for fp16.  At first
     // both are -inf
     __device__ static __forceinline__ float moved(float m, float top, float &hi, float lift = kLift) {
