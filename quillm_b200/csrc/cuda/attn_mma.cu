@@ -342,14 +342,14 @@ __device__ __forceinline__ void mma_job(const AttnArgs &a, const Job &jb, uint8_
     }
 }
 
-// WM: 16-row groups of a prefix job's tile; own jobs have one
+// WM: 16-row groups of a prefix job's tile; own jobs, which come here with heads above 128 alone, have one
 template <typename T, typename CT, int HDP, int WM>
-__global__ void __launch_bounds__(128) attn_mma_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(128, 2) attn_mma_kernel(const AttnArgs a) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ Scratch sc;
     const Job jb = job_of(a, blockIdx.x, 16 * WM, 16, kTP);
     pdl_launch_dependents();
-    if (WM > 1 && jb.b < 0) mma_job<T, CT, HDP, WM>(a, jb, sm, sc);
+    if (HDP <= 128 || (WM > 1 && jb.b < 0)) mma_job<T, CT, HDP, WM>(a, jb, sm, sc);
     else mma_job<T, CT, HDP, 1>(a, jb, sm, sc);
     // launched beside the prefix's kernel, this grid ends after it, which the join relies on: one block waits, the others make room
     if (blockIdx.x == 0) pdl_wait();
@@ -368,11 +368,10 @@ int launch_t(const AttnArgs &a, bool after, cudaStream_t s) {
 }
 template <typename T, typename CT, int HDP>
 int launch_m(const AttnArgs &a, bool after, cudaStream_t s) {
-    switch (attn_mma_tile(a.rows)) {
-        case 16: return launch_t<T, CT, HDP, 1>(a, after, s);
-        case 32: return launch_t<T, CT, HDP, 2>(a, after, s);
-        default: return launch_t<T, CT, HDP, 4>(a, after, s);
-    }
+    const int tile = attn_mma_tile(a.rows);
+    if constexpr (HDP > 128)  // narrower heads of so few rows go to attn_warp
+        if (tile == 16) return launch_t<T, CT, HDP, 1>(a, after, s);
+    return tile == 32 ? launch_t<T, CT, HDP, 2>(a, after, s) : launch_t<T, CT, HDP, 4>(a, after, s);
 }
 template <typename T, typename CT>
 int launch_h(const AttnArgs &a, bool after, cudaStream_t s) {

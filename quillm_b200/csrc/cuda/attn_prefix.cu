@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
             float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (slot_s[pp] >= 0) {
                 const CT *p = kc + (slot_s[pp] * a.kv + jb.h) * hd + 4 * c;
-                if (vec) load_chunk<CT, 4>(p, v);
+                if (sizeof(CT) == 2 && vec) load_chunk<CT, 4>(p, v);  // aligned floats have a kernel of their own
                 else
                     for (int k = 0; k < 4; k++) v[k] = 4 * c + k < hd ? to_f32(p[k]) : 0.0f;
             }
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool v
             float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (slot_s[pp] >= 0) {
                 const CT *p = vc + (slot_s[pp] * a.kv + jb.h) * hd + 4 * c;
-                if (vec) load_chunk<CT, 4>(p, v);
+                if (sizeof(CT) == 2 && vec) load_chunk<CT, 4>(p, v);
                 else
                     for (int k = 0; k < 4; k++) v[k] = 4 * c + k < hd ? to_f32(p[k]) : 0.0f;
             }
