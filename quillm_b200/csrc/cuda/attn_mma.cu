@@ -26,11 +26,6 @@ __host__ __device__ constexpr int stages() {
     return HDP == 256 ? 2 : 3;
 }
 
-__device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22; below 2^-126 it is 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -42,27 +37,6 @@ __device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t a) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(a)
                  : "memory");
-}
-__device__ __forceinline__ void mma16(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// two floats as a pair of 16-bit elements, the first in the low half; lo: what the rounding left over
-__device__ __forceinline__ uint32_t pack2(__half, float x, float y, float *lx = nullptr, float *ly = nullptr) {
-    const __half2 h = __floats2half2_rn(x, y);
-    if (lx) *lx = x - __low2float(h), *ly = y - __high2float(h);
-    return *(const uint32_t *)&h;
-}
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y, float *lx = nullptr, float *ly = nullptr) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    if (lx) *lx = x - __low2float(h), *ly = y - __high2float(h);
-    return *(const uint32_t *)&h;
 }
 // 16 bytes from global to shared memory, or zeros
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
@@ -258,9 +232,9 @@ __device__ __forceinline__ void mma_job(const AttnArgs &a, const Job &jb, uint8_
             uint32_t p[4], pl[4];
             if constexpr (SPLIT) {
                 float r[8];
-                p[0] = pack2(CT(), s[n][0], s[n][1], &r[0], &r[1]), p[1] = pack2(CT(), s[n][2], s[n][3], &r[2], &r[3]);
-                p[2] = pack2(CT(), s[n + 1][0], s[n + 1][1], &r[4], &r[5]);
-                p[3] = pack2(CT(), s[n + 1][2], s[n + 1][3], &r[6], &r[7]);
+                p[0] = pack2(CT(), s[n][0], s[n][1], &r[0]), p[1] = pack2(CT(), s[n][2], s[n][3], &r[2]);
+                p[2] = pack2(CT(), s[n + 1][0], s[n + 1][1], &r[4]);
+                p[3] = pack2(CT(), s[n + 1][2], s[n + 1][3], &r[6]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) pl[i] = pack2(CT(), r[2 * i], r[2 * i + 1]);
             } else {

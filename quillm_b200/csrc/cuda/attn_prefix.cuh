@@ -98,6 +98,28 @@ struct Window {
     }
 };
 
+__device__ __forceinline__ void mma16(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two floats as a pair of 16-bit elements, the first in the low half; lo: what the rounding left over
+__device__ __forceinline__ uint32_t pack2(__half, float x, float y, float *lo = nullptr) {
+    const __half2 h = __floats2half2_rn(x, y);
+    if (lo) lo[0] = x - __low2float(h), lo[1] = y - __high2float(h);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y, float *lo = nullptr) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    if (lo) lo[0] = x - __low2float(h), lo[1] = y - __high2float(h);
+    return *(const uint32_t *)&h;
+}
+
 // the kernel's dynamic shared memory limit, raised once per device (twice where two threads make the first call)
 template <typename F>
 int raise_smem(F fn, int bytes, std::atomic<bool> (&done)[64]) {

@@ -57,19 +57,6 @@ __host__ __device__ constexpr int smem_bytes() {
     return 1024 + ((PAIR ? 2 : 1) + ring<HDP, PAIR>()) * tile_bytes<HDP>();
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack2(__half, float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *(const uint32_t *)&h;
-}
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *(const uint32_t *)&h;
-}
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),

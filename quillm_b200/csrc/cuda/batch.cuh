@@ -79,6 +79,12 @@ __device__ __forceinline__ void store_chunk(T *p, const float (&v)[C]) {
     *(Chunk<T, C> *)p = c;
 }
 
+__device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22; below 2^-126 it is 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 inline bool is_row_dtype(int d) { return d == QMC_F32 || d == QMC_F16 || d == QMC_BF16; }
 inline int dtype_size(int d) { return d == QMC_F32 ? 4 : 2; }
 // arrays of 4-byte elements

@@ -57,11 +57,6 @@ __device__ __forceinline__ float order_value(uint32_t u) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-__device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22; below 2^-126 it is 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // by one warp: the largest T that at least n of the 256 values reach (their n-th largest, or a value above it that exactly n
 // reach), at least 1
 __device__ __forceinline__ uint32_t nth_largest(const uint32_t *vals, int lane, int n) {
