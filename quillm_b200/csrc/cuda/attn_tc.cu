@@ -156,25 +156,17 @@ __device__ __forceinline__ float fma_sat(float x, float y, float c) {
 // 2^t of a pair without the special-function unit.  t comes as x = (t + 112) / 128, held in [0, 1] by the instruction that forms it: below
 // 2^-112 a weight counts for nothing, and 2^16 is above what a tile's sum may reach, so that the reference moves (beyond 127 the
 // exponent would run into the sign).  x is off by 2^-25, the result by 2^-18.5 of itself.  n = t rounded to an integer (as the low
-// bits of t + 1.5 * 2^23), 2^(t - n) by the minimax polynomial of the relative error on [-1/2, 1/2] (degree 3: 2^-13.7, under a bf16
-// step's 1/50; degree 4: 2^-18.5, for fp16), n added to its exponent
+// bits of t + 1.5 * 2^23), 2^(t - n) by the minimax polynomial of the relative error on [-1/2, 1/2] (degree 4: 2^-18.5; one of degree 3,
+// 2^-13.7, would do for bf16 weights but not for their float sum), n added to its exponent
 constexpr float kSpan = 128.0f, kBelow = 112.0f;
-template <bool BF>
 __device__ __forceinline__ void ex2_pair(uint64_t x, float &p0, float &p1) {
     const float kRnd = 12582912.0f;
     const uint64_t span = pair_of(kSpan, kSpan), rnd = pair_of(kRnd - kBelow, kRnd - kBelow);
     const uint64_t up = fma2(x, span, rnd), f = fma2(x, span, fma2(up, pair_of(-1.0f, -1.0f), rnd));
-    uint64_t v;
-    if (BF) {
-        v = fma2(f, pair_of(0.05517166852951f, 0.05517166852951f), pair_of(0.24261112511158f, 0.24261112511158f));
-        v = fma2(f, v, pair_of(0.69326096773148f, 0.69326096773148f));
-        v = fma2(f, v, pair_of(0.99992805719376f, 0.99992805719376f));
-    } else {
-        v = fma2(f, pair_of(0.00957010220736f, 0.00957010220736f), pair_of(0.05591785907745f, 0.05591785907745f));
-        v = fma2(f, v, pair_of(0.24024744331837f, 0.24024744331837f));
-        v = fma2(f, v, pair_of(0.69312179088593f, 0.69312179088593f));
-        v = fma2(f, v, pair_of(0.99999928474426f, 0.99999928474426f));
-    }
+    uint64_t v = fma2(f, pair_of(0.00957010220736f, 0.00957010220736f), pair_of(0.05591785907745f, 0.05591785907745f));
+    v = fma2(f, v, pair_of(0.24024744331837f, 0.24024744331837f));
+    v = fma2(f, v, pair_of(0.69312179088593f, 0.69312179088593f));
+    v = fma2(f, v, pair_of(0.99999928474426f, 0.99999928474426f));
     float u0, u1, v0, v1;
     of_pair(up, u0, u1);
     of_pair(v, v0, v1);
@@ -186,7 +178,6 @@ __device__ __forceinline__ void ex2_pair(uint64_t x, float &p0, float &p1) {
 // pipe instead.  MASK: only the first `left` positions exist
 template <typename CT, bool MASK>
 __device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *pk, float scale, float m, int left, float &most) {
-    constexpr bool BF = __is_same(CT, __nv_bfloat16);
     const uint64_t sc = pair_of(scale, scale), mm = pair_of(-m, -m);
     const float part = scale * (1.0f / kSpan), from = (kBelow - m) * (1.0f / kSpan);
     const uint32_t live = MASK ? live_bits(left, 0) : 0xffffffffu;
@@ -196,7 +187,7 @@ __device__ __forceinline__ float row_weights(const uint32_t (&x)[32], uint32_t *
         const float s0 = __uint_as_float(x[k]), s1 = __uint_as_float(x[k + 1]);
         float p0, p1;
         if (!MASK && (k >> 1) % 8 % 3 == 1) {
-            ex2_pair<BF>(pair_of(fma_sat(s0, part, from), fma_sat(s1, part, from)), p0, p1);
+            ex2_pair(pair_of(fma_sat(s0, part, from), fma_sat(s1, part, from)), p0, p1);
         } else {
             float t0, t1;
             of_pair(fma2(pair_of(s0, s1), sc, mm), t0, t1);
