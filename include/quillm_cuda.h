@@ -224,19 +224,19 @@ int qmc_model_forward_sample(qmc_model *m, int32_t token, int32_t pos, qmc_sampl
  * beams are selected and their pages reordered.
  *
  * Common to all of them: pointers are device memory of the current device unless said otherwise, aligned to their
- * elements (a workspace: anyhow); rows are
- * `ld` elements apart (ld >= the row's elements) and a row's heads follow one another; `dtype` is the rows'
- * QMC_F32, QMC_F16 or QMC_BF16; sums, softmax statistics and norms are float (log-sum-exp of a vocabulary:
- * double) and every output is rounded once.  No call allocates or synchronises and each may be captured in a
- * CUDA graph; a workspace belongs to one call at a time (two calls, or two graphs, whose executions may
- * overlap need one each) and needs no initial contents.  Index errors that only the device can see (a
- * page outside the pool, a position past the page table) skip the access and set the device error word:
- * the next qmc_check_device_error() / qmc_sync() returns QMC_EINVAL.  Outputs must not overlap inputs, other
+ * elements (a workspace: anyhow); rows are `ld` elements apart (ld >= the row's elements) and a row's heads follow
+ * one another; `dtype` is the rows' QMC_F32, QMC_F16 or QMC_BF16; sums, softmax statistics and norms are float and
+ * every output is rounded once (what is rounded in between is said with the operator).  No call allocates or
+ * synchronises and each may be captured in a CUDA graph; a workspace belongs to one call at a time (two calls, or two
+ * graphs, whose executions may overlap need one each) and needs no initial contents.  Index errors that only the
+ * device can see (a page outside the pool, a position past the page table) skip the access and set the device error
+ * word: the next qmc_check_device_error() / qmc_sync() returns QMC_EINVAL.  Outputs must not overlap inputs, other
  * than where a call allows it. */
 
 /* rotary positions: pair i of the first rot_dim dimensions of a head turns by pos * f_i radians, with
- * f_i = theta^(-2 i / rot_dim) before scaling; the other dimensions stay.  Angles are formed in double, so
- * far positions lose nothing. */
+ * f_i = theta^(-2 i / rot_dim) before scaling; the other dimensions stay.  f_i is a double,
+ * kept as turns in 64-bit fixed point, whose product with the position loses whole turns only; the angle is then off by
+ * 2^-32 turns or a float's half step, whichever is more, at any position, and cos and sin are floats. */
 enum { QMC_ROPE_INTERLEAVED = 0 /* pair (2i, 2i + 1), as qmc_rope */, QMC_ROPE_HALF = 1 /* pair (i, i + rot_dim / 2) */ };
 enum {
     QMC_ROPE_PLAIN = 0,
@@ -246,7 +246,7 @@ enum {
                             s = (t - low) / (high - low) */
     QMC_ROPE_YARN = 3,   /* f_i / factor r + f_i (1 - r) with r rising from 0 to 1 between the pair indices
                             floor(d(high)) and ceil(d(low)), d(t) = rot_dim ln(orig_ctx / (2 pi t)) / (2 ln theta),
-                            clamped to [0, rot_dim - 1]; cos and sin times 0.1 ln(factor) + 1, for factors up to 1 as they are */
+                            clamped to [0, rot_dim - 1]; cos and sin times 0.1 ln(factor) + 1 where factor > 1 */
 };
 typedef struct {
     int32_t head_dim, rot_dim; /* even; 2 <= rot_dim <= head_dim <= 256 */
@@ -296,9 +296,17 @@ int qmc_kv_append_paged(const qmc_rope_plan *plan, const qmc_paged_cache *cache,
  * entries for whole prefix pages are not read; prefix_len may end inside a page).  seq_lens[b] counts
  * the prefix too: it is 0 (an empty row: zeros) or at least prefix_len; any other value, a length past
  * ld_table * page_size, or a page outside the pool sets the error word, and then the rows concerned are undefined (but
- * written).  scale is not negative, and scale log2(e) and the scaled scores are finite floats; n_heads is a multiple of the cache's n_kv_heads (head h reads kv
- * head h / (n_heads / n_kv_heads)), head_dim <= 256, ld_table * page_size < 2^31 - 1024.  Types (rows, cache): (F32, F32), (F32, F16), (F16, F16), (BF16, BF16).  Keys and values
- * at positions that are read must be finite; what lies in slots past a sequence's end does not matter. */
+ * written).  scale is not negative, and scale log2(e) and the scaled scores are finite floats; n_heads is a multiple of
+ * the cache's n_kv_heads (head h reads kv head h / (n_heads / n_kv_heads)), head_dim <= 256, ld_table * page_size <
+ * 2^31 - 1024.  Types (rows, cache): (F32, F32), (F32, F16), (F16, F16), (BF16, BF16).  Keys and values at positions
+ * that are read must be finite; what lies in slots past a sequence's end does not matter.
+ * Over caches of 16 bits the softmax weights may be rounded to the cache's type for their product with the values, by
+ * half a step each, which their float sum is not; in fp16 that holds down to 2^-12 of the largest weight of its 16 to
+ * 128 neighbours, and smaller ones are off by half a step of that.  With float rows queries and weights go in two such
+ * halves.
+ * The workspace's size goes by the cache's sizes, types and alignment of its pools as well as by the numbers given: ask
+ * with the cache of the call.  The work is split for sequences that may fill the table: one much wider than the
+ * sequences are long costs time and workspace. */
 int qmc_attn_prefix_workspace(int dtype, const qmc_paged_cache *cache, int32_t n_seq, int32_t n_heads,
                               int32_t prefix_len, int32_t ld_table, size_t *bytes);
 int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, const void *q, int64_t ldq, void *out,
@@ -312,7 +320,9 @@ int qmc_attn_prefix(const qmc_paged_cache *cache, int32_t layer, int dtype, cons
  * [n_prompts][n_out].  logits is [n_prompts * beams][ld].  A finished beam (finished[row] != 0; NULL: none)
  * offers one continuation, eos_token at its score unchanged; all its others, those of a beam whose score is
  * -inf or NaN, and tokens whose logit is -inf or NaN, score -inf.  Where a row holds +inf, its infinities share the
- * probability.  beams <= 64, n_out <= min(64, beams * n_vocab). */
+ * probability.  Scores are not +inf.  The exponentials are floats, summed in float within a thread and in double
+ * beyond, one float for each 4096 or 8192 logits: the log-sum-exp is off by up to 2^-18, so of beams whose exact scores
+ * lie closer than that either may come first.  beams <= 64, n_out <= min(64, beams * n_vocab). */
 int qmc_beam_workspace(int32_t n_prompts, int32_t beams, int32_t n_vocab, int32_t n_out, size_t *bytes);
 int qmc_beam_select(int dtype, const void *logits, int64_t ld, int32_t n_prompts, int32_t beams, int32_t n_vocab,
                     const float *scores, const uint8_t *finished, int32_t eos_token, int32_t n_out, int32_t *parents,
