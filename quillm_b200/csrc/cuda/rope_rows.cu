@@ -75,9 +75,9 @@ __device__ __forceinline__ int spread(int t, int e) {
 // (a, b) of a pair through its row of the table, times the head's factor.  A pair that stays keeps its elements apart: a product with
 // the other's zero would be NaN for an infinite one
 __device__ __forceinline__ void rotate(float &a, float &b, float4 r, float f, bool turns) {
-    const float u = a, v = b;
-    a = (turns ? u * r.x - v * r.y : u * r.x) * f;
-    b = (turns ? u * r.z + v * r.w : v * r.w) * f;
+    const float u = a, v = b, u0 = turns ? u : 0.0f, v0 = turns ? v : 0.0f;
+    a = (u * r.x - v0 * r.y) * f;
+    b = (u0 * r.z + v * r.w) * f;
 }
 
 // T rows, CT cache elements, C elements per chunk, NIT items per lane, R rows a block: their elements are all on their way before
