@@ -227,10 +227,11 @@ int qmc_model_forward_sample(qmc_model *m, int32_t token, int32_t pos, qmc_sampl
  * elements (a workspace: anyhow); rows are `ld` elements apart (ld >= the row's elements) and a row's heads follow
  * one another; `dtype` is the rows' QMC_F32, QMC_F16 or QMC_BF16; sums, softmax statistics and norms are float and
  * every output is rounded once (what is rounded in between is said with the operator).  No call allocates or
- * synchronises and each may be captured in a CUDA graph; a workspace belongs to one call at a time (two calls, or two
- * graphs, whose executions may overlap need one each) and needs no initial contents.  Index errors that only the
- * device can see (a page outside the pool, a position past the page table) skip the access and set the device error
- * word: the next qmc_check_device_error() / qmc_sync() returns QMC_EINVAL.  Outputs must not overlap inputs, other
+ * synchronises and each may be captured in a CUDA graph, once any call of the library has been made on the device
+ * before; a workspace belongs to one call at a time (two calls, or two graphs, whose executions may overlap need one
+ * each) and needs no initial contents.  Index errors that only the device can see (a page outside the pool, a position
+ * past the page table) skip the access and set the device error word: the next qmc_check_device_error() / qmc_sync()
+ * returns QMC_EINVAL.  Outputs must not overlap inputs, other
  * than where a call allows it. */
 
 /* rotary positions: pair i of the first rot_dim dimensions of a head turns by pos * f_i radians, with

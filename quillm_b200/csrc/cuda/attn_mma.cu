@@ -7,8 +7,8 @@
 // and accumulators are joined through shared memory at the end.  Rows of K, V and Q lie in shared memory with 16-byte
 // chunk c of row r at c ^ (r & 7): the eight rows of one matrix load hit distinct banks.
 //
-// Bound by the matrix instructions' issue and the loads from shared memory between them (512 rows over 32768 positions: 334 us, 206
-// TFLOP/s; float rows, of twice the products each way, 447 us), with few rows by the copies (32 rows 46 us, 2.9 TB/s).  Its cases are
+// Bound by the matrix instructions' issue and the loads from shared memory between them (512 rows over 32768 positions: 311 us, 221
+// TFLOP/s; float rows, of twice the products each way, 474 us), with few rows by the copies (32 rows 45 us, 3.0 TB/s).  Its cases are
 // those that the faster two cannot take: pages that are no multiple of 8, float rows in number, heads above 128.
 //
 // Weights are rounded to the cache's type for the second product: bf16 by half a step each at most, as the outputs are, fp16 likewise down to

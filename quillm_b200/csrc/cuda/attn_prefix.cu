@@ -7,15 +7,16 @@
 // head), shared by the group's heads.  Each job leaves its rows' running maximum m, sum l and unnormalised o in the workspace, and
 // a last launch joins the parts of every row: o = sum_j e^(m_j - M) o_j / sum_j e^(m_j - M) l_j.
 //
-// Kernels of the jobs, by what they measured (us; 8 KV heads of 128, fp16, 32768 shared positions, floor 20.5, unless stated):
+// Kernels of the jobs, by what they measured alone with cold caches (us; 8 KV heads of 128, fp16, 32768 shared positions, floor
+// 20.5, unless stated):
 //   attn_tc    more than 16 rows per KV head, rows of the cache's 16-bit type, head_dim <= 128, pages of a multiple of 8:
-//              32 rows 30.4, 64 30.5, 128 32.3, 512 (two tiles of 256) 83
-//   attn_warp  up to 16 rows and all own positions, 16-bit caches, head_dim <= 128: 16 rows 30.5, and 64 sequences of <= 1024
-//              own positions 39 (floor 21)
-//   attn_mma   the other 16-bit caches of whole 16-byte chunks: pages of 20, 32 rows 46, 64 57, 512 334; float rows 512 447
-//   attn_vec   float caches of whole 16-byte chunks: 128 rows over 2048 positions 80, one row of 32 heads over 4096 28 (floor 20.5)
-//   this file  what is left, any head_dim up to 256 and any alignment: fp16 heads of 100, 128 rows over 2048 positions 124, float
-//              heads of 50, 8 rows of 32 heads over 1024 32
+//              32 rows 30.5, 64 32.5, 128 32.9, 256 48, 512 (two tiles of 256) 77
+//   attn_warp  up to 16 rows and all own positions, 16-bit caches, head_dim <= 128: 16 rows 31, and 64 sequences of <= 1024
+//              own positions 41 (floor 21)
+//   attn_mma   the other 16-bit caches of whole 16-byte chunks: pages of 20, 32 rows 45, 64 54, 512 311; float rows 512 474
+//   attn_vec   float caches of whole 16-byte chunks: 128 rows over 2048 positions 81, one row of 32 heads over 4096 28 (floor 20.5)
+//   this file  what is left, any head_dim up to 256 and any alignment: fp16 heads of 100, 128 rows over 2048 positions 125, float
+//              heads of 50, 8 rows of 32 heads over 1024 33
 // Where two of them serve a call, they run beside each other: prefix blocks first, own jobs on the SMs that they leave.
 #include <algorithm>
 #include <cmath>
@@ -43,7 +44,7 @@ constexpr int kPT = 32;  // positions per staged tile (one per lane)
 // The general kernel, in float on the CUDA cores: any head_dim up to 256, any types, strides and alignments.  Per row and tile of
 // 32 positions lane p scores position p, the warp updates the row's maximum and sum once, and each lane
 // accumulates four of the head's dimensions (eight above 128).  Bound by the shared-memory reads of both products: 8 rows of 32
-// heads of 50 over 1024 positions 32 us.
+// heads of 50 over 1024 positions 33 us.
 template <typename T, typename CT, int NG>
 __global__ void __launch_bounds__(128) attn_rows_kernel(const AttnArgs a, bool vec) {
     extern __shared__ __align__(16) float smf[];
@@ -156,7 +157,7 @@ constexpr int kMostSplits = 64;
 // Joins the parts of a row, W warps each: a warp takes the factors 2^(m_j - M) of all parts, a lane each, and sums every W-th
 // part over the row's dimensions, V (once, twice above 128, as often as needed one by one) a lane, with loads that do not
 // wait for one another.  Bound by latency: the lengths, the statistics, the parts and the warps' sums follow on one another
-// (128 rows 2.9 us, 1024 rows of 9 parts 5 us).
+// (with cold caches 30 to 128 rows 4.5 to 5.3 us, 1024 rows of 9 parts 6.3 us).
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, int parts) {
     constexpr int NV = 256 / 32 / V, NB = 2 * kMostSplits / 32;

@@ -152,14 +152,14 @@ int attn_mma_tile(int rows);  // query rows of a prefix job, for `rows` of them 
 int launch_attn_mma(const AttnArgs &a, int dtype, int cdt, bool after, cudaStream_t s);
 
 // up to 16 rows a tile, straight from global memory into the matrix instructions (attn_warp.cu): such caches with head_dim <= 128.  Up
-// to 16 rows it is ahead of the tensor-core kernel (whole calls over 8192 shared positions of 8 heads: 8 rows 18.6 and 20.3 us, 16
-// rows 20.8 and 20.5), with more it reads them again (24 rows 24.6 and 20.6 us; over 32768 49 and 40)
+// to 16 rows it is ahead of the tensor-core kernel (whole calls over 8192 shared positions of 8 heads: 8 rows 18.5 and 20.3 us, 16
+// rows 20.5 both ways), with more it reads them again (24 rows 24.6 and 20.5 us; over 32768 49 and 38)
 constexpr int kWarpRows = 16;
 int launch_attn_warp(const AttnArgs &a, int dtype, int cdt, bool after, cudaStream_t s);
 
 // caches of floats, heads of whole 16-byte chunks (attn_vec.cu): tiles of 1, 4 or 8 rows, the smallest that takes the rows of a
-// group, and of the prefix if 8 do (4 rows of 8 heads over 4096 positions 18.6 us with tiles of 4, 32.2 with 1; 16 rows
-// 34.6 us with 8, 37.0 with 4)
+// group, and of the prefix if 8 do (4 rows of 8 heads over 4096 positions 18.5 us with tiles of 4, 28.9 with 1; 16 rows
+// 29.3 us with 8, 35.0 with 4)
 int attn_vec_tile(int rows);
 int launch_attn_vec(const AttnArgs &a, int tile, cudaStream_t s);
 

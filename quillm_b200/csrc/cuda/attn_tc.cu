@@ -14,9 +14,9 @@
 //
 // Bound by the chain of a stream, scores 500 cycles, weights 1300, product 500 and the waits between (3500 cycles for the two tiles
 // of PAIR, in which the tensor cores have 2050 to do), and before that by the start and the end of a block, 5 us together.
-// 256 rows of 8 heads over 32768 positions in 9 ranges: 72 us, 950 TFLOP/s of the measured 1613; beside own jobs, in 7: 83 us.  128
-// rows 32 us, 4.2 TB/s.  Tried and not kept: four threads a row (84 us), copies by threads instead of TMA (192 us), one
-// wait with a lane for each barrier (97 us against 83).
+// 512 rows of 8 heads over 32768 positions in 8 ranges: 77 us, 890 TFLOP/s of the measured 1613; beside own jobs, in 7: 84 us.  128
+// rows 33 us, 4.1 TB/s.  Tried and not kept, each against the 80 us or 83 us of its day: four threads a row (84 us), copies by threads
+// instead of TMA (192 us), one wait with a lane for each barrier (97 us).
 //
 // Warps 0-15: weights; 16: TMA; 17: one lane issues the MMAs.  A box is a run of rows within a page (the largest power of two that
 // divides the page size, 8 to 128 of them) and 64 dimensions wide, the 128-byte swizzle's row.  Dimensions past the head are the next
@@ -601,8 +601,8 @@ int launch_h(const AttnArgs &a, CUtensorMapDataType type, cudaStream_t s) {
 }  // namespace
 
 int attn_tc_box(int page_size) { return std::min(kN, page_size & -page_size); }
-// two row tiles a block above 128 rows (whole calls over 32768 positions of 8 heads: 136 rows 47.5 us, 53.4 with a tile each; 512 rows
-// 84 and 95; over 4096 positions they are even)
+// two row tiles a block above 128 rows (the calls of their day over 32768 positions of 8 heads: 136 rows 47.5 us, 53.4 with a tile
+// each; 512 rows 84 and 95; over 4096 positions they are even)
 int attn_tc_tile(int rows) { return rows > kM ? 2 * kM : kM; }
 
 int launch_attn_tc(const AttnArgs &a, int cdt, cudaStream_t s) {

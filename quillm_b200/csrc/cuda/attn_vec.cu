@@ -7,9 +7,9 @@
 // each on their way per lane while the group before is used; no shared memory, no barrier.  A row's accumulators are rescaled only
 // when a score passes its reference by more than 2^kLift.
 //
-// HBM bound with few rows: one row of 32 heads over 4096 positions 28 us (4.7 TB/s), 8 sequences of up to 4096 94 us (5.1 TB/s).  With
+// HBM bound with few rows: one row of 32 heads over 4096 positions 28 us (4.7 TB/s), 8 sequences of up to 4096 95 us (5.6 TB/s).  With
 // many rows each tile of 8 reads the prefix again, from L2, and the instructions bound it, about 14 a row and position: 128 rows of
-// 8 heads over 2048 positions 80 us (staged through shared memory, 16 rows a block, 174 us).  All sums of a step's rows are formed
+// 8 heads over 2048 positions 81 us (staged through shared memory, 16 rows a block, 174 us).  All sums of a step's rows are formed
 // side by side: row by row the shuffles' latency made that 155 us.
 #include "attn_prefix.cuh"
 

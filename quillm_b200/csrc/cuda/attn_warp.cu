@@ -1,9 +1,9 @@
 // Shared-prefix attention for up to 16 query rows per tile over caches of 16-bit elements: own positions (a group's heads) and the
 // prefix of a few sequences.  HBM bound: with so few rows the products cost little, so keys and values go from global memory
 // straight into the registers that the matrix instructions (m16n8k16, float accumulators) take, no shared memory, no barrier; the
-// group after the next is on its way to L2.  Measured: 4 rows of 32 heads over 32768 shared positions 85 us (6.3 TB/s), 16 rows of 8
-// heads 30.5 us (4.4 TB/s; short ranges), 64 sequences of up to 1024 own positions 39 us, 16 of up to 8192 67 us (without the
-// way to L2 80 us; through shared memory, two or three groups ahead, 87 us).
+// group after the next is on its way to L2.  Measured: 4 rows of 32 heads over 32768 shared positions 86 us (6.3 TB/s), 16 rows of 8
+// heads 31 us (4.4 TB/s; short ranges), 64 sequences of up to 1024 own positions 41 us with cold caches, 16 of up to 8192 65 us a call
+// (without the way to L2 it took 13 us more; through shared memory, two or three groups ahead, 20 us).
 //
 // Every warp of a block takes 16 positions at a time, every fourth group of the job's range.  Of the two operand layouts only the
 // dimensions' order is free, and that is enough: with g = lane / 4 and t = lane % 4,

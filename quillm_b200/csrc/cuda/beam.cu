@@ -4,17 +4,18 @@
 // Selection in two launches.  Both the log-sum-exp and the order need every logit once, so the first reads each row
 // once, a chunk per block held in registers: the chunk's maximum m and sum of exp(x - m), and its n best logits.
 // Within a row the order of scores is the order of logits, so n per chunk suffice whatever the row's log-sum-exp
-// turns out to be.  The second, one block per prompt, joins a row's (m, sum) pairs in double and takes the n best of the rows'
-// sorted lists.
+// turns out to be.  The second, one block per prompt, joins a row's (m, sum) pairs and takes the n best of the rows' sorted lists.
+// Exponentials are floats (2^-22), summed in float within a thread and in double over the block; a chunk's sum is stored as a float, and the
+// chunks are added in double.
 //
 // The n best of a chunk: with w warps, the smallest of the warps' ceil(n / w)-th largest thread maxima is a lower bound T that at
 // least n elements reach, found in a few warp-wide maxima (in the 32-bit order-preserving form); the few elements >= T are
 // collected in shared memory and ranked by counting, with the index, so that ties go to the lower one.  Where too many reach T
 // (equal logits), the exact n-th largest of the threads' maxima is built from the top bit, and its bits continued over the indices, after
 // which at most n threads' elements remain.  Blocks stay and take chunk after chunk, the next one's logits on their way to registers.
-// Measured: 24 x 8 rows of 128000 bf16 logits 34 us (1.4 TB/s: the barriers and the warp-wide steps of a chunk bind it, three blocks
-// an SM; spans of chunks with a running bound took longer), with two of eight beams ended 26.5 us (31.5 us before the live rows
-// were listed), 4 rows of 32000 floats 4.2 us; the merge 10 and 5 us; the reordering 15 us for 67 MB (4.5 TB/s) and 6 us.
+// Measured with cold caches: 24 x 8 rows of 128000 bf16 logits, two of eight beams ended, 26.7 us (1.4 TB/s: the barriers and the
+// warp-wide steps of a chunk bind it, three blocks an SM; spans of chunks with a running bound took longer, as did all rows in turn without
+// a list of the live ones), 4 rows of 32000 floats 5.4 us; the merge 9.7 and 6.5 us; the reordering 14.4 us for 67 MB (4.7 TB/s) and 6.7 us.
 // Of the lists' heads, whose beams' scores lie apart, the exact n-th largest is taken at once; where too many reach it, n rounds of a
 // block-wide maximum over the heads.
 #include <algorithm>

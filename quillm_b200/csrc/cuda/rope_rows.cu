@@ -4,13 +4,15 @@
 // For every head x of a row:  y = x / sqrt(mean(x^2) + eps) * w  (optional), then each pair (a, b) of the first
 // rot dimensions becomes (a c - b s, a s + b c) with (c, s) = m (cos, sin)(pos f_i).  The angle is formed in turns in fixed point:
 // f_i / 2 pi is kept as a fraction of 2^64, and pos times it modulo 2^64 is the fraction of a turn, off by pos times the double's
-// rounding of f_i (2^-36 turns at position 10^6, where a float angle would be off by a sixteenth of a radian); its upper half,
-// rounded to float, goes to sincospi.
+// rounding of f_i (2^-36 turns at position 10^6, where a float angle would be off by a sixteenth of a radian); its upper half
+// (2^-32 turns), rounded to float, goes to sincospi.
 //
 // HBM bound: each element is read once and written once with ~10 operations between.  8192 rows of 64 + 8 heads of 128 in bf16, with
-// norms: 67 us, 4.5 TB/s of the measured 6.56, and 80 us with the append of keys and values; the issue of instructions binds
-// what is left (a block that stays and loops over rows: 115 us and more).  A token's call is the launch, 2.4 us.
-//  A lane group of 1 to 32 lanes
+// norms: 67 us, 4.5 TB/s of the measured 6.56, and 81 us with the append of keys and values; the issue of instructions binds
+// what is left (a block that stays and loops over rows: 115 us and more).  A token's kernel takes 2.4 us, 3.6 with cold caches, its
+// call from Python 6.6.
+//
+// A lane group of 1 to 32 lanes
 // holds one head, each lane two chunks of C elements (16 bytes each where the layout allows it) that hold whole
 // pairs between them: in the half layout the chunks at t C and t C + rot / 2, in the interleaved one neighbours.  So a
 // rotation needs no exchange, a norm log2(lanes) shuffles, and every access is a full vector.  While the elements are in flight the
