@@ -231,13 +231,12 @@ int qmc_model_forward_sample(qmc_model *m, int32_t token, int32_t pos, qmc_sampl
  * before; a workspace belongs to one call at a time (two calls, or two graphs, whose executions may overlap need one
  * each) and needs no initial contents.  Index errors that only the device can see (a page outside the pool, a position
  * past the page table) skip the access and set the device error word: the next qmc_check_device_error() / qmc_sync()
- * returns QMC_EINVAL.  Outputs must not overlap inputs, other
- * than where a call allows it. */
+ * returns QMC_EINVAL.  Outputs must not overlap inputs, other than where a call allows it. */
 
 /* rotary positions: pair i of the first rot_dim dimensions of a head turns by pos * f_i radians, with
  * f_i = theta^(-2 i / rot_dim) before scaling; the other dimensions stay.  f_i is a double,
- * kept as turns in 64-bit fixed point, whose product with the position loses whole turns only; the angle is then off by
- * 2^-32 turns or a float's half step, whichever is more, at any position, and cos and sin are floats. */
+ * kept as turns in 64-bit fixed point, whose product with the position loses whole turns only: the angle is off by the
+ * position times f_i's half step, and by 2^-32 turns or a float's half step, whichever is more.  cos and sin are floats. */
 enum { QMC_ROPE_INTERLEAVED = 0 /* pair (2i, 2i + 1), as qmc_rope */, QMC_ROPE_HALF = 1 /* pair (i, i + rot_dim / 2) */ };
 enum {
     QMC_ROPE_PLAIN = 0,
