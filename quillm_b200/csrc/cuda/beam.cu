@@ -329,7 +329,7 @@ __device__ __forceinline__ bool before(const Head &a, const Head &b) {
 constexpr int kMergeCap = 512;  // candidates that are ranked by counting
 
 __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
-    __shared__ double lse_s[kMaxOut], cum_s[kMaxOut];
+    __shared__ double lse_s[kMaxOut], cum_s[kMaxOut];  // lse: of the logits above the row's largest, top_s
     __shared__ float top_s[kMaxOut];
     __shared__ uint8_t kind_s[kMaxOut];  // 0 logits, 1 finished, 2 dead
     __shared__ Head buf[kMergeCap];
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
         if (lane == 0) {
             cum_s[b] = cum, top_s[b] = m;
             kind_s[b] = ended ? 1 : (dead || !(m > -INFINITY)) ? 2 : 0;
-            lse_s[b] = m == INFINITY ? log(s) : (double)m + log(s);
+            lse_s[b] = log(s);
         }
     }
     if (tid == 0) cnt_s = 0;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
         const float x = order_value((uint32_t)(key >> 32));
         h.at = (uint64_t)b << 32 | (uint32_t)~(uint32_t)key;
         if (top_s[b] == INFINITY) {
-            // lse is the log of the number of infinities, which come first.  All other tokens score -inf, so their order is the
+            // lse_s is the log of the number of infinities, which come first.  All other tokens score -inf, so their order is the
             // tokens', not the logits': chunk 0's list goes on with the lowest ones that are not infinite.  The first i of
             // these end below n_out, as do the infinities that they pass over, all of which are in the list
             if (x == INFINITY) {
@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
                 h.at = ~0ull;
             }
         } else {
-            h.score = cum_s[b] + ((double)x - lse_s[b]);
+            // rows that differ by a constant have the same scores to the last bit, since x - m loses nothing
+            h.score = cum_s[b] + (((double)x - (double)top_s[b]) - lse_s[b]);
         }
         if (h.score != h.score) h.score = -INFINITY;
         return h;

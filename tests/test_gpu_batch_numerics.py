@@ -284,3 +284,35 @@ def test_attn_repeats_its_bits(cuda_dev, dtype, cdt):
         do_attn(c, 0, dtype, q, o, heads, 0.09, pp, prefix, table, lens)
     clean()
     assert all(torch.equal(o.view(torch.int16), outs[0].view(torch.int16)) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_beam_select_ties_of_shifted_rows(cuda_dev, dtype):
+    """rows of logits that differ by a constant have the same scores: the lower beam's come first"""
+    prompts, beams, vocab, n_out = 40, 6, 9, 20
+    g = gen(41)
+    x = torch.randint(-4, 5, (prompts, 1, vocab), generator=g, device="cuda") + torch.randint(-30, 30, (prompts, beams, 1), generator=g, device="cuda")
+    x = x.to(DT[dtype]).view(prompts * beams, vocab).contiguous()
+    scores = torch.randint(-9, 0, (prompts, 1), generator=g, device="cuda").float().expand(-1, beams).reshape(-1).contiguous()
+    par, tok, sc = do_select(dtype, x, vocab, prompts, beams, scores, None, 0, n_out)
+    clean()
+    # ordered by the logit above that of the row's first token, then by beam, then by token
+    rel = (x.view(prompts, beams, vocab) - x.view(prompts, beams, vocab)[:, :, :1]).float().cpu().numpy().reshape(prompts, -1)
+    at = np.argsort(-rel, axis=1, kind="stable")[:, :n_out]
+    assert np.array_equal(par.cpu().numpy(), at // vocab) and np.array_equal(tok.cpu().numpy(), at % vocab)
+    check_select((par, tok, sc), (at // vocab, at % vocab, ref_select(f64(x), f64(scores), None, 0, n_out, prompts, beams)[2]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_beam_select_rows_of_the_lowest_value(cuda_dev, dtype):
+    """a mask of the type's lowest value over a whole row leaves every token the same share, 1 / vocab, not all of it"""
+    prompts, beams, vocab, n_out, g = 2, 2, 9000, 8, gen(43)
+    x = rand(g, (prompts * beams, vocab), dtype, 3.0)
+    x[1] = x[2] = x[3] = torch.finfo(DT[dtype]).min
+    scores = -torch.rand(prompts * beams, generator=g, device="cuda")
+    par, tok, sc = do_select(dtype, x, vocab, prompts, beams, scores, None, 0, n_out)
+    clean()
+    want = scores.double()[:, None] + torch.log_softmax(x.double() - x.double().amax(1, keepdim=True), 1)
+    want, at = torch.sort(want.view(prompts, -1), dim=1, descending=True, stable=True)
+    want, at = want[:, :n_out].cpu().numpy(), at[:, :n_out].cpu().numpy()
+    check_select((par, tok, sc), (at // vocab, at % vocab, want))
