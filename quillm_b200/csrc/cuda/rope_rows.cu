@@ -10,7 +10,7 @@
 // HBM bound: each element is read once and written once with ~10 operations between.  8192 rows of 64 + 8 heads of 128 in bf16, with
 // norms: 67 us, 4.5 TB/s of the measured 6.56, and 81 us with the append of keys and values; the issue of instructions binds
 // what is left (a block that stays and loops over rows: 115 us and more).  A token's kernel takes 2.4 us, 3.6 with cold caches, its
-// call from Python 6.6.
+// call from Python 6.8.
 //
 // A lane group of 1 to 32 lanes
 // holds one head, each lane two chunks of C elements (16 bytes each where the layout allows it) that hold whole
