@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kBT) beam_merge_kernel(const SelArgs a) {
                 h.at = ~0ull;
             }
         } else {
-            // rows that differ by a constant have the same scores to the last bit, since x - m loses nothing
+            // the distance first: a large logit would round the logarithm away, and rows that differ by a constant are to tie
             h.score = cum_s[b] + (((double)x - (double)top_s[b]) - lse_s[b]);
         }
         if (h.score != h.score) h.score = -INFINITY;

@@ -303,6 +303,20 @@ def test_beam_select_ties_of_shifted_rows(cuda_dev, dtype):
     check_select((par, tok, sc), (at // vocab, at % vocab, ref_select(f64(x), f64(scores), None, 0, n_out, prompts, beams)[2]))
 
 
+def best(x, scores, n_out, prompts, beams):
+    """parents, tokens and scores in 64 bits, from the distances to a row's largest logit; x [rows, vocab], no NaN"""
+    sc = np.full(x.shape, -np.inf)
+    for r in range(x.shape[0]):
+        m = x[r].max()
+        if scores[r] > -np.inf and np.isfinite(m):
+            sc[r] = scores[r] + ((x[r] - m) - np.log(np.exp(x[r] - m).sum()))
+        elif scores[r] > -np.inf and m > 0:
+            sc[r] = np.where(x[r] == np.inf, scores[r] - np.log((x[r] == np.inf).sum()), -np.inf)
+    flat = sc.reshape(prompts, -1)
+    at = np.argsort(-flat, axis=1, kind="stable")[:, :n_out]
+    return at // x.shape[1], at % x.shape[1], np.take_along_axis(flat, at, 1)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_beam_select_rows_of_the_lowest_value(cuda_dev, dtype):
     """a mask of the type's lowest value over a whole row leaves every token the same share, 1 / vocab, not all of it"""
@@ -310,9 +324,35 @@ def test_beam_select_rows_of_the_lowest_value(cuda_dev, dtype):
     x = rand(g, (prompts * beams, vocab), dtype, 3.0)
     x[1] = x[2] = x[3] = torch.finfo(DT[dtype]).min
     scores = -torch.rand(prompts * beams, generator=g, device="cuda")
-    par, tok, sc = do_select(dtype, x, vocab, prompts, beams, scores, None, 0, n_out)
+    got = do_select(dtype, x, vocab, prompts, beams, scores, None, 0, n_out)
     clean()
-    want = scores.double()[:, None] + torch.log_softmax(x.double() - x.double().amax(1, keepdim=True), 1)
-    want, at = torch.sort(want.view(prompts, -1), dim=1, descending=True, stable=True)
-    want, at = want[:, :n_out].cpu().numpy(), at[:, :n_out].cpu().numpy()
-    check_select((par, tok, sc), (at // vocab, at % vocab, want))
+    check_select(got, best(f64(x), f64(scores), n_out, prompts, beams))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_beam_select_masked_rows_together(cuda_dev, dtype):
+    """equal rows, masks of -inf and of the lowest value, NaN, infinities, dead beams and the first step in one call"""
+    prompts, beams, vocab, g = 6, 4, 9000, gen(47)
+    low = torch.finfo(DT[dtype]).min
+    x = rand(g, (prompts * beams, vocab), dtype, 3.0)
+    scores = -torch.rand(prompts * beams, generator=g, device="cuda") * 5
+    x[0:4] = 1.5
+    x[4] = -math.inf
+    x[5, 1:] = -math.inf
+    x[6, 7000:] = low
+    x[7] = low
+    x[8:12, ::2] = math.nan
+    x[9] = math.nan
+    x[10, 5] = math.inf
+    x[11, 5] = x[11, 8000] = math.inf
+    scores[12:16] = -math.inf
+    scores[17:20] = -math.inf
+    scores[18] = math.nan
+    x[20:24] = x[20].clone()
+    scores[20:24] = -1.0
+    x[20:24, 11] = 0.0
+    x[22, 11] = -0.0
+    for n_out in (1, 4, 8, 64):
+        got = do_select(dtype, x, vocab, prompts, beams, scores, None, 0, n_out)
+        clean()
+        check_select(got, best(np.nan_to_num(f64(x), nan=-np.inf, posinf=np.inf, neginf=-np.inf), f64(scores), n_out, prompts, beams))
